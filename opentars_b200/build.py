@@ -41,7 +41,7 @@ def sources() -> list[Path]:
 def _needs(obj: Path, src: Path) -> bool:
     if not obj.exists():
         return True
-    deps = [src, *CSRC.glob("*.h"), *CSRC.glob("*.cuh"), ROOT / "include" / "tarscuda.h"]
+    deps = [src, *CSRC.glob("*.h"), *CSRC.glob("*.cuh"), *(ROOT / "include").glob("*.h")]
     t = obj.stat().st_mtime
     return any(d.stat().st_mtime > t for d in deps if d.exists())
 

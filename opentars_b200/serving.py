@@ -1,0 +1,379 @@
+"""Serving operators over a paged key-value cache (include/tarscuda_serve.h), on torch CUDA tensors.
+
+    cache = PagedCache.empty(n_pages, page_size, n_kv, head_dim, batch, max_pages, track=True)
+    cache.table[b, :n] = pages                        # the caller hands out the pages
+    cache.length.add_(n_new); cache.seen.add_(n_new)  # a step's tokens count before it appends them
+    append(cache, k, v, cu)                           # the new rows into the pages
+    o = attend_prompt(cache, q, cu, scale)            # the tokens of a prompt, or of a chunk of one
+    o = attend(cache, q, scale, weight_out=cache.weight)   # one token per sequence
+    evict(cache, budget, sinks=4, recent=256)         # back to the budget by accumulated weight
+    token = adjust_logits(logits, history=ids, repetition=r, mask=grammar)
+
+Work is enqueued on torch's current stream of the tensors' device and can be captured into a CUDA
+graph. Wrong arguments raise ValueError before anything is enqueued; what only the device can see
+(a page id outside the pool, a length beyond the page list) is left out and recorded, and
+`device_error` reads it. Only forward passes: the framework trains nothing.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ._lib import TC_ERR_ARG
+from ._lib import lib as _machine_lib
+
+P = ctypes.c_void_p
+I32, I64 = ctypes.c_int32, ctypes.c_int64
+FP32, BF16, FP16 = 0, 1, 3
+DTYPES = {torch.float32: FP32, torch.bfloat16: BF16, torch.float16: FP16}
+PAGE_SIZES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 128, 256)
+
+
+class Cache_t(ctypes.Structure):
+    _fields_ = [("k", P), ("v", P), ("page_stride", I64), ("slot_stride", I64), ("head_stride", I64),
+                ("n_pages", I32), ("page_size", I32), ("n_kv", I32), ("head_dim", I32), ("dtype", I32),
+                ("batch", I32), ("max_pages", I32), ("table", P), ("table_stride", I64), ("length", P),
+                ("weight", P), ("pos", P), ("track_stride", I64), ("seen", P)]
+
+
+class Rules_t(ctypes.Structure):
+    _fields_ = [("logits", P), ("out", P), ("logits_stride", I64), ("out_stride", I64), ("rows", I32), ("vocab", I32),
+                ("history", P), ("history_stride", I64), ("max_history", I32), ("n_history", P), ("n_prompt", P),
+                ("repetition", P), ("presence", P), ("frequency", P), ("bias_ids", P), ("bias", P),
+                ("bias_stride", I64), ("n_bias", I32), ("mask", P), ("mask_stride", I64), ("token", P), ("none", I32)]
+
+
+_C, _R = ctypes.POINTER(Cache_t), ctypes.POINTER(Rules_t)
+SERVE_SIGNATURES = {
+    "tc_kv_append": (ctypes.c_int, [_C, P, P, I32, I64, I64, P, I32, P]),
+    "tc_attend": (ctypes.c_int, [_C, P, I64, I64, P, I64, I64, I32, ctypes.c_float, I32, I32, P, P, ctypes.c_uint64,
+                                 P]),
+    "tc_attend_workspace": (ctypes.c_uint64, [_C, I32, I32]),
+    "tc_attend_prompt": (ctypes.c_int, [_C, P, I64, I64, P, I64, I64, I32, P, I32, ctypes.c_float, I32, I32, P]),
+    "tc_kv_evict": (ctypes.c_int, [_C, I32, I32, I32, P, P, P, P, ctypes.c_uint64, P]),
+    "tc_kv_evict_workspace": (ctypes.c_uint64, [_C, I32]),
+    "tc_adjust_logits": (ctypes.c_int, [_R, P]),
+}
+
+
+def lib():
+    L = _machine_lib()
+    if not getattr(L, "_serve_bound", False):
+        for name, (res, args) in SERVE_SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.restype, fn.argtypes = res, args
+        L._serve_bound = True
+    return L
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _check(rc: int, what: str) -> None:
+    if rc == TC_ERR_ARG:
+        raise ValueError(f"{what}: an argument is out of range or not 16-byte aligned")
+    if rc != 0:
+        raise RuntimeError(f"{what} failed ({rc})")
+
+
+def _ints(t: torch.Tensor, shape: tuple, device: torch.device, name: str) -> None:
+    _need(t.dtype == torch.int32 and tuple(t.shape) == shape and t.device == device and t.is_contiguous(),
+          f"{name}: a contiguous int32 tensor of shape {shape} on {device} is wanted")
+
+
+class _On:
+    """The device of a call's tensors current, and its current stream's handle."""
+
+    def __init__(self, device: torch.device):
+        self.device = device
+
+    def __enter__(self) -> int:
+        self.was = torch.cuda.current_device()
+        if self.was != self.device.index:
+            torch.cuda.set_device(self.device)
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        if self.was != self.device.index:
+            torch.cuda.set_device(self.was)
+
+
+def _stride(t: torch.Tensor, d: int) -> int:
+    """A dimension's stride; one of a single entry is never stepped over and may be anything."""
+    return t.stride(d) if t.shape[d] > 1 else 0
+
+
+def _apart(t: torch.Tensor) -> bool:
+    """Whether the rows of t [rows, heads, dim] lie apart in memory, in either order."""
+    width = t.shape[2]
+    for stride, n in sorted((t.stride(d), t.shape[d]) for d in (0, 1) if t.shape[d] > 1):
+        if stride < width:
+            return False
+        width = stride * n
+    return True
+
+
+class PagedCache:
+    """Pools, page lists and lengths of `batch` sequences: a handle over the caller's tensors.
+
+    k, v      [n_pages, page_size, n_kv, head_dim] bf16 or fp16, the last dimension contiguous, equal
+              strides (a permuted view of another order is fine; [page, kv head, slot, dim] in memory
+              reads fastest)
+    table     [batch, max_pages] int32 page ids; entries behind a sequence's length are not read
+    length    [batch] int32 slots in use
+    weight, pos, seen   what eviction needs, all or none: [batch, n_kv, slots] fp32 attention weight and
+              int32 position of each slot (slots >= max_pages * page_size), [batch] int32 tokens taken
+
+    The tensors are fixed for the handle's life; their contents are the caller's to change.
+    """
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, length: torch.Tensor,
+                 weight: torch.Tensor | None = None, pos: torch.Tensor | None = None,
+                 seen: torch.Tensor | None = None):
+        _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype and
+              k.device == v.device, "k and v: two pools of one shape, type and stride")
+        _need(k.dtype in (torch.bfloat16, torch.float16), f"the pools are bf16 or fp16, not {k.dtype}")
+        _need(k.is_cuda, "the pools must be on a CUDA device")
+        n_pages, page, n_kv, hd = k.shape
+        _need(page in PAGE_SIZES, f"page size {page}: one of {PAGE_SIZES}")
+        _need(hd in HEAD_DIMS, f"head dim {hd}: one of {HEAD_DIMS}")
+        _need(k.stride(3) == 1, "a row's head_dim elements must be contiguous")
+        strides = [_stride(k, d) for d in range(3)]
+        _need(all(s % 8 == 0 for s in strides) and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0,
+              "the pools' rows must be 16-byte aligned")
+        _need(table.dim() == 2 and table.dtype == torch.int32 and table.device == k.device and table.shape[0] >= 1
+              and table.shape[1] >= 1 and (table.stride(1) == 1 or table.shape[1] == 1) and
+              (table.stride(0) >= table.shape[1] or table.shape[0] == 1), "table: int32 [batch, max_pages] on the pools' device")
+        batch, max_pages = table.shape
+        _ints(length, (batch,), k.device, "length")
+        track = [t is not None for t in (weight, pos, seen)]
+        _need(all(track) or not any(track), "weight, pos and seen come together")
+        if weight is not None:
+            _need(weight.dim() == 3 and tuple(weight.shape[:2]) == (batch, n_kv) and
+                  weight.shape[2] >= max_pages * page and weight.dtype == torch.float32 and weight.is_contiguous() and
+                  weight.device == k.device, "weight: contiguous fp32 [batch, n_kv, slots of the page list]")
+            _ints(pos, tuple(weight.shape), k.device, "pos")
+            _ints(seen, (batch,), k.device, "seen")
+        self._t = (k, v, table, length, weight, pos, seen)
+        self.device, self.dtype = k.device, k.dtype
+        self.n_pages, self.page_size, self.n_kv, self.head_dim = n_pages, page, n_kv, hd
+        self.batch, self.max_pages = batch, max_pages
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self.desc = Cache_t(k.data_ptr(), v.data_ptr(), *strides, n_pages, page, n_kv, hd,
+                            DTYPES[k.dtype], batch, max_pages, table.data_ptr(), max(_stride(table, 0), max_pages),
+                            length.data_ptr(), ptr(weight), ptr(pos), 0 if weight is None else weight.shape[2],
+                            ptr(seen))
+        self.ref = ctypes.byref(self.desc)
+
+    k = property(lambda self: self._t[0])
+    v = property(lambda self: self._t[1])
+    table = property(lambda self: self._t[2])
+    length = property(lambda self: self._t[3])
+    weight = property(lambda self: self._t[4])
+    pos = property(lambda self: self._t[5])
+    seen = property(lambda self: self._t[6])
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, n_kv: int, head_dim: int, batch: int, max_pages: int,
+              dtype: torch.dtype = torch.bfloat16, track: bool = False, device=None) -> "PagedCache":
+        """A cache of empty sequences; the pools lie in memory as [page, kv head, slot, dim]."""
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        pool = lambda: torch.empty(n_pages, n_kv, page_size, head_dim, dtype=dtype,  # noqa: E731
+                                   device=device).permute(0, 2, 1, 3)
+        ints = lambda *s: torch.zeros(*s, dtype=torch.int32, device=device)  # noqa: E731
+        more = {}
+        if track:
+            cap = max_pages * page_size
+            more = dict(weight=torch.zeros(batch, n_kv, cap, device=device), pos=ints(batch, n_kv, cap), seen=ints(batch))
+        return cls(pool(), pool(), ints(batch, max_pages), ints(batch), **more)
+
+
+def _rows(t: torch.Tensor, cache: PagedCache, heads: int | None, name: str) -> None:
+    _need(t.dim() == 3 and t.shape[2] == cache.head_dim and (heads is None or t.shape[1] == heads) and
+          t.device == cache.device and t.stride(2) == 1, f"{name}: [rows, heads, {cache.head_dim}] on {cache.device}")
+
+
+def _cu(cu: torch.Tensor, cache: PagedCache) -> int:
+    _ints(cu, (cache.batch + 1,), cache.device, "cu")
+    return cu.data_ptr()
+
+
+def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor | None = None) -> None:
+    """The new tokens' rows [tokens, n_kv, head_dim] (fp32, bf16 or fp16) into the cache, rounded to its
+    type. Sequence b owns rows cu[b] .. cu[b+1]-1 (cu None: row b), counted in length and seen already."""
+    _rows(k, cache, cache.n_kv, "k")
+    _need(k.dtype in DTYPES and v.dtype == k.dtype and v.shape == k.shape and v.stride() == k.stride() and
+          v.device == k.device, "k and v: rows of one shape, type (fp32, bf16 or fp16) and stride")
+    _need(cu is not None or k.shape[0] <= cache.batch, "without cu there is one row per sequence")
+    cu_p = None if cu is None else _cu(cu, cache)
+    if k.shape[0] == 0:
+        return
+    with _On(cache.device) as stream:
+        _check(lib().tc_kv_append(cache.ref, k.data_ptr(), v.data_ptr(), DTYPES[k.dtype], _stride(k, 0), _stride(k, 1),
+                                  cu_p, k.shape[0], stream), "append")
+
+
+def _attend_args(cache: PagedCache, q: torch.Tensor, out: torch.Tensor | None, window: int, sinks: int) -> torch.Tensor:
+    _rows(q, cache, None, "q")
+    _need(q.dtype == cache.dtype, f"q has the cache's type {cache.dtype}, not {q.dtype}")
+    _need(q.shape[1] >= 1 and q.shape[1] % cache.n_kv == 0, f"{q.shape[1]} heads over {cache.n_kv} key-value heads")
+    _need(window >= 0 and sinks >= 0, "window and sinks are not negative")
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _rows(out, cache, q.shape[1], "out")
+    _need(out.dtype == q.dtype and out.shape == q.shape and _apart(out), "out has q's shape and type, its rows apart")
+    return out
+
+
+def attend(cache: PagedCache, q: torch.Tensor, scale: float, window: int = 0, sinks: int = 0,
+           out: torch.Tensor | None = None, weight_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one query row per sequence, q [batch, heads, head_dim], over its slots: those of the
+    last `window` (0: all) and the first `sinks`. weight_out (cache.weight, or a tensor like it)
+    receives cache.weight plus the attention weight each slot draws. Length 0 gives zeros."""
+    out = _attend_args(cache, q, out, window, sinks)
+    _need(q.shape[0] == cache.batch, f"{q.shape[0]} query rows for {cache.batch} sequences")
+    w = None
+    if weight_out is not None:
+        _need(cache.weight is not None, "the cache keeps no weights")
+        _need(weight_out.dtype == torch.float32 and weight_out.shape == cache.weight.shape and
+              weight_out.is_contiguous() and weight_out.device == cache.device, "weight_out is laid out as cache.weight")
+        w = weight_out.data_ptr()
+    L = lib()
+    with _On(cache.device) as stream:
+        n = L.tc_attend_workspace(cache.ref, q.shape[1], w is not None)
+        ws = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
+        _check(L.tc_attend(cache.ref, q.data_ptr(), _stride(q, 0), _stride(q, 1), out.data_ptr(),
+                           _stride(out, 0), _stride(out, 1), q.shape[1], scale, window, sinks, w, None if ws is None else ws.data_ptr(), n,
+                           stream), "attend")
+    return out
+
+
+def attend_prompt(cache: PagedCache, q: torch.Tensor, cu: torch.Tensor, scale: float, window: int = 0, sinks: int = 0,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the last tokens of each sequence, rows cu[b] .. cu[b+1]-1 of q [tokens, heads,
+    head_dim] for sequence b, each over the slots up to its own position, of the last `window` (0: all)
+    and the first `sinks`. Rows at and behind cu[batch] are left alone."""
+    out = _attend_args(cache, q, out, window, sinks)
+    cu_p = _cu(cu, cache)
+    if q.shape[0] == 0:
+        return out
+    with _On(cache.device) as stream:
+        _check(lib().tc_attend_prompt(cache.ref, q.data_ptr(), _stride(q, 0), _stride(q, 1), out.data_ptr(),
+                                      _stride(out, 0), _stride(out, 1), q.shape[1], cu_p, q.shape[0], scale, window, sinks, stream),
+               "attend_prompt")
+    return out
+
+
+def evict(cache: PagedCache, budget: int, sinks: int = 0, recent: int = 0, length_out: torch.Tensor | None = None,
+          weight_out: torch.Tensor | None = None, pos_out: torch.Tensor | None = None) -> None:
+    """Cuts every sequence longer than `budget` to it, per key-value head: the first `sinks` and the last
+    `recent` positions stay, then the slots of largest weight. Kept slots behind the budget move into
+    the holes before it. The new lengths, weights and positions go to the *_out tensors (None: the
+    cache's own)."""
+    _need(cache.weight is not None, "the cache keeps no weights")
+    _need(budget >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= budget, "0 <= sinks + recent <= budget")
+    length_out = cache.length if length_out is None else length_out
+    weight_out = cache.weight if weight_out is None else weight_out
+    pos_out = cache.pos if pos_out is None else pos_out
+    _ints(length_out, (cache.batch,), cache.device, "length_out")
+    _ints(pos_out, tuple(cache.pos.shape), cache.device, "pos_out")
+    _need(weight_out.dtype == torch.float32 and weight_out.shape == cache.weight.shape and weight_out.is_contiguous()
+          and weight_out.device == cache.device, "weight_out is laid out as cache.weight")
+    L = lib()
+    with _On(cache.device) as stream:
+        n = L.tc_kv_evict_workspace(cache.ref, budget)
+        ws = torch.empty(n, dtype=torch.uint8, device=cache.device)
+        _check(L.tc_kv_evict(cache.ref, budget, sinks, recent, length_out.data_ptr(), weight_out.data_ptr(),
+                             pos_out.data_ptr(), ws.data_ptr(), n, stream), "evict")
+
+
+def _per_row(t: torch.Tensor | None, dtype: torch.dtype, rows: int, device: torch.device, name: str) -> int | None:
+    if t is None:
+        return None
+    _need(t.dtype == dtype and tuple(t.shape) == (rows,) and t.device == device and t.is_contiguous(),
+          f"{name}: {dtype} [{rows}] on {device}")
+    return t.data_ptr()
+
+
+def rules_of(logits: torch.Tensor, out: torch.Tensor | None = None, history: torch.Tensor | None = None,
+             n_history: torch.Tensor | None = None, n_prompt: torch.Tensor | None = None,
+             repetition: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+             frequency: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
+             bias: torch.Tensor | None = None, mask: torch.Tensor | None = None, token: torch.Tensor | None = None,
+             none: int = -1) -> Rules_t:
+    """The checked C description of adjust_logits' arguments."""
+    out = logits if out is None else out
+    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.is_cuda and logits.stride(1) == 1 and
+          logits.shape[0] >= 1 and logits.shape[1] >= 1, "logits: fp32 [rows, vocab] on a CUDA device")
+    _need(out.dtype == torch.float32 and out.shape == logits.shape and out.device == logits.device and
+          out.stride(1) == 1, "out has the logits' shape, type and device")
+    rows, vocab = logits.shape
+    dev = logits.device
+    r = Rules_t()
+
+    def wide(t: torch.Tensor) -> int:
+        """A matrix' row stride; rows must not overlap (a single row's stride may be anything)."""
+        _need(t.shape[0] == 1 or t.stride(0) >= t.shape[1], "rows of logits, history, biases and masks lie apart")
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    r.logits, r.out, r.rows, r.vocab, r.none = logits.data_ptr(), out.data_ptr(), rows, vocab, none
+    r.logits_stride, r.out_stride = wide(logits), wide(out)
+    if history is not None and history.numel() == 0:
+        _need(tuple(history.shape) == (rows, 0), "history: int32 [rows, ids]")
+        history = n_history = n_prompt = repetition = presence = frequency = None
+    if history is not None:
+        _need(history.dim() == 2 and history.shape[0] == rows and history.dtype == torch.int32 and
+              history.device == dev and (history.stride(1) == 1 or history.shape[1] <= 1), "history: int32 [rows, ids]")
+        r.history, r.history_stride, r.max_history = history.data_ptr(), wide(history), history.shape[1]
+    else:
+        _need(all(t is None for t in (n_history, n_prompt, repetition, presence, frequency)),
+              "the penalties need the history")
+    r.n_history = _per_row(n_history, torch.int32, rows, dev, "n_history")
+    r.n_prompt = _per_row(n_prompt, torch.int32, rows, dev, "n_prompt")
+    r.repetition = _per_row(repetition, torch.float32, rows, dev, "repetition")
+    r.presence = _per_row(presence, torch.float32, rows, dev, "presence")
+    r.frequency = _per_row(frequency, torch.float32, rows, dev, "frequency")
+    _need((bias is None) == (bias_ids is None), "bias and bias_ids come together")
+    if bias is not None and bias.numel() == 0 == bias_ids.numel():
+        bias = bias_ids = None
+    if bias is not None:
+        _need(bias_ids.dim() == 2 and bias_ids.shape[0] == rows and bias_ids.dtype == torch.int32 and
+              bias.dtype == torch.float32 and bias.shape == bias_ids.shape and bias.stride() == bias_ids.stride() and
+              bias.device == dev and bias_ids.device == dev and (bias.stride(1) == 1 or bias.shape[1] <= 1),
+              "bias_ids int32 and bias fp32, [rows, entries]")
+        r.bias_ids, r.bias, r.bias_stride, r.n_bias = bias_ids.data_ptr(), bias.data_ptr(), wide(bias), bias.shape[1]
+    if mask is not None:
+        words = (vocab + 31) // 32
+        _need(mask.dtype == torch.int32 and mask.device == dev and mask.dim() in (1, 2) and mask.shape[-1] == words and
+              mask.stride(-1) == 1 and (mask.dim() == 1 or mask.shape[0] == rows),
+              f"mask: int32 [rows, {words}], or [{words}] for all rows")
+        r.mask, r.mask_stride = mask.data_ptr(), 0 if mask.dim() == 1 else wide(mask)
+    if token is not None:
+        r.token = _per_row(token, torch.int32, rows, dev, "token")
+    return r
+
+
+def adjust_logits(logits: torch.Tensor, token: torch.Tensor | None = None, none: int = -1, **rules) -> torch.Tensor:
+    """Penalties, biases and a grammar mask on fp32 logits [rows, vocab], and the greedy pick: the picks
+    [rows] int32 (`token`, or a new tensor). Keywords, each optional: out (None: in place), history
+    [rows, ids] int32 with n_history and n_prompt [rows] (prompt ids first), repetition / presence /
+    frequency [rows] fp32, bias_ids / bias [rows, entries] (the last entry of a token counts), mask
+    int32 words, bit t % 32 of word t // 32 set where token t is allowed. A row whose mask allows
+    nothing picks `none`."""
+    if token is None:
+        token = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
+    r = rules_of(logits, token=token, none=none, **rules)
+    with _On(logits.device) as stream:
+        _check(lib().tc_adjust_logits(ctypes.byref(r), stream), "adjust_logits")
+    return token
+
+
+def device_error(clear: bool = False) -> int:
+    """The first error the current device has recorded (0: none): 51 append, 52 attend, 53
+    attend_prompt, 54 evict - a page id outside the pool or a length beyond the page list -, 55 and 56
+    a bounded wait that gave up. Waits for the device."""
+    return _machine_lib().tc_wait_error(int(clear))

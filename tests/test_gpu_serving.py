@@ -1,0 +1,723 @@
+"""The serving operators on the GPU against their 64-bit definitions (tests/serving_ref.py).
+
+Every cache is poisoned: pages nobody owns, rows behind a sequence's length and entries behind its page
+list hold NaN and ids outside the pool, so a read past the end shows. Tolerances of an attention output,
+with u half a step of the output's type and vmax the largest |v|: u |ref| for the stored rounding, u vmax
+for probabilities rounded to the type before they meet the values (sum of p is 1), and for fp16 half its
+smallest step per key; the scores' fp32 sums may be off by hd steps of sum |q k| scale, which moves each
+probability by twice that."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from tests import serving_ref as R
+
+pytestmark = pytest.mark.gpu
+NAN = float("nan")
+
+
+def _pools(lens, n_kv, hd, page, dtype, g, order="pages", spare=3):
+    """CPU pools [pages, page, n_kv, hd] poisoned outside the sequences' slots, and a shuffled table."""
+    need = [-(-n // page) for n in lens]
+    total, width = sum(need) + spare, max(1, max(need)) + 1
+    perm = torch.randperm(total, generator=g)
+    table = torch.full((len(lens), width), 10 ** 9, dtype=torch.int32)
+    k = torch.full((total, page, n_kv, hd), NAN, dtype=dtype)
+    v = torch.full_like(k, NAN)
+    at = 0
+    for b, n in enumerate(lens):
+        table[b, :need[b]] = perm[at:at + need[b]].int()
+        at += need[b]
+        slot = torch.arange(n)
+        pages = table[b].long()[slot // page]
+        k[pages, slot % page] = torch.randn(n, n_kv, hd, generator=g).to(dtype)
+        v[pages, slot % page] = torch.randn(n, n_kv, hd, generator=g).to(dtype)
+    return k, v, table
+
+
+def _cuda_pool(x, order):
+    """On the GPU with heads outside slots ("heads") or the plain order ("slots")."""
+    if order == "heads":
+        return x.permute(0, 2, 1, 3).contiguous().cuda().permute(0, 2, 1, 3)
+    return x.cuda()
+
+
+def _cache(k, v, table, lens, order="heads", track=None):
+    from opentars_b200 import serving as S
+    length = torch.tensor(lens, dtype=torch.int32).cuda()
+    more = {} if track is None else dict(weight=track[0].cuda(), pos=track[1].cuda(), seen=track[2].cuda())
+    return S.PagedCache(_cuda_pool(k, order), _cuda_pool(v, order), table.cuda(), length, **more)
+
+
+def _finite(x):
+    return torch.nan_to_num(x.float(), 0, 0, 0).abs()
+
+
+def _tolerance(ref, q, k, v, scale, dtype):
+    u = torch.finfo(dtype).eps / 2
+    vmax = float(_finite(v).max()) if v.numel() else 0.0
+    hd = q.shape[-1]
+    smax = abs(scale) * hd * float(_finite(q).max()) * float(_finite(k).max())
+    slots = k.shape[0] * k.shape[1]
+    tiny = slots * 2.0 ** -25 if dtype == torch.float16 else 0.0
+    return u * ref.abs() + (u + tiny + 2 * hd * 2.0 ** -23 * smax / 8 + 2.0 ** -18) * vmax
+
+
+def _close(got, ref, tol, what=""):
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)), f"{what}: NaN where there is none, or none where one is"
+    bad = (got - ref).abs() > tol
+    bad &= ~torch.isnan(ref)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {(got - ref).abs()[bad].max()}"
+
+
+def _no_error():
+    from opentars_b200 import serving as S
+    torch.cuda.synchronize()
+    assert S.device_error(clear=True) == 0
+
+
+# dtype, head dim, page, kv heads, group, lengths, window, sinks, pool order
+ATTEND = [
+    (torch.bfloat16, 128, 16, 2, 2, [1, 0, 37, 300], 0, 0, "heads"),
+    (torch.float16, 64, 32, 3, 1, [64, 65, 63, 1, 0], 0, 0, "slots"),
+    (torch.bfloat16, 256, 64, 1, 4, [513, 128, 700], 512, 4, "heads"),
+    (torch.float16, 128, 16, 2, 7, [1000, 17, 16, 15], 100, 1, "slots"),
+    (torch.bfloat16, 64, 128, 1, 16, [257], 0, 0, "heads"),
+    (torch.bfloat16, 128, 256, 1, 33, [400, 2], 64, 30, "heads"),
+    (torch.float16, 256, 16, 2, 3, [130, 5], 1, 0, "slots"),
+    (torch.bfloat16, 128, 32, 8, 2, [2500] + [3] * 20, 0, 0, "heads"),
+    (torch.float16, 64, 16, 1, 8, [9000], 0, 0, "heads"),
+    (torch.bfloat16, 128, 16, 1, 2, [4000, 90], 2 ** 31 - 1, 2 ** 31 - 1, "slots"),
+    (torch.float16, 128, 64, 2, 2, [600, 700], 40, 5000, "heads"),
+]
+
+
+@pytest.mark.parametrize("case", ATTEND, ids=lambda c: f"{c[0]}-{c[1]}-p{c[2]}-{c[3]}x{c[4]}-{max(c[5])}-w{c[6]}-s{c[7]}")
+@pytest.mark.parametrize("weights", [False, True], ids=["", "weights"])
+def test_attend(case, weights):
+    from opentars_b200 import serving as S
+    dtype, hd, page, kv, G, lens, window, sinks, order = case
+    g = torch.Generator().manual_seed(sum(lens) + hd)
+    k, v, table = _pools(lens, kv, hd, page, dtype, g)
+    q = torch.randn(len(lens), kv * G, hd, generator=g).to(dtype)
+    scale = hd ** -0.5
+    track = None
+    cap = table.shape[1] * page + 5
+    if weights:
+        w0 = torch.rand(len(lens), kv, cap, generator=g)
+        track = (w0, torch.zeros(len(lens), kv, cap, dtype=torch.int32), torch.tensor(lens, dtype=torch.int32))
+    cache = _cache(k, v, table, lens, order, track)
+    ref, prob = R.attend(k, v, table, lens, q, scale, window, sinks, page)
+    w_out = torch.full((len(lens), kv, cap), 7.0, device="cuda") if weights else None
+    out = S.attend(cache, q.cuda(), scale, window=window, sinks=sinks, weight_out=w_out)
+    _no_error()
+    _close(out, ref, _tolerance(ref, q, k, v, scale, dtype), "out")
+    if weights:
+        smax = scale * hd * float(_finite(q).max()) * float(_finite(k).max())
+        for b, n in enumerate(lens):
+            got = w_out[b].cpu().double()
+            want = w0[b, :, :n].double() + prob[b]
+            tol = 2.0 ** -23 * want + prob[b] * (2 * hd * 2.0 ** -23 * smax / 8 + 2.0 ** -18) + 1e-30
+            assert ((got[:, :n] - want).abs() <= tol).all(), b
+            assert (got[:, n:] == 7.0).all()                     # slots behind the length are left alone
+        acc = cache.weight.clone()
+        S.attend(cache, q.cuda(), scale, window=window, sinks=sinks, weight_out=cache.weight)   # in place
+        for b, n in enumerate(lens):
+            assert torch.equal(cache.weight[b, :, :n], w_out[b, :, :n])
+            assert torch.equal(cache.weight[b, :, n:], acc[b, :, n:])
+
+
+def test_attend_leaves_hidden_slots_out():
+    """NaN and infinities in slots that the window hides do not reach the output or the weights."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(5)
+    lens, kv, hd, page, window, sinks = [333, 90], 2, 128, 16, 50, 3
+    k, v, table = _pools(lens, kv, hd, page, torch.bfloat16, g)
+    for b, n in enumerate(lens):
+        for s in range(sinks, n - window):
+            p = int(table[b, s // page])
+            k[p, s % page], v[p, s % page] = (NAN, math.inf) if s % 2 else (-math.inf, NAN)
+    q = torch.randn(2, 4, hd, generator=g).bfloat16()
+    cap = table.shape[1] * page
+    cache = _cache(k, v, table, lens, "heads", (torch.zeros(2, kv, cap), torch.zeros(2, kv, cap, dtype=torch.int32),
+                                                torch.tensor(lens, dtype=torch.int32)))
+    ref, prob = R.attend(k, v, table, lens, q, 0.1, window, sinks, page)
+    out = S.attend(cache, q.cuda(), 0.1, window=window, sinks=sinks, weight_out=cache.weight)
+    _no_error()
+    _close(out, ref, _tolerance(ref, q, k[:, :, :, :], v, 0.1, torch.bfloat16))
+    for b, n in enumerate(lens):
+        assert (cache.weight[b, :, sinks:n - window] == 0).all()
+        assert torch.isfinite(cache.weight[b]).all()
+
+
+def test_attend_takes_strided_rows_and_visible_nonfinite_values():
+    """q and out as slices of wider rows; a visible NaN or infinity gives what the formula gives."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(6)
+    lens, kv, hd, page = [40, 40, 40, 40], 2, 64, 32
+    k, v, table = _pools(lens, kv, hd, page, torch.float16, g)
+    v[int(table[1, 0]), 3, 0, 5] = math.inf                    # one element of one head's value
+    v[int(table[2, 0]), 3, 1, 7] = NAN
+    k[int(table[3, 0]), 3, 0] = NAN                            # a whole key: every output of the head is NaN
+    wide = torch.randn(4, 10, 2 * hd, generator=g).half()
+    q = wide[:, 2:6, hd:]
+    cache = _cache(k, v, table, lens)
+    ref, _ = R.attend(k, v, table, lens, q, 0.125, 0, 0, page)
+    dev = torch.zeros(4, 8, hd, dtype=torch.float16, device="cuda")
+    out = S.attend(cache, wide.cuda()[:, 2:6, hd:], 0.125, out=dev[:, ::2])
+    _no_error()
+    assert out.data_ptr() == dev.data_ptr() and (dev[:, 1::2] == 0).all()
+    assert math.isinf(float(ref[1, 0, 5])) and torch.isnan(ref[2, 2:, 7]).all() and torch.isnan(ref[3, :2]).all()
+    assert torch.equal(torch.isinf(out.cpu()), torch.isinf(ref.float()))
+    inf = torch.isinf(ref)
+    tol = _tolerance(torch.where(inf, 0.0, ref), q, k, v, 0.125, torch.float16)
+    _close(torch.where(inf.cuda(), 0.0, out.float()), torch.where(inf, 0.0, ref), tol)
+
+
+# dtype, head dim, page, kv heads, group, (cached, new) per sequence, window, sinks, order
+PROMPT = [
+    (torch.bfloat16, 128, 16, 1, 2, [(0, 1), (0, 300), (5, 0), (77, 40)], 0, 0, "heads"),
+    (torch.float16, 64, 32, 2, 1, [(0, 129), (128, 128), (1, 127)], 0, 0, "slots"),
+    (torch.bfloat16, 256, 64, 1, 4, [(100, 200), (0, 70)], 64, 4, "heads"),
+    (torch.float16, 256, 16, 1, 2, [(0, 150)], 0, 0, "slots"),
+    (torch.float16, 128, 16, 2, 7, [(33, 50), (0, 20)], 30, 1, "slots"),
+    (torch.bfloat16, 64, 128, 1, 16, [(0, 90), (1000, 3)], 0, 0, "heads"),
+    (torch.bfloat16, 128, 256, 1, 3, [(300, 260)], 1, 0, "heads"),
+    (torch.bfloat16, 128, 16, 2, 1, [(0, 1)] * 9, 0, 0, "heads"),
+    (torch.float16, 64, 16, 1, 33, [(3, 21)], 10, 2, "slots"),
+    (torch.bfloat16, 128, 64, 1, 4, [(700, 170)], 2 ** 31 - 1, 2 ** 31 - 1, "heads"),
+    (torch.bfloat16, 128, 32, 1, 2, [(2000, 4), (10, 4), (0, 4)], 300, 40, "slots"),
+]
+
+
+def _rows(case, extra, g):
+    dtype, hd, page, kv, G, seqs, window, sinks, order = case
+    cu = [0]
+    for _, n in seqs:
+        cu.append(cu[-1] + n)
+    q = torch.randn(cu[-1] + extra, kv * G, hd, generator=g).to(dtype)
+    return q, torch.tensor(cu, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("case", PROMPT, ids=lambda c: f"{c[0]}-{c[1]}-p{c[2]}-{c[3]}x{c[4]}-{c[5][0]}-w{c[6]}-s{c[7]}")
+def test_attend_prompt(case):
+    from opentars_b200 import serving as S
+    dtype, hd, page, kv, G, seqs, window, sinks, order = case
+    g = torch.Generator().manual_seed(hd + len(seqs))
+    lens = [c + n for c, n in seqs]
+    k, v, table = _pools(lens, kv, hd, page, dtype, g)
+    q, cu = _rows(case, 3, g)
+    cache = _cache(k, v, table, lens, order)
+    scale = hd ** -0.5
+    ref = R.attend_prompt(k, v, table, lens, q, cu, scale, window, sinks, page)
+    out = torch.full(q.shape, 9.0, dtype=dtype, device="cuda")
+    S.attend_prompt(cache, q.cuda(), cu.cuda(), scale, window=window, sinks=sinks, out=out)
+    _no_error()
+    n = int(cu[-1])
+    assert (out[n:] == 9.0).all()                              # rows behind the last sequence are left alone
+    _close(out[:n], ref[:n], _tolerance(ref[:n], q, k, v, scale, dtype))
+
+
+def test_attend_prompt_keeps_later_tokens_out():
+    """NaN and infinities in a later token's key and value do not reach the rows before it."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(8)
+    lens, hd, page = [200], 128, 16
+    k, v, table = _pools(lens, 1, hd, page, torch.bfloat16, g)
+    for s, (kk, vv) in {60: (NAN, 1.0), 90: (1.0, NAN), 91: (1.0, math.inf), 150: (-math.inf, NAN)}.items():
+        k[int(table[0, s // page]), s % page] = kk
+        v[int(table[0, s // page]), s % page] = vv
+    q = torch.randn(200, 2, hd, generator=g).bfloat16()
+    cu = torch.tensor([0, 200], dtype=torch.int32)
+    ref = R.attend_prompt(k, v, table, lens, q, cu, 0.09, 20, 0, page)
+    out = S.attend_prompt(_cache(k, v, table, lens), q.cuda(), cu.cuda(), 0.09, window=20)
+    _no_error()
+    assert torch.isfinite(ref[:60]).all() and torch.isfinite(ref[80:90]).all() and torch.isfinite(ref[170:]).all()
+    assert torch.isnan(ref[60]).all()
+    _close(out, ref, _tolerance(ref, q, k, v, 0.09, torch.bfloat16))
+
+
+def test_attend_prompt_rows_at_negative_positions_get_zeros():
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(9)
+    k, v, table = _pools([5], 1, 64, 16, torch.bfloat16, g)
+    q = torch.randn(9, 1, 64, generator=g).bfloat16()
+    cu = torch.tensor([0, 9], dtype=torch.int32)
+    out = S.attend_prompt(_cache(k, v, table, [5]), q.cuda(), cu.cuda(), 0.125)
+    _no_error()
+    assert (out[:4] == 0).all() and (out[4:] != 0).any()
+    ref = R.attend_prompt(k, v, table, [5], q, cu, 0.125, 0, 0, 16)
+    _close(out, ref, _tolerance(ref, q, k, v, 0.125, torch.bfloat16))
+
+
+@pytest.mark.parametrize("op", ["attend", "prompt"])
+def test_bad_pages_and_lengths_are_left_out_and_recorded(op):
+    """Ids outside the pool inside the used slots, and a length beyond the page list: the kernels check
+    every id against the pool and clamp the length before they read."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(10)
+    lens, hd, page = [100, 70, 64], 128, 16
+    k, v, table = _pools(lens, 2, hd, page, torch.bfloat16, g)
+    table[0, 2], table[1, 4], table[1, 0] = -1, k.shape[0], 2 ** 31 - 1
+    q = torch.randn(3, 4, hd, generator=g).bfloat16()
+    cache = _cache(k, v, table, lens)
+    if op == "attend":
+        out, code = S.attend(cache, q.cuda(), 0.09), 52
+        ref, _ = R.attend(k, v, table, lens, q, 0.09, 0, 0, page)
+    else:
+        cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32)
+        out, code = S.attend_prompt(cache, q.cuda(), cu.cuda(), 0.09), 53
+        ref = R.attend_prompt(k, v, table, lens, q, cu, 0.09, 0, 0, page)
+    torch.cuda.synchronize()
+    assert S.device_error(clear=True) == code and S.device_error() == 0
+    _close(out, ref, _tolerance(ref, q, k, v, 0.09, torch.bfloat16))
+    table[2, 4] = int(table[2, 3])                             # all pages of sequence 2's list are real now
+    cache = _cache(k, v, table[2:, :5].contiguous(), [10 ** 6])
+    ref_len = [80]
+    if op == "attend":
+        out = S.attend(cache, q[2:].cuda(), 0.09, window=16)
+    else:
+        out = S.attend_prompt(cache, q[2:].cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda(), 0.09, window=16)
+    torch.cuda.synchronize()
+    assert S.device_error(clear=True) == code
+    if op == "attend":
+        ref, _ = R.attend(k, v, table[2:, :5], ref_len, q[2:], 0.09, 16, 0, page)
+        _close(out, ref, _tolerance(ref, q, k, v, 0.09, torch.bfloat16))
+
+
+def test_attend_offsets_past_32_bits():
+    """A pool of more than 2^32 elements: rows in its last pages are found."""
+    from opentars_b200 import serving as S
+    n_pages, page, hd = (1 << 32) // (256 * 256) + 40, 256, 256
+    k = torch.zeros(n_pages, page, 1, hd, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    g = torch.Generator().manual_seed(11)
+    lens = [300]
+    table = torch.tensor([[n_pages - 1, n_pages - 30]], dtype=torch.int32)
+    for i, p in enumerate(table[0].tolist()):
+        k[p] = torch.randn(page, 1, hd, generator=g).bfloat16().cuda()
+        v[p] = torch.randn(page, 1, hd, generator=g).bfloat16().cuda()
+    cache = S.PagedCache(k, v, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    q = torch.randn(1, 2, hd, generator=g).bfloat16()
+    small = torch.tensor([[0, 1]], dtype=torch.int32)
+    ks, vs = k[table[0].long().cuda()].cpu(), v[table[0].long().cuda()].cpu()
+    ref, _ = R.attend(ks, vs, small, lens, q, 0.06, 0, 0, page)
+    tol = _tolerance(ref, q, ks, vs, 0.06, torch.bfloat16)
+    _close(S.attend(cache, q.cuda(), 0.06), ref, tol)
+    cu = torch.tensor([0, 1], dtype=torch.int32).cuda()
+    _close(S.attend_prompt(cache, q.cuda(), cu, 0.06), ref, tol)
+    S.append(cache, torch.ones(1, 1, hd, device="cuda"), torch.full((1, 1, hd), 2.0, device="cuda"))
+    _no_error()
+    assert (k[n_pages - 30, 43, 0] == 1).all() and (v[n_pages - 30, 43, 0] == 2).all()
+
+
+# ------------------------------------------------------------------------------------------ append
+@pytest.mark.parametrize("src", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype,hd,page,kv,seqs", [
+    (torch.bfloat16, 128, 16, 2, [(0, 5), (16, 0), (15, 2), (3, 40)]),
+    (torch.float16, 64, 32, 3, [(31, 1), (0, 33)]),
+    (torch.bfloat16, 256, 256, 1, [(200, 100)])])
+def test_append(src, dtype, hd, page, kv, seqs):
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(hd)
+    lens = [c + n for c, n in seqs]
+    k, v, table = _pools(lens, kv, hd, page, dtype, g)
+    cap = table.shape[1] * page
+    track = (torch.full((len(lens), kv, cap), 3.0), torch.full((len(lens), kv, cap), -5, dtype=torch.int32),
+             torch.tensor([n + 100 for n in lens], dtype=torch.int32))
+    cache = _cache(k, v, table, lens, "heads", track)
+    cu = [0]
+    for _, n in seqs:
+        cu.append(cu[-1] + n)
+    kn = (torch.randn(cu[-1] + 2, kv, hd, generator=g) * 3).to(src)      # two rows behind the last sequence
+    vn = (torch.randn(cu[-1] + 2, kv, hd, generator=g) * 3).to(src)
+    S.append(cache, kn.cuda(), vn.cuda(), torch.tensor(cu, dtype=torch.int32).cuda())
+    _no_error()
+    w, p = track[0].clone(), track[1].clone()
+    for b, (c, n) in enumerate(seqs):
+        for i in range(n):
+            s = c + i
+            k[int(table[b, s // page]), s % page] = kn[cu[b] + i].to(dtype)
+            v[int(table[b, s // page]), s % page] = vn[cu[b] + i].to(dtype)
+            w[b, :, s], p[b, :, s] = 0.0, s + 100
+    same = lambda a, b: torch.equal(a.cpu().view(torch.int16), b.view(torch.int16))  # noqa: E731
+    assert same(cache.k.contiguous(), k) and same(cache.v.contiguous(), v)
+    assert torch.equal(cache.weight.cpu(), w) and torch.equal(cache.pos.cpu(), p)
+
+
+def test_append_one_row_each_skips_empty_sequences_and_bad_pages():
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(1)
+    k, v, table = _pools([17, 0, 16, 5], 1, 64, 16, torch.bfloat16, g)
+    table[3, 0] = -7
+    cache = _cache(k, v, table, [17, 0, 16, 5])
+    rows = torch.randn(4, 2, 64, generator=g).cuda()
+    S.append(cache, rows[:, :1], rows[:, 1:])
+    torch.cuda.synchronize()
+    assert S.device_error(clear=True) == 51
+    k[int(table[0, 1]), 0], v[int(table[0, 1]), 0] = rows[0, :1].cpu().bfloat16(), rows[0, 1:].cpu().bfloat16()
+    k[int(table[2, 0]), 15], v[int(table[2, 0]), 15] = rows[2, :1].cpu().bfloat16(), rows[2, 1:].cpu().bfloat16()
+    assert torch.equal(cache.k.cpu().view(torch.int16), k.view(torch.int16))
+    assert torch.equal(cache.v.cpu().view(torch.int16), v.view(torch.int16))
+
+
+# ------------------------------------------------------------------------------------------- evict
+EVICT = [  # head dim, page, kv heads, lengths, budget, sinks, recent, kind of weights
+    (128, 16, 2, [33, 32, 5, 0, 100], 32, 4, 8, "plain"),
+    (64, 32, 3, [40, 41], 1, 0, 0, "plain"),
+    (256, 16, 1, [130], 129, 0, 129, "plain"),
+    (128, 64, 2, [3000, 2049], 2048, 4, 500, "ties"),
+    (64, 16, 1, [500, 480], 100, 60, 40, "ties"),
+    (128, 16, 2, [700, 300], 64, 2, 10, "nonfinite"),
+    (64, 16, 1, [70000], 3000, 4, 100, "ties"),
+    (64, 256, 2, [5000], 4999, 0, 0, "zeros"),
+]
+
+
+def _weights(kind, shape, g):
+    w = torch.exp(2 * torch.randn(shape, generator=g))
+    if kind == "ties":
+        w = torch.randint(0, 6, shape, generator=g).float() - 1
+    if kind == "zeros":
+        w = torch.zeros(shape)
+        w[..., ::3] = -0.0
+    if kind == "nonfinite":
+        r = torch.rand(shape, generator=g)
+        w = torch.where(r < 0.01, torch.tensor(NAN), w)
+        w = torch.where((r > 0.01) & (r < 0.03), torch.tensor(math.inf), w)
+        w = torch.where((r > 0.03) & (r < 0.5), torch.tensor(-math.inf), w)
+        w = torch.where((r > 0.5) & (r < 0.6), torch.tensor(1e-42), w)
+    return w
+
+
+@pytest.mark.parametrize("case", EVICT, ids=lambda c: f"{c[0]}-{max(c[3])}to{c[4]}-{c[7]}")
+@pytest.mark.parametrize("inplace", [True, False], ids=["inplace", "out"])
+def test_evict(case, inplace):
+    from opentars_b200 import serving as S
+    hd, page, kv, lens, budget, sinks, recent, kind = case
+    g = torch.Generator().manual_seed(budget)
+    k, v, table = _pools(lens, kv, hd, page, torch.bfloat16, g)
+    B, cap = len(lens), table.shape[1] * page + 3
+    w = _weights(kind, (B, kv, cap), g)
+    # a history of evictions: positions are not the slots, and differ between heads
+    pos = torch.stack([torch.stack([torch.randperm(cap, generator=g) for _ in range(kv)]) for _ in range(B)]).int()
+    seen = torch.full((B,), cap, dtype=torch.int32)
+    cache = _cache(k, v, table, lens, "heads", (w, pos, seen))
+    lo, wo, po = cache.length, cache.weight, cache.pos
+    if not inplace:
+        lo, wo, po = torch.full_like(lo, -1), torch.full_like(wo, 5.0), torch.full_like(po, -9)
+    want = R.evict(w, pos, lens, seen, budget, sinks, recent)
+    S.evict(cache, budget, sinks=sinks, recent=recent, length_out=lo, weight_out=wo, pos_out=po)
+    _no_error()
+    assert lo.tolist() == [min(n, budget) for n in lens]
+    if not inplace:
+        assert cache.length.tolist() == lens
+    bits = lambda t: t.view(torch.int32)  # noqa: E731
+    for b in range(B):
+        slot = torch.arange(lens[b])
+        pages, rows = table[b].long()[slot // page], slot % page
+        for h in range(kv):
+            old = torch.tensor(want[b * kv + h], dtype=torch.long)
+            n = len(old)
+            assert torch.equal(bits(wo[b, h, :n].cpu()), bits(w[b, h, old])), (b, h)
+            assert torch.equal(po[b, h, :n].cpu(), pos[b, h, old])
+            if not inplace:
+                assert (wo[b, h, n:] == 5.0).all() and (po[b, h, n:] == -9).all()
+            for pool, was in ((cache.k, k), (cache.v, v)):
+                now = pool[pages.cuda(), rows.cuda(), h].cpu().view(torch.int16)
+                src = torch.cat([old, torch.arange(n, lens[b])])
+                assert torch.equal(now, was[pages[src], rows[src], h].view(torch.int16))
+
+
+def test_evict_skips_rows_on_bad_pages():
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(3)
+    lens, page, hd = [64], 16, 64
+    k, v, table = _pools(lens, 1, hd, page, torch.bfloat16, g)
+    cap = table.shape[1] * page
+    w = torch.arange(cap).float().reshape(1, 1, cap)           # the last slots stay and move to the front
+    pos = torch.arange(cap, dtype=torch.int32).reshape(1, 1, cap)
+    bad = int(table[0, 2])
+    table[0, 2] = -1
+    cache = _cache(k, v, table, lens, "heads", (w, pos, torch.tensor(lens, dtype=torch.int32)))
+    S.evict(cache, 32)
+    torch.cuda.synchronize()
+    assert S.device_error(clear=True) == 54
+    p = table[0].tolist()
+    assert torch.equal(cache.k[p[0]].cpu(), k[p[0]])           # its rows would have come from the bad page
+    assert torch.equal(cache.k[p[1]].cpu(), k[p[3]]) and torch.equal(cache.v[p[1]].cpu(), v[p[3]])
+    assert torch.equal(cache.k[bad].cpu(), k[bad])
+    assert cache.pos[0, 0, :32].tolist() == list(range(32, 64))
+
+
+# ------------------------------------------------------------------------------------ logits rules
+@pytest.mark.parametrize("vocab", [1, 3, 31, 32, 100, 1001, 5000, 70001, 151936])
+@pytest.mark.parametrize("inplace", [True, False], ids=["inplace", "out"])
+def test_adjust_logits(vocab, inplace):
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(vocab)
+    rows, H, NB = 5, 90, 12
+    x = torch.randn(rows, vocab, generator=g) * 4
+    x[0, vocab // 2] = NAN
+    x[1, vocab - 1] = math.inf
+    x[2] = -3.4028234663852886e38
+    x[3, vocab // 3] = 0.0
+    hist = torch.randint(-2, vocab + 2, (rows, H), generator=g, dtype=torch.int32)     # some ids outside
+    hist[3, :40] = vocab - 1
+    n_hist = torch.tensor([0, H, 50, H, 1], dtype=torch.int32)
+    n_prompt = torch.tensor([0, 30, 50, 0, 5], dtype=torch.int32)
+    rep, pres, freq = 1 + torch.rand(rows, generator=g), torch.rand(rows, generator=g), torch.rand(rows, generator=g)
+    ids = torch.randint(-1, vocab + 1, (rows, NB), generator=g, dtype=torch.int32)
+    ids[1] = vocab // 2                                       # one token listed twelve times
+    bias = torch.randn(rows, NB, generator=g)
+    words = (vocab + 31) // 32
+    mask = torch.randint(-2 ** 31, 2 ** 31, (rows, words), generator=g).int()
+    mask[4] = 0                                               # nothing allowed
+    tail = vocab % 32
+    if tail:
+        mask[:, -1] |= -1 << tail                             # bits behind the vocabulary mean nothing
+        mask[4, -1] = -1 << tail if tail < 32 else 0
+    wide = torch.full((rows, vocab + 3), 1e30)
+    wide[:, :vocab] = x
+    dev = wide.cuda() if vocab % 2 else x.cuda()
+    out = None if inplace else torch.empty(rows, vocab, device="cuda")
+    view = dev[:, :vocab]
+    c = lambda t: t.cuda()  # noqa: E731
+    token = S.adjust_logits(view, history=c(hist), n_history=c(n_hist), n_prompt=c(n_prompt), repetition=c(rep),
+                            presence=c(pres), frequency=c(freq), bias_ids=c(ids), bias=c(bias), mask=c(mask), out=out,
+                            none=-5)
+    _no_error()
+    got = (view if inplace else out).cpu()
+    t = torch.arange(vocab)
+    for r in range(rows):
+        allowed = (mask[r][t // 32] >> (t % 32).int()) & 1 == 1
+        want, pick = R.adjust(x[r], hist[r], int(n_hist[r]), min(int(n_prompt[r]), int(n_hist[r])), float(rep[r]),
+                              float(pres[r]), float(freq[r]), ids[r], bias[r], allowed)
+        big = torch.isinf(want.float()) | torch.isnan(want)
+        assert torch.equal(torch.isnan(got[r]), torch.isnan(want)) and torch.equal(got[r][big & ~torch.isnan(want)],
+                                                                                   want[big & ~torch.isnan(want)].float())
+        # five roundings of numbers no larger than |x| rep + freq count + presence + |bias|
+        size = x[r].abs().double() * 2 + H + 1 + bias[r].abs().max()
+        assert ((got[r].double() - want).abs()[~big] <= 5 * 2.0 ** -24 * size[~big]).all()
+        if pick is None:
+            assert int(token[r]) == -5
+        else:                                                 # the pick of the rounded values, in np.argmax's order
+            ok = torch.nonzero(allowed)[:, 0]
+            import numpy as np
+            assert int(token[r]) == int(ok[int(np.argmax(got[r][ok].numpy()))])
+    if not inplace:
+        assert torch.equal(torch.nan_to_num(view.cpu()), torch.nan_to_num(x))
+    if vocab % 2:
+        assert (dev[:, vocab:] == 1e30).all()
+
+
+def test_adjust_logits_without_rules_is_the_greedy_pick():
+    from opentars_b200 import serving as S
+    x = torch.randn(3, 4097).cuda()
+    was = x.clone()
+    assert S.adjust_logits(x).tolist() == was.argmax(1).tolist() and torch.equal(x, was)
+    empty = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
+    assert S.adjust_logits(x, history=empty, repetition=torch.full((3,), 2.0).cuda()).tolist() == was.argmax(1).tolist()
+    mask = torch.zeros(129, dtype=torch.int32, device="cuda")  # one mask for all rows
+    mask[2] = 1 << 5
+    assert S.adjust_logits(x, mask=mask).tolist() == [69] * 3
+    hist = torch.tensor([[7, 7, 7]] * 3, dtype=torch.int32, device="cuda")
+    y = was.clone()
+    S.adjust_logits(y, history=hist, frequency=torch.tensor([0.5, 0.25, 0.0]).cuda())
+    assert torch.allclose((was - y)[:, 7].cpu(), torch.tensor([1.5, 0.75, 0.0]), atol=1e-6)
+    y[:, 7] = was[:, 7]
+    assert torch.equal(y, was)
+
+
+# --------------------------------------------------------------------------------------- refusals
+def test_refusals_of_the_wrappers():
+    from opentars_b200 import serving as S
+    cache = S.PagedCache.empty(4, 16, 2, 64, 2, 2)
+    tracked = S.PagedCache.empty(4, 16, 2, 64, 2, 2, track=True)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    bad = [lambda: S.attend(cache, q.half(), 1.0), lambda: S.attend(cache, q[:1], 1.0), lambda: S.attend(cache, q[:, :3], 1.0),
+           lambda: S.attend(cache, q.cpu(), 1.0), lambda: S.attend(cache, q, 1.0, window=-1),
+           lambda: S.attend(cache, q, float("nan")), lambda: S.attend(cache, q, 1.0, weight_out=tracked.weight),
+           lambda: S.attend(cache, q, 1.0, out=q[:1].expand(2, 4, 64)), lambda: S.attend(cache, q[:, :, ::2], 1.0),
+           lambda: S.attend(tracked, q, 1.0, weight_out=tracked.weight[:, :, :8]),
+           lambda: S.attend_prompt(cache, q, cu[:2], 1.0), lambda: S.attend_prompt(cache, q, cu.long(), 1.0),
+           lambda: S.append(cache, q, q), lambda: S.append(cache, q[:, :2], q[:, :2].float()),
+           lambda: S.append(cache, torch.zeros(3, 2, 64, device="cuda"), torch.zeros(3, 2, 64, device="cuda")),
+           lambda: S.evict(cache, 8), lambda: S.evict(tracked, 0), lambda: S.evict(tracked, 8, sinks=4, recent=5),
+           lambda: S.evict(tracked, 8, pos_out=tracked.weight),
+           lambda: S.adjust_logits(torch.zeros(2, 10, device="cuda").half()),
+           lambda: S.adjust_logits(torch.zeros(1, 10, device="cuda").expand(2, 10)),
+           lambda: S.adjust_logits(torch.zeros(2, 10, device="cuda"), repetition=torch.ones(2, device="cuda")),
+           lambda: S.adjust_logits(torch.zeros(2, 10, device="cuda"), mask=torch.zeros(2, 2, dtype=torch.int32, device="cuda")),
+           lambda: S.adjust_logits(torch.zeros(2, 10, device="cuda"), token=torch.zeros(3, dtype=torch.int32, device="cuda"))]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    with pytest.raises(ValueError):
+        S.PagedCache(cache.k, cache.v, cache.table, cache.length, weight=tracked.weight)
+    with pytest.raises(ValueError):
+        S.PagedCache(cache.k[:, :8], cache.v[:, :8], cache.table, cache.length)
+
+
+# ----------------------------------------------------------------------------- a run of them together
+def _conversation(S, cache, tokens, kv, nh, hd, budget, g, stream=None):
+    """Prompt chunks, single tokens and evictions over one cache; returns every output."""
+    outs, cu0 = [], torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for n in tokens:
+        new = torch.randn(2 * n, kv, hd, generator=g, device="cuda")
+        val = torch.randn(2 * n, kv, hd, generator=g, device="cuda")
+        q = torch.randn(2 * n, nh, hd, generator=g, device="cuda").bfloat16()
+        cache.length.add_(n)
+        cache.seen.add_(n)
+        S.append(cache, new, val, cu0 * n)
+        if n > 1:
+            outs.append(S.attend_prompt(cache, q, cu0 * n, hd ** -0.5))
+        else:
+            outs.append(S.attend(cache, q, hd ** -0.5, weight_out=cache.weight))
+        S.evict(cache, budget, sinks=2, recent=16)
+    return outs
+
+
+def test_a_conversation_with_evictions_against_the_definitions():
+    """append, attend_prompt, attend with weights and evict in turn, every step's outputs against the
+    64-bit forms over the same token history."""
+    from opentars_b200 import serving as S
+    kv, nh, hd, page, budget = 2, 4, 64, 16, 48
+    cache = S.PagedCache.empty(12, page, kv, hd, 2, 6, track=True)
+    cache.table.copy_(torch.randperm(12, generator=torch.Generator().manual_seed(0)).reshape(2, 6).int())
+    cache.k.fill_(NAN)
+    cache.v.fill_(NAN)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    steps = [30, 1, 1, 25, 1, 1, 1, 40, 1]
+    # the model of the cache: per (sequence, head) lists of (key, value, weight, position)
+    model = [[[] for _ in range(kv)] for _ in range(2)]
+    seen = 0
+    for n in steps:
+        gs = torch.Generator(device="cuda")
+        gs.set_state(g.get_state())
+        new = torch.randn(2 * n, kv, hd, generator=gs, device="cuda").bfloat16().cpu()
+        val = torch.randn(2 * n, kv, hd, generator=gs, device="cuda").bfloat16().cpu()
+        q = torch.randn(2 * n, nh, hd, generator=gs, device="cuda").bfloat16().cpu()
+        out = _conversation(S, cache, [n], kv, nh, hd, budget, g)[0].cpu()
+        for b in range(2):
+            for h in range(kv):
+                for i in range(n):
+                    model[b][h].append([new[b * n + i, h], val[b * n + i, h], 0.0, seen + i])
+        ref = torch.zeros(out.shape, dtype=torch.float64)
+        for b in range(2):
+            for h in range(kv):
+                m = model[b][h]
+                kk, vv = torch.stack([e[0] for e in m])[:, None], torch.stack([e[1] for e in m])[:, None]
+                for i in range(n):
+                    end = len(m) - n + i + 1
+                    heads = slice(2 * h, 2 * h + 2)
+                    o, p = R.attend_row(q[b * n + i, heads], kk[:end], vv[:end], torch.ones(end, dtype=torch.bool), hd ** -0.5)
+                    ref[b * n + i, heads] = o
+                    if n == 1:
+                        for j in range(end):
+                            m[j][2] += float(p[:, j].sum())
+        kk = torch.stack([e[0] for e in model[0][0]])[:, None]
+        vv = torch.stack([e[1] for e in model[0][0]])[:, None]
+        tol = _tolerance(ref, q, torch.cat([kk, new.reshape(-1, 1, hd)]), torch.cat([vv, val.reshape(-1, 1, hd)]), hd ** -0.5,
+                         torch.bfloat16)
+        _close(out, ref, tol + 2.0 ** -8 * ref.abs().max(), f"step of {n}")
+        seen += n
+        for b in range(2):
+            for h in range(kv):
+                m = model[b][h]
+                if len(m) > budget:
+                    # the device's own sums rank the slots (ties of 64-bit sums may fall otherwise)
+                    order = sorted(range(len(m)), key=lambda s: (not (m[s][3] < 2 or m[s][3] >= seen - 16), -m[s][2], s))
+                    kept = set(order[:budget])
+                    arrive = iter(sorted(s for s in kept if s >= budget))
+                    model[b][h] = [m[s] if s in kept else m[next(arrive)] for s in range(budget)]
+                assert cache.pos[b, h, :len(model[b][h])].tolist() == [e[3] for e in model[b][h]], (n, b, h)
+        assert cache.length.tolist() == [len(model[0][0])] * 2
+    _no_error()
+
+
+def test_captured_calls_replay_and_share_nothing():
+    """The calls captured into two CUDA graphs, replayed in turn with eager calls between, on a stream of
+    their own: the same bits as eager calls."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(12)
+    made = []
+    for seed, lens in ((0, [700, 33, 0]), (1, [64, 1500, 129])):
+        k, v, table = _pools(lens, 2, 128, 16, torch.bfloat16, g)
+        cap = table.shape[1] * 16
+        w = torch.rand(3, 2, cap, generator=g)
+        pos = torch.arange(cap, dtype=torch.int32).repeat(3, 2, 1)
+        cache = _cache(k, v, table, lens, "heads", (w, pos, torch.tensor(lens, dtype=torch.int32)))
+        q = torch.randn(3, 4, 128, generator=g).bfloat16().cuda()
+        logits = torch.randn(3, 5000, generator=g).cuda()
+        hist = torch.randint(0, 5000, (3, 64), generator=g, dtype=torch.int32).cuda()
+        cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32).cuda()
+        out = dict(w=torch.zeros_like(cache.weight), w2=torch.zeros_like(cache.weight), p2=torch.zeros_like(cache.pos),
+                   n2=torch.zeros_like(cache.length), x=torch.empty_like(logits))
+        rep = torch.full((3,), 1.3).cuda()
+
+        def calls(cache=cache, q=q, logits=logits, hist=hist, cu=cu, out=out, rep=rep):
+            a = S.attend(cache, q, 0.09, window=600, sinks=4, weight_out=out["w"])
+            b = S.attend_prompt(cache, q, cu, 0.09)
+            S.evict(cache, 1600, 4, 16, out["n2"], out["w2"], out["p2"])
+            t = S.adjust_logits(logits, history=hist, repetition=rep, out=out["x"])
+            return [a, b, t, out["w"], out["w2"], out["p2"], out["n2"], out["x"]]
+        want = [x.clone() for x in calls()]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=side):
+            got = calls()
+        made.append((graph, got, want, calls))
+    for _ in range(3):
+        for graph, got, want, calls in made:
+            for x in got:
+                x.zero_()
+            graph.replay()
+            calls()
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(got, want):
+                assert torch.equal(x, y)
+    _no_error()
+
+
+def test_calls_on_two_streams_at_once():
+    """Two batches' calls on two streams give what they give one after the other."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(13)
+    jobs = []
+    for lens in ([3000, 5, 900], [100, 2000, 64]):
+        k, v, table = _pools(lens, 2, 64, 16, torch.float16, g)
+        cache = _cache(k, v, table, lens)
+        q = torch.randn(3, 4, 64, generator=g).half().cuda()
+        jobs.append((cache, q, S.attend(cache, q, 0.125).clone()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(10):
+        outs = []
+        for (cache, q, _), st in zip(jobs, streams):
+            with torch.cuda.stream(st):
+                outs.append(S.attend(cache, q, 0.125))
+        torch.cuda.synchronize()
+        for o, (_, _, want) in zip(outs, jobs):
+            assert torch.equal(o, want)
+    _no_error()
+
+
+def test_symbol_addresses_are_reached_through_ctypes():
+    """The C entry point itself, as a caller without torch's wrappers uses it."""
+    from opentars_b200.serving import Rules_t, lib
+    x = torch.randn(2, 300, device="cuda")
+    tok = torch.zeros(2, dtype=torch.int32, device="cuda")
+    r = Rules_t(logits=x.data_ptr(), out=x.data_ptr(), logits_stride=300, out_stride=300, rows=2, vocab=300,
+                token=tok.data_ptr(), none=-1)
+    assert lib().tc_adjust_logits(ctypes.byref(r), None) == 0
+    torch.cuda.synchronize()
+    assert tok.tolist() == x.argmax(1).tolist()
