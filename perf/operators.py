@@ -348,6 +348,8 @@ def _own(st):
         S.append(cache, st["k_new"], st["v_new"], st["cu"])
         return _kept(st)
     if op == "attend":
+        if "weight" in st:
+            st["weight_out"].copy_(st["weight"])            # the call writes the slots in use only
         out = S.attend(cache, st["q"], st["scale"], window=c["window"], sinks=c["sinks"], out=st["out"],
                        weight_out=st.get("weight_out"))
         return dict(out=out, weight=st["weight_out"]) if "weight" in st else out
