@@ -32,14 +32,11 @@ __device__ __forceinline__ void row_store(uint8_t* base, int64_t at, int lane, c
   for (int i = 0; i < HD / 64; ++i) reinterpret_cast<uint32_t*>(p)[i] = Elem<T>::pack(x[2 * i], x[2 * i + 1]);
 }
 
-// The row's visible slots are [0, min(sinks, end)) and [max(sinks, end - window), end).
-__device__ __forceinline__ int first_in_window(int end, int window) { return window < end ? end - window : 0; }
-
-// o = the attention of query q (head g's keys of sequence b) over the visible slots before `end`; the
-// scores (as powers of two) go to s_out where it is given. Statistics and sums in fp32.
+// o = the attention of query q (head g's keys of sequence b) over the visible slots before `end`.
+// Statistics and sums in fp32.
 template <class T, int HD>
 __device__ void attend_row(const KvCache& c, int b, int g, const float (&q)[HD / 32], float scale2, int end, int window,
-                           int sinks, int code, float (&o)[HD / 32], float* s_out, float* m_out, float* l_out) {
+                           int sinks, int code, float (&o)[HD / 32]) {
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31;
   float m = __int_as_float(0xFF800000), l = 0.0f;
@@ -64,7 +61,6 @@ __device__ void attend_row(const KvCache& c, int b, int g, const float (&q)[HD /
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
     s *= scale2;
-    if (s_out && lane == 0) s_out[j] = s;
     any = true;
     const float m2 = fmaxf(m, s), base = m2 == __int_as_float(0xFF800000) ? 0.0f : m2;
     const float f = exp2f(m - base), p = exp2f(s - base);
@@ -77,10 +73,6 @@ __device__ void attend_row(const KvCache& c, int b, int g, const float (&q)[HD /
     const float r = 1.0f / l;
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] *= r;
-  }
-  if (m_out && lane == 0) {
-    *m_out = m;
-    *l_out = l;
   }
 }
 

@@ -39,6 +39,7 @@
 #include "gemm_epi.cuh"
 #include "mma.h"
 #include "ops.h"
+#include "paged_map.h"
 #include "umma.cuh"
 #include "pdl.cuh"
 
@@ -783,6 +784,18 @@ bool make_map_u8(CUtensorMap* m, const void* ptr, uint64_t cols, uint64_t rows, 
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_map_pool(CUtensorMap* m, const KvCache& c, const void* pool, int rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  // a dimension of one entry is never stepped over: any legal stride serves
+  auto stride = [&](int64_t s, int n) { return (cuuint64_t)(n > 1 && s > 0 ? 2 * s : 2 * (int64_t)c.hd); };
+  const cuuint64_t dims[4] = {(cuuint64_t)c.hd, (cuuint64_t)1 << c.shift, (cuuint64_t)c.n_kv, (cuuint64_t)c.n_pages};
+  const cuuint64_t strides[3] = {stride(c.ss, 1 << c.shift), stride(c.sh, c.n_kv), stride(c.sp, c.n_pages)};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(pool), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 bool mma_engine_ok(const EngGemvArgs& g) {
   if (g.M < 2 || g.K % 16 || g.kb % 16 || (uintptr_t)g.A % 16 || g.lda % 16 || !encode_fn()) return false;

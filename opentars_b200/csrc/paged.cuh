@@ -47,6 +47,9 @@ __device__ __forceinline__ int seq_of(const int* cu, int batch, int i) {
   return lo;
 }
 
+// The visible slots of a row whose last one is end - 1: [0, min(sinks, first)) and [first, end).
+__device__ __forceinline__ int first_in_window(int end, int window) { return window < end ? end - window : 0; }
+
 template <class T>
 struct Elem;
 template <>

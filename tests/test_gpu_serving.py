@@ -721,3 +721,29 @@ def test_symbol_addresses_are_reached_through_ctypes():
     assert lib().tc_adjust_logits(ctypes.byref(r), None) == 0
     torch.cuda.synchronize()
     assert tok.tolist() == x.argmax(1).tolist()
+
+
+@pytest.mark.parametrize("op,code", [("attend", 55)])
+def test_waits_that_run_out_are_recorded(op, code):
+    """With a poll limit of 0 every wait for work gives up at once: the call ends, the word holds its code, and
+    the next call is right again."""
+    from opentars_b200 import serving as S
+    from opentars_b200._lib import lib
+    g = torch.Generator().manual_seed(14)
+    lens = [500, 0, 90]
+    k, v, table = _pools(lens, 2, 128, 16, torch.bfloat16, g)
+    cache = _cache(k, v, table, lens)
+    q = torch.randn(3, 4, 128, generator=g).bfloat16().cuda()
+    cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32).cuda()
+    call = (lambda: S.attend(cache, q, 0.09)) if op == "attend" else (lambda: S.attend_prompt(cache, q, cu, 0.09))
+    want = call().clone()
+    _no_error()
+    was = lib().tc_set_spin_limit(0)
+    try:
+        call()
+        torch.cuda.synchronize()
+        assert S.device_error(clear=True) == code
+    finally:
+        lib().tc_set_spin_limit(was)
+    assert torch.equal(call(), want)
+    _no_error()
