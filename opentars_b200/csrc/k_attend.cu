@@ -109,12 +109,6 @@ __device__ __forceinline__ long long plan(const AttendArgs& a, int nsub, PlanSha
   return total;
 }
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int x, int y, int z, int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
-          "r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -139,12 +133,6 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float neg_inf() { return __int_as_float(0xFF800000); }
 // The factor a state kept at maximum m takes at maximum m2 >= m (1 where both are still -infinity).
 __device__ __forceinline__ float shrink(float m, float m2) { return m2 == neg_inf() ? 1.0f : ex2(m - m2); }
 
@@ -339,7 +327,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
               for (int x = lane; x < HD / 8; x += 32)
                 *reinterpret_cast<uint4*>(s_tiles + stage * 2 * Sh::kMat + Sh::kMat + (x >> 3) * kTile * 128 +
                                           (16 * warp + r) * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          fence_async_shared();
           __syncwarp();
         }
         float m2[2];

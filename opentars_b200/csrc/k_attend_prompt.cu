@@ -1,45 +1,476 @@
-// Attention of the rows of a prompt over the paged cache (tc_attend_prompt), one warp per (row, head).
+// Attention of the rows of a prompt over the paged cache (tc_attend_prompt), on the 5th-generation
+// tensor cores.
+//
+// A tile is 128 query rows: the heads of one key-value head (at most 32 of them) for 128 / heads
+// consecutive tokens, so a group's heads share every key and value tile that is staged. A CTA takes
+// two tiles (one for head dim 256, whose output alone fills half of TMEM) of one sequence and walks
+// the blocks of key slots that any of its rows sees: the sinks' blocks, then those of the windows.
+//   producer   one warp: a block's keys and values page by page by TMA (64 columns x page rows
+//              boxes, 128-byte swizzle) into a ring; value rows behind the sequence's end, which
+//              may hold anything, are cleared there (0 x NaN is not 0)
+//   MMA        one thread: S = Q K^T into TMEM (tcgen05 kind::f16), then O += P V with P as the
+//              TMEM operand where S was; with two tiles one is multiplied while the other is
+//              exponentiated, with one tile S is double-buffered
+//   softmax    a warpgroup per tile, a thread per row: the row's scores stay in registers, the
+//              running maximum is only moved (and O rescaled) when it grows by more than 2^8, and
+//              P is rounded to the cache's type, whose range holds 2^8; the row's sum is of the
+//              unrounded fp32 values
+// A row whose output is not finite, and every row of a CTA that met a page id outside the pool, is
+// computed again by attend_row over its visible slots alone: a NaN or an infinity in a slot that the
+// mask hides from this row but not from its tile reaches it as 0 x inf.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "attend_row.cuh"
+#include "mma.h"
+#include "paged_map.h"
+#include "pdl.cuh"
+#include "umma.cuh"
 
 namespace tc {
 namespace {
 
-constexpr int kRowThreads = 128;
+constexpr int kRows = 128, kMaxHeads = 32;
+
+template <int HD>
+struct PromptShape {
+  static constexpr int kTiles = HD == 256 ? 1 : 2;           // query tiles of a CTA
+  static constexpr int kBlock = HD == 256 ? 64 : 128;        // key slots of a block
+  static constexpr int kQ = kRows * HD * 2, kMat = kBlock * HD * 2;
+  static constexpr int kSlots = HD == 64 ? 8 : 5;            // ring of key / value blocks
+  static constexpr int kThreads = 128 * kTiles + 64;
+  static constexpr int kSmem = 1024 + kTiles * kQ + kSlots * kMat;
+  static constexpr uint32_t kS = 0, kO = 256;                // TMEM columns: two S (and P) buffers, the outputs
+};
+
+struct PromptMaps {
+  CUtensorMap k, v;
+};
+
+// What a CTA works on, the same in every thread.
+struct Work {
+  int b, kvh, h0, hb;               // sequence, key-value head, first query head and how many
+  int row0, n, len;                 // first row of the sequence in q, its rows, its slots
+  int tok[2];                       // first token (of the sequence's n) of each tile
+  int ntok[2], end[2], nb[2];       // its tokens, one past its last position, its blocks
+  int first, head, na, t0, nmax;    // visible slots [0, head) and [first, end): blocks 0 .. na - 1, t0 on
+  __device__ __forceinline__ int block(int j) const { return j < na ? j : t0 + j - na; }
+};
 
 template <class T, int HD>
-__global__ void __launch_bounds__(kRowThreads) k_prompt_rows(AttendArgs a) {
-  const KvCache& c = a.c;
-  const int64_t u = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) / 32;
-  const int lane = threadIdx.x & 31;
-  if (u >= (int64_t)a.tokens * a.nh) return;
-  const int i = (int)(u / a.nh), h = (int)(u - (int64_t)i * a.nh);
-  const int b = seq_of(a.cu, c.batch, i);
-  if (b < 0) return;
-  const int end = kv_length(c, b, kErrPrompt) - (__ldg(a.cu + b + 1) - i) + 1;
+__device__ __noinline__ void redo_row(const AttendArgs& a, int b, int kvh, int64_t row, int h, int end) {
   float q[HD / 32], o[HD / 32];
-  row_load<T, HD>(a.q, (int64_t)i * a.qr + (int64_t)h * a.qh, lane, q);
-  attend_row<T, HD>(c, b, h / (a.nh / c.n_kv), q, a.scale2, max(end, 0), a.window, a.sinks, kErrPrompt, o);
-  row_store<T, HD>(a.out, (int64_t)i * a.orow + (int64_t)h * a.oh, lane, o);
+  const int lane = threadIdx.x & 31;
+  row_load<T, HD>(a.q, row * a.qr + (int64_t)h * a.qh, lane, q);
+  attend_row<T, HD>(a.c, b, kvh, q, a.scale2, end, a.window, a.sinks, kErrPrompt, o);
+  row_store<T, HD>(a.out, row * a.orow + (int64_t)h * a.oh, lane, o);
+}
+
+template <class T, int HD>
+__global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
+    k_prompt(const __grid_constant__ PromptMaps maps, const __grid_constant__ AttendArgs a, int gblocks, int hb, int tokens) {
+  using Sh = PromptShape<HD>;
+  constexpr int NT = Sh::kTiles, BN = Sh::kBlock;
+  extern __shared__ uint8_t s_raw[];
+  __shared__ __align__(8) uint64_t s_full[Sh::kSlots], s_free[Sh::kSlots], s_sfull[2], s_pfull[2], s_odone[2], s_fix, s_end;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_scan[16], s_found[2], s_bad, s_dead;
+  const KvCache& c = a.c;
+  uint8_t* s_q = s_raw + (1024 - (smem_u32(s_raw) & 1023)) % 1024;
+  uint8_t* s_kv = s_q + NT * Sh::kQ;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kProducer = 4 * NT, kMma = kProducer + 1;
+
+  // ---- which rows: pairs of tiles, sequence by sequence; the last pairs (the longest rows) go first
+  Work w;
+  {
+    const int nsub = c.n_kv * gblocks, span = NT * tokens;
+    const int pairs = gridDim.x / nsub, pr = pairs - 1 - (int)(blockIdx.x / nsub), sub = blockIdx.x % nsub;
+    const int per = (c.batch + Sh::kThreads - 1) / Sh::kThreads, lo = min(c.batch, (int)threadIdx.x * per), hi = min(c.batch, lo + per);
+    if (threadIdx.x == 0) s_found[0] = -1;
+    int mine = 0;
+    for (int b = lo; b < hi; ++b) mine += (max(__ldg(a.cu + b + 1) - __ldg(a.cu + b), 0) + span - 1) / span;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    if (lane == 31) s_scan[warp] = sum;
+    __syncthreads();
+    int at = sum - mine;
+    for (int k = 0; k < warp; ++k) at += s_scan[k];
+    if (pr >= at && pr < at + mine) {
+      int b = lo;
+      for (; b < hi - 1; ++b) {
+        const int k = (max(__ldg(a.cu + b + 1) - __ldg(a.cu + b), 0) + span - 1) / span;
+        if (pr < at + k) break;
+        at += k;
+      }
+      s_found[0] = b;
+      s_found[1] = pr - at;
+    }
+    __syncthreads();
+    w.b = s_found[0];
+    if (w.b < 0) return;
+    w.kvh = sub / gblocks;
+    const int G = a.nh / c.n_kv, g0 = (sub - w.kvh * gblocks) * hb;
+    w.h0 = w.kvh * G + g0;
+    w.hb = min(hb, G - g0);
+    w.row0 = __ldg(a.cu + w.b);
+    w.n = __ldg(a.cu + w.b + 1) - w.row0;
+    const int rows = w.row0 < 0 ? 0 : min(w.n, a.tokens - w.row0);       // (rows outside q are left out)
+    w.len = kv_length(c, w.b, kErrPrompt);
+    const int tok0 = s_found[1] * span, p0 = w.len - w.n + tok0;
+    w.first = p0 + 1 > 0 ? first_in_window(p0 + 1, a.window) : 0;
+    w.head = min(a.sinks, w.first);
+    w.t0 = w.first / BN;
+    w.na = min((w.head + BN - 1) / BN, w.t0);
+    w.nmax = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      w.tok[t] = tok0 + t * tokens;
+      w.ntok[t] = t < NT ? min(max(rows - w.tok[t], 0), tokens) : 0;
+      w.end[t] = w.ntok[t] ? max(w.len - w.n + w.tok[t] + w.ntok[t], 0) : 0;
+      w.nb[t] = w.end[t] ? w.na + (w.end[t] + BN - 1) / BN - w.t0 : 0;
+      w.nmax = max(w.nmax, w.nb[t]);
+    }
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Sh::kSlots; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_sfull[i], 1);
+      mbar_init(&s_pfull[i], 4);
+      mbar_init(&s_odone[i], 1);
+    }
+    mbar_init(&s_fix, 1);
+    mbar_init(&s_end, 1);
+    mbar_fence_init();
+    s_bad = s_dead = 0;
+  }
+  if (warp == kMma) tmem_alloc(&s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp == kProducer) {
+    int slot = 0, phase = 0, issued = 0, fixes = 0;
+    const int end = max(w.end[0], w.end[1]), box = min(BN, 1 << c.shift), per = box / 16;
+    auto load = [&](int j, bool is_v) {
+      if (issued >= Sh::kSlots &&
+          !__all_sync(0xFFFFFFFFu, mbar_wait(&s_free[slot], phase ^ 1, c.err, kErrPromptWait, a.spin)))
+        return false;
+      const int j0 = w.block(j) * BN, js = j0 + 16 * lane;
+      int page = -1;
+      if (lane < BN / 16 && js < end) {
+        page = __ldg(c.table + (int64_t)w.b * c.ts + (js >> c.shift));
+        if ((unsigned)page >= (unsigned)c.n_pages) {
+          page = -1;
+          if (js + 16 > w.first || js < w.head) {      // (a page that no row sees may be gone)
+            kv_fail(c, kErrPrompt);
+            s_bad = 1;
+          }
+        }
+      }
+      const uint32_t have = __ballot_sync(0xFFFFFFFFu, page >= 0);
+      const bool fix = is_v && (have != (1u << BN / 16) - 1 || j0 + BN > w.len);
+      uint64_t* bar = fix ? &s_fix : &s_full[slot];
+      auto groups = [&](int u) { return have >> (u * per) & ((1u << per) - 1); };   // of box u
+      uint32_t bytes = 0;
+      for (int u = 0; u < BN / box; ++u) bytes += groups(u) ? box * HD * 2 : 0;
+      if (lane == 0) mbar_expect_tx(bar, bytes);
+      __syncwarp();
+      uint8_t* dst = s_kv + slot * Sh::kMat;
+      const int boxes = BN / box * (HD / 64), x = min(lane, boxes - 1), u = x / (HD / 64), half = x - u * (HD / 64);
+      const uint32_t here = groups(u);
+      const int pg = __shfl_sync(0xFFFFFFFFu, page, here ? u * per + __ffs(here) - 1 : 0);
+      if (here && lane < boxes)
+        tma_load_4d(smem_u32(dst) + half * BN * 128 + u * box * 128, is_v ? &maps.v : &maps.k, 64 * half,
+                    (j0 + u * box) & ((1 << c.shift) - 1), w.kvh, pg, bar);
+      if (fix) {
+        const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_fix, fixes & 1, c.err, kErrPromptWait));
+        ++fixes;
+        if (!ok) return false;
+        for (int r = 0; r < BN; ++r)
+          if (!(have >> (r >> 4) & 1) || j0 + r >= w.len)
+            for (int y = lane; y < HD / 8; y += 32)
+              *reinterpret_cast<uint4*>(dst + (y >> 3) * BN * 128 + r * 128 + (y & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_full[slot]);
+      }
+      ++issued;
+      if (++slot == Sh::kSlots) { slot = 0; phase ^= 1; }
+      return true;
+    };
+    bool ok = w.nmax == 0 || load(0, false);
+    for (int j = 0; ok && j < w.nmax; ++j) {
+      // in the order of use: with two tiles V(j), K(j + 1); with one K(j + 1), V(j)
+      if (NT == 2) ok = load(j, true) && (j + 1 == w.nmax || load(j + 1, false));
+      else ok = (j + 1 == w.nmax || load(j + 1, false)) && load(j, true);
+    }
+    if (!ok) s_dead = 1;
+    // no copy is in flight when the block ends: the last use of every slot has arrived
+    for (int k = 0; k < Sh::kSlots && k < issued; ++k) {
+      if (--slot < 0) { slot = Sh::kSlots - 1; phase ^= 1; }
+      mbar_wait(&s_full[slot], phase, c.err, kErrPromptWait);
+    }
+  } else if (warp == kMma) {
+    asm volatile("bar.sync 1, %0;" ::"n"(128 * NT + 32) : "memory");       // Q is in shared memory
+    tc_fence_after();
+    if (lane == 0) {
+      constexpr bool bf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
+      constexpr uint32_t id_s = idesc_f16(kRows, BN, bf16, false), id_o = idesc_f16(kRows, HD, bf16, true);
+      int slot = 0, phase = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int parity) { return ok = ok && mbar_wait(bar, parity, c.err, kErrPromptWait, a.spin); };
+      auto next = [&] {
+        if (++slot == Sh::kSlots) { slot = 0; phase ^= 1; }
+      };
+      // S = Q K^T of tile t with the keys in `at`, into buffer `buf`
+      auto scores = [&](int t, int at, int buf) {
+        const uint32_t q = smem_u32(s_q) + t * Sh::kQ, k = smem_u32(s_kv) + at * Sh::kMat;
+#pragma unroll
+        for (int x = 0; x < HD / 16; ++x)
+          mma_f16(tmem + Sh::kS + buf * BN, sdesc_k128(q + (x >> 2) * kRows * 128) + 2 * (x & 3),
+                  sdesc_k128(k + (x >> 2) * BN * 128) + 2 * (x & 3), id_s, x > 0);
+        mma_commit(&s_sfull[buf]);
+      };
+      auto values = [&](int t, int at, int buf, bool more) {
+        const uint32_t v = smem_u32(s_kv) + at * Sh::kMat;
+#pragma unroll
+        for (int x = 0; x < BN / 16; ++x)
+          mma_f16_ta(tmem + Sh::kO + t * HD, tmem + Sh::kS + buf * BN + 8 * x, sdesc_mn128(v + x * 2048, BN * 128), id_o,
+                     more || x > 0);
+        mma_commit(&s_odone[t]);
+      };
+      if (w.nmax && wait(&s_full[0], 0)) {
+        tc_fence_after();
+        for (int t = 0; t < NT; ++t)
+          if (w.nb[t]) scores(t, 0, t);
+        mma_commit(&s_free[0]);
+        next();
+      }
+      for (int j = 0; ok && j < w.nmax; ++j) {
+        if constexpr (NT == 2) {
+          const int vs = slot, vph = phase;
+          next();
+          const int ks = slot, kph = phase;
+          const bool more = j + 1 < w.nmax;
+          if (more) next();
+          bool have_v = false, have_k = false;
+          for (int t = 0; t < 2; ++t) {
+            if (j >= w.nb[t]) continue;
+            if (!have_v && !wait(&s_full[vs], vph)) break;
+            have_v = true;
+            if (!wait(&s_pfull[t], j & 1)) break;
+            tc_fence_after();
+            values(t, vs, t, j > 0);
+            if (j + 1 < w.nb[t]) {
+              if (!have_k && !wait(&s_full[ks], kph)) break;
+              have_k = true;
+              scores(t, ks, t);
+            }
+          }
+          if (!ok) break;
+          mma_commit(&s_free[vs]);
+          if (more) mma_commit(&s_free[ks]);
+        } else {
+          if (j + 1 < w.nmax) {
+            if (!wait(&s_full[slot], phase)) break;
+            tc_fence_after();
+            scores(0, slot, (j + 1) & 1);
+            mma_commit(&s_free[slot]);
+            next();
+          }
+          if (!wait(&s_full[slot], phase) || !wait(&s_pfull[j & 1], j >> 1 & 1)) break;
+          tc_fence_after();
+          values(0, slot, j & 1, j > 0);
+          mma_commit(&s_free[slot]);
+          next();
+        }
+      }
+      if (!ok) s_dead = 1;
+      mma_commit(&s_end);                          // nothing this thread issued is still running when the block ends
+      mbar_wait(&s_end, 0, c.err, kErrPromptWait);
+    }
+    __syncwarp();
+  }
+
+  // ---- softmax: thread = row
+  const int t = NT == 2 ? warp >> 2 : 0, r = threadIdx.x & 127;
+  const uint32_t lanes = (uint32_t)(warp & 3) << 21;                     // this warp's TMEM lanes, 32 (warp % 4) on
+  const int tok = r / w.hb, h = w.h0 + r - tok * w.hb;
+  const bool mine = warp < kProducer && tok < w.ntok[t];
+  const int p = mine ? w.len - w.n + w.tok[t] + tok : -1;
+  float l = 0.0f;
+  if (warp < kProducer) {
+    // the query rows into shared memory (16-byte pieces, 128-byte swizzle); a negative scale goes into their signs
+    const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
+    for (int x = r; x < kRows * HD / 8; x += 128) {
+      const int row = x / (HD / 8), e = x - row * (HD / 8), rt = row / w.hb;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (rt < w.ntok[t]) {
+        v = __ldg(reinterpret_cast<const uint4*>(a.q + 2 * ((int64_t)(w.row0 + w.tok[t] + rt) * a.qr +
+                                                             (int64_t)(w.h0 + row - rt * w.hb) * a.qh + 8 * e)));
+        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+      }
+      *reinterpret_cast<uint4*>(s_q + t * Sh::kQ + (e >> 3) * kRows * 128 + row * 128 + (((e & 7) ^ (row & 7)) << 4)) = v;
+    }
+    fence_async_shared();
+    asm volatile("bar.sync 1, %0;" ::"n"(128 * NT + 32) : "memory");
+    const float scale2 = fabsf(a.scale2);
+    const int pmin = w.len - w.n + w.tok[t], pmax = w.end[t] - 1, n = w.nb[t];
+    const int from = first_in_window(p + 1, a.window);
+    float m = neg_inf();
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int buf = NT == 2 ? t : j & 1, ph = NT == 2 ? j & 1 : j >> 1 & 1;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_sfull[buf], ph, c.err, kErrPromptWait, a.spin));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t st = tmem + lanes + Sh::kS + buf * BN;
+      uint32_t v[BN];
+#pragma unroll
+      for (int x = 0; x < BN; x += 32) tmem_ld32(st + x, v + x);
+      tmem_wait_ld();
+#pragma unroll
+      for (int x = 0; x < BN; ++x) asm volatile("" : "+r"(v[x]));        // no use moves before the wait
+      const int j0 = w.block(j) * BN;
+      if (j0 + BN - 1 > pmin || (pmax - j0 >= a.window && j0 + BN > a.sinks)) {
+        const int hi = p + 1 - j0, lo = from - j0, sk = a.sinks - j0;
+#pragma unroll
+        for (int x = 0; x < BN; ++x)
+          if (!(x < hi && (x >= lo || x < sk))) v[x] = 0xFF800000u;
+      }
+      float mx[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+      for (int x = 0; x < BN; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+      const bool grow = top > m + 8.0f || (m == neg_inf() && top > m);
+      if (__any_sync(0xFFFFFFFFu, grow)) {
+        const float f = grow ? ex2(m - top) : 1.0f;
+        if (grow) m = top;
+        l *= f;
+        if (j > 0) {
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_odone[t], (j - 1) & 1, c.err, kErrPromptWait, a.spin));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t ot = tmem + lanes + Sh::kO + t * HD;
+#pragma unroll
+          for (int x = 0; x < HD; x += 32) {
+            uint32_t o[32];
+            tmem_ld32(ot + x, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 32; ++y) {
+              asm volatile("" : "+r"(o[y]));
+              o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+            }
+            tmem_st32(ot + x, o);
+          }
+        }
+      }
+      const float base = m == neg_inf() ? 0.0f : m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int x = 0; x < BN; x += 2) {
+        const float p0 = ex2(fmaf(__uint_as_float(v[x]), scale2, -base)), p1 = ex2(fmaf(__uint_as_float(v[x + 1]), scale2, -base));
+        sum[x >> 1 & 3] += p0 + p1;
+        v[x >> 1] = Elem<T>::pack(p0, p1);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+      for (int x = 0; x < BN / 2; x += 32) tmem_st32(st + x, v + x);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_pfull[buf]);
+    }
+    if (ok && n) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_odone[t], (n - 1) & 1, c.err, kErrPromptWait, a.spin));
+    if (!ok) s_dead = 1;
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp < kProducer && !s_dead) {
+    const bool any = p >= 0;
+    const float inv = any ? 1.0f / l : 0.0f;
+    bool good = true;
+    const int64_t row = w.row0 + w.tok[t] + tok;
+    uint8_t* to = a.out + 2 * (row * a.orow + (int64_t)h * a.oh);
+#pragma unroll
+    for (int x = 0; x < HD; x += 32) {
+      uint32_t o[32];
+      if (w.nb[t]) {
+        tmem_ld32(tmem + lanes + Sh::kO + t * HD + x, o);
+        tmem_wait_ld();
+      }
+      uint32_t pk[16];
+#pragma unroll
+      for (int y = 0; y < 32; y += 2) {
+        asm volatile("" : "+r"(o[y]), "+r"(o[y + 1]));
+        const float o0 = any ? __uint_as_float(o[y]) * inv : 0.0f, o1 = any ? __uint_as_float(o[y + 1]) * inv : 0.0f;
+        good &= fabsf(o0) + fabsf(o1) < __int_as_float(0x7F800000);
+        pk[y >> 1] = Elem<T>::pack(o0, o1);
+      }
+      if (mine) {
+#pragma unroll
+        for (int y = 0; y < 16; y += 4)
+          *reinterpret_cast<uint4*>(to + 2 * x + 4 * y) = make_uint4(pk[y], pk[y + 1], pk[y + 2], pk[y + 3]);
+      }
+    }
+    __syncwarp();
+    uint32_t redo = __ballot_sync(0xFFFFFFFFu, mine && any && (!good || s_bad));
+    while (redo) {
+      const int from_lane = __ffs(redo) - 1;
+      redo &= redo - 1;
+      redo_row<T, HD>(a, w.b, w.kvh, __shfl_sync(0xFFFFFFFFu, row, from_lane), __shfl_sync(0xFFFFFFFFu, h, from_lane),
+                      __shfl_sync(0xFFFFFFFFu, p, from_lane) + 1);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMma) tmem_dealloc(tmem, 512);
+}
+
+template <class T, int HD>
+cudaError_t prompt_hd(const AttendArgs& a, cudaStream_t st) {
+  using Sh = PromptShape<HD>;
+  const KvCache& c = a.c;
+  PromptMaps maps;
+  const int box = std::min(Sh::kBlock, 1 << c.shift);
+  if (!make_map_pool(&maps.k, c, c.k, box) || !make_map_pool(&maps.v, c, c.v, box)) return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(k_prompt<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+  if (e != cudaSuccess) return e;
+  // a group's heads in blocks of nearly equal size; as many tokens as fill a tile with them
+  const int G = a.nh / c.n_kv, gblocks = (G + kMaxHeads - 1) / kMaxHeads, hb = (G + gblocks - 1) / gblocks;
+  const int tokens = kRows / hb, span = Sh::kTiles * tokens;
+  // every sequence ends in at most one span that is not full
+  const int64_t pairs = std::min<int64_t>(a.tokens, a.tokens / span + std::min(a.tokens, c.batch));
+  const int64_t grid = pairs * c.n_kv * gblocks;
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  k_prompt<T, HD><<<(unsigned)grid, Sh::kThreads, Sh::kSmem, st>>>(maps, a, gblocks, hb, tokens);
+  return cudaGetLastError();
 }
 
 template <class T>
-cudaError_t rows_of(const AttendArgs& a, cudaStream_t st) {
-  const int64_t blocks = ((int64_t)a.tokens * a.nh * 32 + kRowThreads - 1) / kRowThreads;
+cudaError_t prompt_of(const AttendArgs& a, cudaStream_t st) {
   switch (a.c.hd) {
-    case 64: k_prompt_rows<T, 64><<<blocks, kRowThreads, 0, st>>>(a); break;
-    case 128: k_prompt_rows<T, 128><<<blocks, kRowThreads, 0, st>>>(a); break;
-    default: k_prompt_rows<T, 256><<<blocks, kRowThreads, 0, st>>>(a); break;
+    case 64: return prompt_hd<T, 64>(a, st);
+    case 128: return prompt_hd<T, 128>(a, st);
+    default: return prompt_hd<T, 256>(a, st);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_attend_prompt(const AttendArgs& a, cudaStream_t st) {
-  if (a.tokens == 0) return cudaSuccess;
-  return a.dtype == TC_BF16 ? rows_of<__nv_bfloat16>(a, st) : rows_of<__half>(a, st);
+  return a.dtype == TC_BF16 ? prompt_of<__nv_bfloat16>(a, st) : prompt_of<__half>(a, st);
 }
 
 }  // namespace tc

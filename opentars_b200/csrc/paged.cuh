@@ -50,6 +50,14 @@ __device__ __forceinline__ int seq_of(const int* cu, int batch, int i) {
 // The visible slots of a row whose last one is end - 1: [0, min(sinks, first)) and [first, end).
 __device__ __forceinline__ int first_in_window(int end, int window) { return window < end ? end - window : 0; }
 
+// 2^x to 2 units in the last place (0 below 2^-126).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xFF800000); }
+
 template <class T>
 struct Elem;
 template <>

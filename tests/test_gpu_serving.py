@@ -723,7 +723,7 @@ def test_symbol_addresses_are_reached_through_ctypes():
     assert tok.tolist() == x.argmax(1).tolist()
 
 
-@pytest.mark.parametrize("op,code", [("attend", 55)])
+@pytest.mark.parametrize("op,code", [("attend", 55), ("prompt", 56)])
 def test_waits_that_run_out_are_recorded(op, code):
     """With a poll limit of 0 every wait for work gives up at once: the call ends, the word holds its code, and
     the next call is right again."""
