@@ -39,7 +39,7 @@ struct PromptShape {
   static constexpr int kBlock = HD == 256 ? 64 : 128;        // key slots of a block
   static constexpr int kQ = kRows * HD * 2, kMat = kBlock * HD * 2;
   static constexpr int kSlots = HD == 64 ? 8 : 5;            // ring of key / value blocks
-  static constexpr int kThreads = 128 * kTiles + 64;
+  static constexpr int kThreads = kTiles == 2 ? 384 : 192;   // (whole warpgroups where registers are split)
   static constexpr int kSmem = 1024 + kTiles * kQ + kSlots * kMat;
   static constexpr uint32_t kS = 0, kO = 256;                // TMEM columns: two S (and P) buffers, the outputs
 };
@@ -158,255 +158,268 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = s_tmem;
 
-  if (warp == kProducer) {
-    int slot = 0, phase = 0, issued = 0, fixes = 0;
-    const int end = max(w.end[0], w.end[1]), box = min(BN, 1 << c.shift), per = box / 16;
-    auto load = [&](int j, bool is_v) {
-      if (issued >= Sh::kSlots &&
-          !__all_sync(0xFFFFFFFFu, mbar_wait(&s_free[slot], phase ^ 1, c.err, kErrPromptWait, a.spin)))
-        return false;
-      const int j0 = w.block(j) * BN, js = j0 + 16 * lane;
-      int page = -1;
-      if (lane < BN / 16 && js < end) {
-        page = __ldg(c.table + (int64_t)w.b * c.ts + (js >> c.shift));
-        if ((unsigned)page >= (unsigned)c.n_pages) {
-          page = -1;
-          if (js + 16 > w.first || js < w.head) {      // (a page that no row sees may be gone)
-            kv_fail(c, kErrPrompt);
-            s_bad = 1;
-          }
-        }
-      }
-      const uint32_t have = __ballot_sync(0xFFFFFFFFu, page >= 0);
-      const bool fix = is_v && (have != (1u << BN / 16) - 1 || j0 + BN > w.len);
-      uint64_t* bar = fix ? &s_fix : &s_full[slot];
-      auto groups = [&](int u) { return have >> (u * per) & ((1u << per) - 1); };   // of box u
-      uint32_t bytes = 0;
-      for (int u = 0; u < BN / box; ++u) bytes += groups(u) ? box * HD * 2 : 0;
-      if (lane == 0) mbar_expect_tx(bar, bytes);
-      __syncwarp();
-      uint8_t* dst = s_kv + slot * Sh::kMat;
-      const int boxes = BN / box * (HD / 64), x = min(lane, boxes - 1), u = x / (HD / 64), half = x - u * (HD / 64);
-      const uint32_t here = groups(u);
-      const int pg = __shfl_sync(0xFFFFFFFFu, page, here ? u * per + __ffs(here) - 1 : 0);
-      if (here && lane < boxes)
-        tma_load_4d(smem_u32(dst) + half * BN * 128 + u * box * 128, is_v ? &maps.v : &maps.k, 64 * half,
-                    (j0 + u * box) & ((1 << c.shift) - 1), w.kvh, pg, bar);
-      if (fix) {
-        const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_fix, fixes & 1, c.err, kErrPromptWait));
-        ++fixes;
-        if (!ok) return false;
-        for (int r = 0; r < BN; ++r)
-          if (!(have >> (r >> 4) & 1) || j0 + r >= w.len)
-            for (int y = lane; y < HD / 8; y += 32)
-              *reinterpret_cast<uint4*>(dst + (y >> 3) * BN * 128 + r * 128 + (y & 7) * 16) = make_uint4(0, 0, 0, 0);
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_full[slot]);
-      }
-      ++issued;
-      if (++slot == Sh::kSlots) { slot = 0; phase ^= 1; }
-      return true;
-    };
-    bool ok = w.nmax == 0 || load(0, false);
-    for (int j = 0; ok && j < w.nmax; ++j) {
-      // in the order of use: with two tiles V(j), K(j + 1); with one K(j + 1), V(j)
-      if (NT == 2) ok = load(j, true) && (j + 1 == w.nmax || load(j + 1, false));
-      else ok = (j + 1 == w.nmax || load(j + 1, false)) && load(j, true);
-    }
-    if (!ok) s_dead = 1;
-    // no copy is in flight when the block ends: the last use of every slot has arrived
-    for (int k = 0; k < Sh::kSlots && k < issued; ++k) {
-      if (--slot < 0) { slot = Sh::kSlots - 1; phase ^= 1; }
-      mbar_wait(&s_full[slot], phase, c.err, kErrPromptWait);
-    }
-  } else if (warp == kMma) {
-    asm volatile("bar.sync 1, %0;" ::"n"(128 * NT + 32) : "memory");       // Q is in shared memory
-    tc_fence_after();
-    if (lane == 0) {
-      constexpr bool bf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
-      constexpr uint32_t id_s = idesc_f16(kRows, BN, bf16, false), id_o = idesc_f16(kRows, HD, bf16, true);
-      int slot = 0, phase = 0;
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, int parity) { return ok = ok && mbar_wait(bar, parity, c.err, kErrPromptWait, a.spin); };
-      auto next = [&] {
-        if (++slot == Sh::kSlots) { slot = 0; phase ^= 1; }
-      };
-      // S = Q K^T of tile t with the keys in `at`, into buffer `buf`
-      auto scores = [&](int t, int at, int buf) {
-        const uint32_t q = smem_u32(s_q) + t * Sh::kQ, k = smem_u32(s_kv) + at * Sh::kMat;
-#pragma unroll
-        for (int x = 0; x < HD / 16; ++x)
-          mma_f16(tmem + Sh::kS + buf * BN, sdesc_k128(q + (x >> 2) * kRows * 128) + 2 * (x & 3),
-                  sdesc_k128(k + (x >> 2) * BN * 128) + 2 * (x & 3), id_s, x > 0);
-        mma_commit(&s_sfull[buf]);
-      };
-      auto values = [&](int t, int at, int buf, bool more) {
-        const uint32_t v = smem_u32(s_kv) + at * Sh::kMat;
-#pragma unroll
-        for (int x = 0; x < BN / 16; ++x)
-          mma_f16_ta(tmem + Sh::kO + t * HD, tmem + Sh::kS + buf * BN + 8 * x, sdesc_mn128(v + x * 2048, BN * 128), id_o,
-                     more || x > 0);
-        mma_commit(&s_odone[t]);
-      };
-      if (w.nmax && wait(&s_full[0], 0)) {
-        tc_fence_after();
-        for (int t = 0; t < NT; ++t)
-          if (w.nb[t]) scores(t, 0, t);
-        mma_commit(&s_free[0]);
-        next();
-      }
-      for (int j = 0; ok && j < w.nmax; ++j) {
-        if constexpr (NT == 2) {
-          const int vs = slot, vph = phase;
-          next();
-          const int ks = slot, kph = phase;
-          const bool more = j + 1 < w.nmax;
-          if (more) next();
-          bool have_v = false, have_k = false;
-          for (int t = 0; t < 2; ++t) {
-            if (j >= w.nb[t]) continue;
-            if (!have_v && !wait(&s_full[vs], vph)) break;
-            have_v = true;
-            if (!wait(&s_pfull[t], j & 1)) break;
-            tc_fence_after();
-            values(t, vs, t, j > 0);
-            if (j + 1 < w.nb[t]) {
-              if (!have_k && !wait(&s_full[ks], kph)) break;
-              have_k = true;
-              scores(t, ks, t);
+  // With two tiles the launch's 168 registers a thread (3 warpgroups) are split 208 + 208 + 88, their sum unchanged
+  if (warp >= kProducer) {
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == kProducer) {
+      int slot = 0, phase = 0, issued = 0, fixes = 0;
+      const int end = max(w.end[0], w.end[1]), box = min(BN, 1 << c.shift), per = box / 16;
+      auto load = [&](int j, bool is_v) {
+        if (issued >= Sh::kSlots &&
+            !__all_sync(0xFFFFFFFFu, mbar_wait(&s_free[slot], phase ^ 1, c.err, kErrPromptWait, a.spin)))
+          return false;
+        const int j0 = w.block(j) * BN, js = j0 + 16 * lane;
+        int page = -1;
+        if (lane < BN / 16 && js < end) {
+          page = __ldg(c.table + (int64_t)w.b * c.ts + (js >> c.shift));
+          if ((unsigned)page >= (unsigned)c.n_pages) {
+            page = -1;
+            if (js + 16 > w.first || js < w.head) {      // (a page that no row sees may be gone)
+              kv_fail(c, kErrPrompt);
+              s_bad = 1;
             }
           }
-          if (!ok) break;
-          mma_commit(&s_free[vs]);
-          if (more) mma_commit(&s_free[ks]);
-        } else {
-          if (j + 1 < w.nmax) {
-            if (!wait(&s_full[slot], phase)) break;
+        }
+        const uint32_t have = __ballot_sync(0xFFFFFFFFu, page >= 0);
+        const bool fix = is_v && (have != (1u << BN / 16) - 1 || j0 + BN > w.len);
+        uint64_t* bar = fix ? &s_fix : &s_full[slot];
+        auto groups = [&](int u) { return have >> (u * per) & ((1u << per) - 1); };   // of box u
+        uint32_t bytes = 0;
+        for (int u = 0; u < BN / box; ++u) bytes += groups(u) ? box * HD * 2 : 0;
+        if (lane == 0) mbar_expect_tx(bar, bytes);
+        __syncwarp();
+        uint8_t* dst = s_kv + slot * Sh::kMat;
+        const int boxes = BN / box * (HD / 64), x = min(lane, boxes - 1), u = x / (HD / 64), half = x - u * (HD / 64);
+        const uint32_t here = groups(u);
+        const int pg = __shfl_sync(0xFFFFFFFFu, page, here ? u * per + __ffs(here) - 1 : 0);
+        if (here && lane < boxes)
+          tma_load_4d(smem_u32(dst) + half * BN * 128 + u * box * 128, is_v ? &maps.v : &maps.k, 64 * half,
+                      (j0 + u * box) & ((1 << c.shift) - 1), w.kvh, pg, bar);
+        if (fix) {
+          const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_fix, fixes & 1, c.err, kErrPromptWait));
+          ++fixes;
+          if (!ok) return false;
+          for (int r = 0; r < BN; ++r)
+            if (!(have >> (r >> 4) & 1) || j0 + r >= w.len)
+              for (int y = lane; y < HD / 8; y += 32)
+                *reinterpret_cast<uint4*>(dst + (y >> 3) * BN * 128 + r * 128 + (y & 7) * 16) = make_uint4(0, 0, 0, 0);
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_full[slot]);
+        }
+        ++issued;
+        if (++slot == Sh::kSlots) { slot = 0; phase ^= 1; }
+        return true;
+      };
+      bool ok = w.nmax == 0 || load(0, false);
+      for (int j = 0; ok && j < w.nmax; ++j) {
+        // in the order of use: with two tiles V(j), K(j + 1); with one K(j + 1), V(j)
+        if (NT == 2) ok = load(j, true) && (j + 1 == w.nmax || load(j + 1, false));
+        else ok = (j + 1 == w.nmax || load(j + 1, false)) && load(j, true);
+      }
+      if (!ok) s_dead = 1;
+      // no copy is in flight when the block ends: the last use of every slot has arrived
+      for (int k = 0; k < Sh::kSlots && k < issued; ++k) {
+        if (--slot < 0) { slot = Sh::kSlots - 1; phase ^= 1; }
+        mbar_wait(&s_full[slot], phase, c.err, kErrPromptWait);
+      }
+    } else if (warp == kMma) {
+      asm volatile("bar.sync 1, %0;" ::"n"(128 * NT + 32) : "memory");       // Q is in shared memory
+      tc_fence_after();
+      if (lane == 0) {
+        constexpr bool bf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
+        constexpr uint32_t id_s = idesc_f16(kRows, BN, bf16, false), id_o = idesc_f16(kRows, HD, bf16, true);
+        int slot = 0, phase = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, int parity) { return ok = ok && mbar_wait(bar, parity, c.err, kErrPromptWait, a.spin); };
+        auto next = [&] {
+          if (++slot == Sh::kSlots) { slot = 0; phase ^= 1; }
+        };
+        // S = Q K^T of tile t with the keys in `at`, into buffer `buf`
+        auto scores = [&](int t, int at, int buf) {
+          const uint32_t q = smem_u32(s_q) + t * Sh::kQ, k = smem_u32(s_kv) + at * Sh::kMat;
+#pragma unroll
+          for (int x = 0; x < HD / 16; ++x)
+            mma_f16(tmem + Sh::kS + buf * BN, sdesc_k128(q + (x >> 2) * kRows * 128) + 2 * (x & 3),
+                    sdesc_k128(k + (x >> 2) * BN * 128) + 2 * (x & 3), id_s, x > 0);
+          mma_commit(&s_sfull[buf]);
+        };
+        auto values = [&](int t, int at, int buf, bool more) {
+          const uint32_t v = smem_u32(s_kv) + at * Sh::kMat;
+#pragma unroll
+          for (int x = 0; x < BN / 16; ++x)
+            mma_f16_ta(tmem + Sh::kO + t * HD, tmem + Sh::kS + buf * BN + 8 * x, sdesc_mn128(v + x * 2048, BN * 128), id_o,
+                       more || x > 0);
+          mma_commit(&s_odone[t]);
+        };
+        if (w.nmax && wait(&s_full[0], 0)) {
+          tc_fence_after();
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            if (w.nb[t]) scores(t, 0, t);
+          mma_commit(&s_free[0]);
+          next();
+        }
+        for (int j = 0; ok && j < w.nmax; ++j) {
+          if constexpr (NT == 2) {
+            const int vs = slot, vph = phase;
+            next();
+            const int ks = slot, kph = phase;
+            const bool more = j + 1 < w.nmax;
+            if (more) next();
+            bool have_v = false, have_k = false;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (j >= w.nb[t]) continue;
+              if (!have_v && !wait(&s_full[vs], vph)) break;
+              have_v = true;
+              if (!wait(&s_pfull[t], j & 1)) break;
+              tc_fence_after();
+              values(t, vs, t, j > 0);
+              if (t == 1 || j >= w.nb[1]) mma_commit(&s_free[vs]);       // the last tile that reads it
+              if (j + 1 < w.nb[t]) {
+                if (!have_k && !wait(&s_full[ks], kph)) break;
+                have_k = true;
+                scores(t, ks, t);
+              }
+            }
+            if (!ok) break;
+            if (more) mma_commit(&s_free[ks]);
+          } else {
+            if (j + 1 < w.nmax) {
+              if (!wait(&s_full[slot], phase)) break;
+              tc_fence_after();
+              scores(0, slot, (j + 1) & 1);
+              mma_commit(&s_free[slot]);
+              next();
+            }
+            if (!wait(&s_full[slot], phase) || !wait(&s_pfull[j & 1], j >> 1 & 1)) break;
             tc_fence_after();
-            scores(0, slot, (j + 1) & 1);
+            values(0, slot, j & 1, j > 0);
             mma_commit(&s_free[slot]);
             next();
           }
-          if (!wait(&s_full[slot], phase) || !wait(&s_pfull[j & 1], j >> 1 & 1)) break;
-          tc_fence_after();
-          values(0, slot, j & 1, j > 0);
-          mma_commit(&s_free[slot]);
-          next();
         }
+        if (!ok) s_dead = 1;
+        mma_commit(&s_end);                          // nothing this thread issued is still running when the block ends
+        mbar_wait(&s_end, 0, c.err, kErrPromptWait);
       }
-      if (!ok) s_dead = 1;
-      mma_commit(&s_end);                          // nothing this thread issued is still running when the block ends
-      mbar_wait(&s_end, 0, c.err, kErrPromptWait);
+      __syncwarp();
     }
-    __syncwarp();
+    __syncthreads();
+    __syncthreads();                               // the outputs are out of TMEM
+    tc_fence_after();
+    if (warp == kMma) tmem_dealloc(tmem, 512);
+    return;
   }
 
   // ---- softmax: thread = row
+  if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
   const int t = NT == 2 ? warp >> 2 : 0, r = threadIdx.x & 127;
+  // (this tile's entries by selection: an index known only at run time would put them into local memory)
+  const int w_tok = t ? w.tok[1] : w.tok[0], w_ntok = t ? w.ntok[1] : w.ntok[0], w_end = t ? w.end[1] : w.end[0],
+            n = t ? w.nb[1] : w.nb[0];
   const uint32_t lanes = (uint32_t)(warp & 3) << 21;                     // this warp's TMEM lanes, 32 (warp % 4) on
   const int tok = r / w.hb, h = w.h0 + r - tok * w.hb;
-  const bool mine = warp < kProducer && tok < w.ntok[t];
-  const int p = mine ? w.len - w.n + w.tok[t] + tok : -1;
+  const bool mine = tok < w_ntok;
+  const int p = mine ? w.len - w.n + w_tok + tok : -1;
   float l = 0.0f;
-  if (warp < kProducer) {
-    // the query rows into shared memory (16-byte pieces, 128-byte swizzle); a negative scale goes into their signs
-    const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
-    for (int x = r; x < kRows * HD / 8; x += 128) {
-      const int row = x / (HD / 8), e = x - row * (HD / 8), rt = row / w.hb;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (rt < w.ntok[t]) {
-        v = __ldg(reinterpret_cast<const uint4*>(a.q + 2 * ((int64_t)(w.row0 + w.tok[t] + rt) * a.qr +
-                                                             (int64_t)(w.h0 + row - rt * w.hb) * a.qh + 8 * e)));
-        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-      }
-      *reinterpret_cast<uint4*>(s_q + t * Sh::kQ + (e >> 3) * kRows * 128 + row * 128 + (((e & 7) ^ (row & 7)) << 4)) = v;
+  // the query rows into shared memory (16-byte pieces, 128-byte swizzle); a negative scale goes into their signs
+  const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
+  for (int x = r; x < kRows * HD / 8; x += 128) {
+    const int row = x / (HD / 8), e = x - row * (HD / 8), rt = row / w.hb;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (rt < w_ntok) {
+      v = __ldg(reinterpret_cast<const uint4*>(a.q + 2 * ((int64_t)(w.row0 + w_tok + rt) * a.qr +
+                                                           (int64_t)(w.h0 + row - rt * w.hb) * a.qh + 8 * e)));
+      v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
     }
-    fence_async_shared();
-    asm volatile("bar.sync 1, %0;" ::"n"(128 * NT + 32) : "memory");
-    const float scale2 = fabsf(a.scale2);
-    const int pmin = w.len - w.n + w.tok[t], pmax = w.end[t] - 1, n = w.nb[t];
-    const int from = first_in_window(p + 1, a.window);
-    float m = neg_inf();
-    bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      const int buf = NT == 2 ? t : j & 1, ph = NT == 2 ? j & 1 : j >> 1 & 1;
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_sfull[buf], ph, c.err, kErrPromptWait, a.spin));
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t st = tmem + lanes + Sh::kS + buf * BN;
-      uint32_t v[BN];
+    *reinterpret_cast<uint4*>(s_q + t * Sh::kQ + (e >> 3) * kRows * 128 + row * 128 + (((e & 7) ^ (row & 7)) << 4)) = v;
+  }
+  fence_async_shared();
+  asm volatile("bar.sync 1, %0;" ::"n"(128 * NT + 32) : "memory");
+  const float scale2 = fabsf(a.scale2);
+  const int pmin = w.len - w.n + w_tok, pmax = w_end - 1;
+  const int from = first_in_window(p + 1, a.window);
+  float m = neg_inf();
+  bool ok = true;
+  for (int j = 0; j < n; ++j) {
+    const int buf = NT == 2 ? t : j & 1, ph = NT == 2 ? j & 1 : j >> 1 & 1;
+    ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_sfull[buf], ph, c.err, kErrPromptWait, a.spin));
+    if (!ok) break;
+    tc_fence_after();
+    const uint32_t st = tmem + lanes + Sh::kS + buf * BN;
+    uint32_t v[BN];
 #pragma unroll
-      for (int x = 0; x < BN; x += 32) tmem_ld32(st + x, v + x);
-      tmem_wait_ld();
+    for (int x = 0; x < BN; x += 32) tmem_ld32(st + x, v + x);
+    tmem_wait_ld();
 #pragma unroll
-      for (int x = 0; x < BN; ++x) asm volatile("" : "+r"(v[x]));        // no use moves before the wait
-      const int j0 = w.block(j) * BN;
-      if (j0 + BN - 1 > pmin || (pmax - j0 >= a.window && j0 + BN > a.sinks)) {
-        const int hi = p + 1 - j0, lo = from - j0, sk = a.sinks - j0;
+    for (int x = 0; x < BN; ++x) asm volatile("" : "+r"(v[x]));        // no use moves before the wait
+    const int j0 = w.block(j) * BN;
+    if (j0 + BN - 1 > pmin || (pmax - j0 >= a.window && j0 + BN > a.sinks)) {
+      const int hi = p + 1 - j0, lo = from - j0, sk = a.sinks - j0;
 #pragma unroll
-        for (int x = 0; x < BN; ++x)
-          if (!(x < hi && (x >= lo || x < sk))) v[x] = 0xFF800000u;
-      }
-      float mx[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+      for (int x = 0; x < BN; ++x)
+        if (!(x < hi && (x >= lo || x < sk))) v[x] = 0xFF800000u;
+    }
+    float mx[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
-      for (int x = 0; x < BN; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
-      const bool grow = top > m + 8.0f || (m == neg_inf() && top > m);
-      if (__any_sync(0xFFFFFFFFu, grow)) {
-        const float f = grow ? ex2(m - top) : 1.0f;
-        if (grow) m = top;
-        l *= f;
-        if (j > 0) {
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_odone[t], (j - 1) & 1, c.err, kErrPromptWait, a.spin));
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t ot = tmem + lanes + Sh::kO + t * HD;
+    for (int x = 0; x < BN; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x]));
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+    const bool grow = top > m + 8.0f || (m == neg_inf() && top > m);
+    if (__any_sync(0xFFFFFFFFu, grow)) {
+      const float f = grow ? ex2(m - top) : 1.0f;
+      if (grow) m = top;
+      l *= f;
+      if (j > 0) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_odone[t], (j - 1) & 1, c.err, kErrPromptWait, a.spin));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ot = tmem + lanes + Sh::kO + t * HD;
 #pragma unroll
-          for (int x = 0; x < HD; x += 32) {
-            uint32_t o[32];
-            tmem_ld32(ot + x, o);
-            tmem_wait_ld();
+        for (int x = 0; x < HD; x += 32) {
+          uint32_t o[32];
+          tmem_ld32(ot + x, o);
+          tmem_wait_ld();
 #pragma unroll
-            for (int y = 0; y < 32; ++y) {
-              asm volatile("" : "+r"(o[y]));
-              o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-            }
-            tmem_st32(ot + x, o);
+          for (int y = 0; y < 32; ++y) {
+            asm volatile("" : "+r"(o[y]));
+            o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
           }
+          tmem_st32(ot + x, o);
         }
       }
-      const float base = m == neg_inf() ? 0.0f : m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int x = 0; x < BN; x += 2) {
-        const float p0 = ex2(fmaf(__uint_as_float(v[x]), scale2, -base)), p1 = ex2(fmaf(__uint_as_float(v[x + 1]), scale2, -base));
-        sum[x >> 1 & 3] += p0 + p1;
-        v[x >> 1] = Elem<T>::pack(p0, p1);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-      for (int x = 0; x < BN / 2; x += 32) tmem_st32(st + x, v + x);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_pfull[buf]);
     }
-    if (ok && n) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_odone[t], (n - 1) & 1, c.err, kErrPromptWait, a.spin));
-    if (!ok) s_dead = 1;
+    const float base = m == neg_inf() ? 0.0f : m;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int x = 0; x < BN; x += 2) {
+      const float p0 = ex2(fmaf(__uint_as_float(v[x]), scale2, -base)), p1 = ex2(fmaf(__uint_as_float(v[x + 1]), scale2, -base));
+      sum[x >> 1 & 3] += p0 + p1;
+      v[x >> 1] = Elem<T>::pack(p0, p1);
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int x = 0; x < BN / 2; x += 32) tmem_st32(st + x, v + x);
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s_pfull[buf]);
   }
+  if (ok && n) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_odone[t], (n - 1) & 1, c.err, kErrPromptWait, a.spin));
+  if (!ok) s_dead = 1;
   __syncthreads();
   tc_fence_after();
-  if (warp < kProducer && !s_dead) {
+  if (!s_dead) {
     const bool any = p >= 0;
     const float inv = any ? 1.0f / l : 0.0f;
     bool good = true;
-    const int64_t row = w.row0 + w.tok[t] + tok;
+    const int64_t row = w.row0 + w_tok + tok;
     uint8_t* to = a.out + 2 * (row * a.orow + (int64_t)h * a.oh);
 #pragma unroll
     for (int x = 0; x < HD; x += 32) {
       uint32_t o[32];
-      if (w.nb[t]) {
+      if (n) {
         tmem_ld32(tmem + lanes + Sh::kO + t * HD + x, o);
         tmem_wait_ld();
       }
@@ -435,7 +448,6 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kMma) tmem_dealloc(tmem, 512);
 }
 
 template <class T, int HD>
