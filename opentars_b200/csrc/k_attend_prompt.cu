@@ -58,6 +58,12 @@ struct Work {
   __device__ __forceinline__ int block(int j) const { return j < na ? j : t0 + j - na; }
 };
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+
 template <class T, int HD>
 __device__ __noinline__ void redo_row(const AttendArgs& a, int b, int kvh, int64_t row, int h, int end) {
   float q[HD / 32], o[HD / 32];
@@ -326,15 +332,26 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   float l = 0.0f;
   // the query rows into shared memory (16-byte pieces, 128-byte swizzle); a negative scale goes into their signs
   const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
-  for (int x = r; x < kRows * HD / 8; x += 128) {
-    const int row = x / (HD / 8), e = x - row * (HD / 8), rt = row / w.hb;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (rt < w_ntok) {
-      v = __ldg(reinterpret_cast<const uint4*>(a.q + 2 * ((int64_t)(w.row0 + w_tok + rt) * a.qr +
-                                                           (int64_t)(w.h0 + row - rt * w.hb) * a.qh + 8 * e)));
-      v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+  // A warp copies its 32 rows, consecutive lanes consecutive pieces; rows without a token read as zeros
+  constexpr int kPieces = HD / 8, kLanes = kPieces < 32 ? kPieces : 32, kAtOnce = 32 / kLanes;
+  const int64_t row = w.row0 + w_tok + tok;
+  const int64_t from_q = 2 * (mine ? row * a.qr + (int64_t)h * a.qh : 0);
+  const uint32_t live = __ballot_sync(0xFFFFFFFFu, mine);
+#pragma unroll 8
+  for (int x = 0; x < 32; x += kAtOnce) {
+    const int lr = x + lane / kLanes, rr = (warp & 3) * 32 + lr, piece = lane % kLanes;
+    const uint32_t to = smem_u32(s_q) + t * Sh::kQ + (piece >> 3) * kRows * 128 + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to),
+                 "l"(a.q + __shfl_sync(0xFFFFFFFFu, from_q, lr) + 16 * piece), "r"(live >> lr & 1 ? 16 : 0)
+                 : "memory");
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (flip) {
+    __syncwarp();
+    for (int x = 0; x < kPieces; ++x) {
+      uint4* v = reinterpret_cast<uint4*>(s_q + t * Sh::kQ + (x >> 3) * kRows * 128 + r * 128 + (x & 7) * 16);
+      v->x ^= flip; v->y ^= flip; v->z ^= flip; v->w ^= flip;
     }
-    *reinterpret_cast<uint4*>(s_q + t * Sh::kQ + (e >> 3) * kRows * 128 + row * 128 + (((e & 7) ^ (row & 7)) << 4)) = v;
   }
   fence_async_shared();
   asm volatile("bar.sync 1, %0;" ::"n"(128 * NT + 32) : "memory");
@@ -364,7 +381,7 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
     }
     float mx[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
-    for (int x = 0; x < BN; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x]));
+    for (int x = 0; x < BN; x += 2) mx[x >> 1 & 3] = max3(mx[x >> 1 & 3], __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
     const bool grow = top > m + 8.0f || (m == neg_inf() && top > m);
     if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -414,8 +431,9 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
     const bool any = p >= 0;
     const float inv = any ? 1.0f / l : 0.0f;
     bool good = true;
-    const int64_t row = w.row0 + w_tok + tok;
-    uint8_t* to = a.out + 2 * (row * a.orow + (int64_t)h * a.oh);
+    // the warp's rows go out through the query tile's place (no tensor core reads it any more), so
+    // that consecutive lanes store consecutive pieces of a row
+    uint8_t* mine_at = s_q + t * Sh::kQ + r * 128;
 #pragma unroll
     for (int x = 0; x < HD; x += 32) {
       uint32_t o[32];
@@ -431,11 +449,22 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
         good &= fabsf(o0) + fabsf(o1) < __int_as_float(0x7F800000);
         pk[y >> 1] = Elem<T>::pack(o0, o1);
       }
-      if (mine) {
 #pragma unroll
-        for (int y = 0; y < 16; y += 4)
-          *reinterpret_cast<uint4*>(to + 2 * x + 4 * y) = make_uint4(pk[y], pk[y + 1], pk[y + 2], pk[y + 3]);
+      for (int y = 0; y < 4; ++y) {
+        const int piece = x / 8 + y;
+        *reinterpret_cast<uint4*>(mine_at + (piece >> 3) * kRows * 128 + (((piece & 7) ^ (r & 7)) << 4)) =
+            make_uint4(pk[4 * y], pk[4 * y + 1], pk[4 * y + 2], pk[4 * y + 3]);
       }
+    }
+    __syncwarp();
+    const int64_t to_out = 2 * (mine ? row * a.orow + (int64_t)h * a.oh : 0);
+#pragma unroll 8
+    for (int x = 0; x < 32; x += kAtOnce) {
+      const int lr = x + lane / kLanes, rr = (warp & 3) * 32 + lr, piece = lane % kLanes;
+      const int64_t to = __shfl_sync(0xFFFFFFFFu, to_out, lr) + 16 * piece;
+      if (live >> lr & 1)
+        *reinterpret_cast<uint4*>(a.out + to) = *reinterpret_cast<const uint4*>(
+            s_q + t * Sh::kQ + (piece >> 3) * kRows * 128 + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4));
     }
     __syncwarp();
     uint32_t redo = __ballot_sync(0xFFFFFFFFu, mine && any && (!good || s_bad));
