@@ -11,8 +11,8 @@
  * TC_ERR_CUDA. What only the device can see is checked there, and the first code found stays in
  * the word that tc_wait_error reads: 51 append, 52 attend, 53 attend_prompt, 54 evict - a page id
  * outside the pool or a length beyond the page list. A key on such a page is left out of the
- * attention, a row for it is not written, a length counts up to the page list's end. 55 (attend)
- * and 56 (attend_prompt) are bounded waits that gave up, as tc_wait_error describes.
+ * attention, a row for it is not written, a length counts up to the page list's end. 55
+ * (attend_prompt) is a bounded wait that gave up, as tc_wait_error describes.
  */
 #ifndef TARSCUDA_SERVE_H
 #define TARSCUDA_SERVE_H

@@ -1,17 +1,19 @@
 // Attention of one query row per sequence over the paged cache (tc_attend).
 //
-// The G = n_heads / n_kv heads of a key-value head read the same rows, so they are the rows of one
-// warp MMA (m16n8k16; more than 16 go in blocks of 16): each key and value row crosses HBM once and the
-// kernel is bound by that stream. The work of a call is one list of tiles of 64 slots - sequence by
-// sequence, key-value head by key-value head, only tiles with a visible slot - cut into equal runs,
-// one per CTA and one CTA per SM: ragged batches and a single long sequence fill the GPU alike. Every
-// CTA derives its run from the lengths (a scan of the batch); nothing is planned on the host.
-//   warp 4     producer: the tile's key and value rows by TMA (64 x page rows boxes, 128-byte
-//              swizzle) into a ring of stages; a lane per box
-//   warps 0-3  16 of a tile's 64 slots each, with running maximum, sum and output of their own:
-//              S = Q K^T from ldmatrix, p = 2^(s - m), O += P V with P split in two 16-bit parts (the
-//              probabilities keep 16 bits and more at the price of MMAs that the memory bound hides)
-// At an item's end the four warps' states are joined through shared memory. An item that lies in one
+// The G = n_heads / n_kv heads of a key-value head read the same rows, so they are the columns of one
+// warp MMA (m16n8k16: 16 slots x 8 heads; blocks of 8 or 16 heads): each key and value row crosses HBM
+// once and the kernel is bound by that stream. The work of a call is one list of chunks of 16 slots -
+// sequence by sequence, key-value head by key-value head, only chunks with a visible slot - cut into
+// equal runs, one per CTA and one CTA per SM: ragged batches and a single long sequence fill the GPU
+// alike. Every CTA derives its run from the lengths (a scan of the batch); nothing is planned on the
+// host. The warps of a CTA take the chunks of its run in turn, each with a ring of its own that it fills
+// by cp.async (16-byte pieces, hidden rows as zeros: 0 x NaN is not 0) and a running maximum, sum and
+// output of its own, so no warp waits for another within an item:
+//   S^T = K Q^T (ldmatrix), p = 2^(s - m), O^T += V^T P^T (ldmatrix.trans) with P split in two 16-bit
+//   parts: the probabilities keep 16 bits and more at the price of MMAs that the memory bound hides
+// (Boxes of TMA over 16-slot pages were tried in place of cp.async: 3.46 against 4.84 TB/s with
+// 64-slot pages, the boxes of 2 KB being the limit.)
+// At an item's end the warps' states are joined through shared memory. An item that lies in one
 // CTA's run is stored at once; of the others every CTA writes its state (maximum, sum, 16 x HD fp32)
 // to the workspace, and k_join, launched early as a dependent, combines them in run order: no atomics,
 // the same bits every time.
@@ -21,22 +23,21 @@
 
 #include "attend_row.cuh"
 #include "mma.h"
-#include "paged_map.h"
 #include "pdl.cuh"
 #include "umma.cuh"
 
 namespace tc {
 namespace {
 
-constexpr int kTile = 64, kConsumers = 4, kAttendThreads = 32 * (kConsumers + 1), kRowsMma = 16, kMaxGrid = 148;
+constexpr int kTile = 16, kRowsMma = 16, kMaxGrid = 148;
 
 template <int HD>
 struct AttendShape {
-  static constexpr int kHalves = HD / 64;                    // 128-byte column groups of a row
-  static constexpr int kMat = kTile * HD * 2;                // bytes of a tile's keys (or values)
-  static constexpr int kStages = HD == 64 ? 8 : HD == 128 ? 5 : 3;
-  static constexpr int kJoin = 2 * kRowsMma * HD * 4;        // two warps' outputs
-  static constexpr int kSmem = 1024 + kStages * 2 * kMat + kJoin;
+  // a warp's ring: kStages chunks of keys and values
+  static constexpr int kWarps = HD == 256 ? 4 : 8, kThreads = 32 * kWarps, kStages = HD == 64 ? 5 : 3;
+  static constexpr int kMat = kTile * HD * 2, kRing = kStages * 2 * kMat;
+  static constexpr int kSlot = 8 * (HD + 4);                 // floats of a warp's outputs of 8 heads, rows padded
+  static constexpr int kSmem = kWarps * (kRing + kSlot * 4);
   static constexpr int kPart = kRowsMma * HD + 2 * kRowsMma; // floats of a CTA's state of an item
 };
 
@@ -61,9 +62,11 @@ struct PlanShared {
   long long into;
   int b;
 };
-// The tiles of the whole call are cut into runs of total / runs (rounded down) and one more; there are
-// never more runs than tiles, so none is empty.
-__device__ __forceinline__ int runs_of(long long total, int grid) { return (int)min(total, (long long)grid); }
+// The tiles of the whole call are cut into runs of total / runs (rounded down) or one more; there are
+// no more runs than leave every warp of a CTA a tile, so none is empty.
+__device__ __forceinline__ int runs_of(long long total, int grid, int warps) {
+  return (int)min((total + warps - 1) / warps, (long long)grid);
+}
 __device__ __forceinline__ long long run_begin(long long total, int runs, int i) { return total * i / runs; }
 // The run that holds tile t: the last one that begins at or before it.
 __device__ __forceinline__ int run_of(long long total, int runs, long long t) { return (int)(((t + 1) * runs - 1) / total); }
@@ -72,7 +75,7 @@ __device__ __forceinline__ int run_of(long long total, int runs, long long t) { 
 // tiles before sequence `want`; or, want < 0, s.b = the sequence that holds the first tile of run
 // `run` and the tiles of it before that one.
 __device__ __forceinline__ long long plan(const AttendArgs& a, int nsub, PlanShared& s, int want, int run, int grid,
-                                          long long* before) {
+                                          int warps, long long* before) {
   const int T = blockDim.x, t = threadIdx.x, B = a.c.batch, per = (B + T - 1) / T;
   const int lo = min(B, t * per), hi = min(B, lo + per), warp = t >> 5, lane = t & 31;
   long long mine = 0;
@@ -91,7 +94,7 @@ __device__ __forceinline__ long long plan(const AttendArgs& a, int nsub, PlanSha
     total += s.warp[w];
   }
   long long at = base + sum - mine;                          // tiles before this thread's sequences
-  const int runs = runs_of(total, grid);
+  const int runs = runs_of(total, grid, warps);
   const long long find = want < 0 && run < runs ? run_begin(total, runs, run) : total;
   if (want < 0 ? mine && find >= at && find < at + mine : want >= lo && want < hi) {
     int b = lo;
@@ -136,9 +139,6 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (
 // The factor a state kept at maximum m takes at maximum m2 >= m (1 where both are still -infinity).
 __device__ __forceinline__ float shrink(float m, float m2) { return m2 == neg_inf() ? 1.0f : ex2(m - m2); }
 
-struct AttendMaps {
-  CUtensorMap k, v;
-};
 // What a call keeps in its workspace: the CTAs' states, the scores and the final statistics.
 struct AttendWs {
   float* part;
@@ -148,328 +148,291 @@ struct AttendWs {
   int64_t cap;                       // slots a row of scores holds
 };
 
-// A warp's running state over its slots: rows r = lane / 4 and r + 8 of the head block.
-template <int HD>
-struct State {
-  float o[HD / 8][4];
-  float m[2], l[2];                  // l: this lane's share of the row's sum
-  bool any;                          // a visible slot was met
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
-    m[0] = m[1] = neg_inf();
-    l[0] = l[1] = 0.0f;
-    any = false;
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// The parts of items that a CTA's run consists of, one after the other: chunks [i0, i1) of an item.
+struct Walk {
+  int left, b, sub, i0, i1;          // left: chunks of the run from this part on
+  SeqTiles sq;
+  __device__ __forceinline__ Walk(const AttendArgs& a, int left_, int b_, int sub_, int first)
+      : left(left_), b(b_), sub(sub_), i0(first), i1(0), sq(a, b_) {
+    i1 = min(sq.nt, first + left);
   }
-  __device__ __forceinline__ void scale(float f0, float f1) {
-#pragma unroll
-    for (int n = 0; n < HD / 8; ++n) {
-      o[n][0] *= f0; o[n][1] *= f0;
-      o[n][2] *= f1; o[n][3] *= f1;
+  __device__ __forceinline__ bool next(const AttendArgs& a, int nsub) {
+    left -= i1 - i0;
+    if (left <= 0) return false;
+    if (++sub == nsub) {
+      sub = 0;
+      do sq = SeqTiles(a, ++b);
+      while (sq.nt == 0);
     }
-    l[0] *= f0;
-    l[1] *= f1;
+    i0 = 0;
+    i1 = min(sq.nt, left);
+    return true;
   }
 };
 
-template <class T, int HD>
-__global__ void __launch_bounds__(kAttendThreads, 1)
-    k_attend(const __grid_constant__ AttendMaps maps, const __grid_constant__ AttendArgs a, AttendWs ws, int rows_box) {
+template <class T, int HD, int NB>
+__global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
+    k_attend(const __grid_constant__ AttendArgs a, AttendWs ws, int gblocks, int hb) {
   using Sh = AttendShape<HD>;
-  extern __shared__ uint8_t s_raw[];
-  __shared__ __align__(8) uint64_t s_full[Sh::kStages], s_free[Sh::kStages];
-  __shared__ uint32_t s_valid[Sh::kStages];
-  __shared__ float s_ml[kConsumers][2][kRowsMma];
+  constexpr int W = Sh::kWarps, S = Sh::kStages, kPieces = HD / 8;
+  extern __shared__ __align__(16) uint8_t s_raw[];
+  __shared__ float s_m[W][kRowsMma], s_l[W][kRowsMma];
   __shared__ PlanShared s_plan;
-  __shared__ int s_dead;
   griddep_launch();                               // k_join may take its place and wait
   const KvCache& c = a.c;
-  uint8_t* s_tiles = s_raw + (1024 - (smem_u32(s_raw) & 1023)) % 1024;
-  float* s_join = reinterpret_cast<float*>(s_tiles + Sh::kStages * 2 * Sh::kMat);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < Sh::kStages; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], kConsumers);
-    }
-    mbar_fence_init();
-    s_dead = 0;
-  }
-  const int G = a.nh / c.n_kv, gblocks = (G + kRowsMma - 1) / kRowsMma, nsub = c.n_kv * gblocks;
+  const int G = a.nh / c.n_kv, nsub = c.n_kv * gblocks;
   long long into = 0;
-  const long long total = plan(a, nsub, s_plan, -1, blockIdx.x, gridDim.x, &into);   // (also orders the barriers' setup)
-  const int runs = runs_of(total, gridDim.x);
+  const long long total = plan(a, nsub, s_plan, -1, blockIdx.x, gridDim.x, W, &into);
+  const int runs = runs_of(total, gridDim.x, W);
   if ((int)blockIdx.x >= runs) return;
-  int b = s_plan.b, left = (int)(run_begin(total, runs, blockIdx.x + 1) - run_begin(total, runs, blockIdx.x));
-  SeqTiles sq(a, b);
-  int sub = (int)(into / sq.nt), i = (int)(into - (long long)sub * sq.nt);
-  int stage = 0, phase = 0;
-  if (warp == kConsumers) {
-    int issued = 0;
-    bool dead = false;
-    for (; left > 0 && !dead; --left) {
-      const int kvh = sub / gblocks, j0 = sq.tile(i) * kTile;
-      // one lane per box: rows_box slots of one 64-column group of the keys or the values
-      const int chunks = kTile / rows_box, boxes = 2 * chunks * Sh::kHalves;
-      bool ok = issued < Sh::kStages || mbar_wait(&s_free[stage], phase ^ 1, c.err, kErrAttendWait, a.spin);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) {
-        dead = true;
-        break;
-      }
-      // 16-slot groups with a visible slot on a page of the pool; a box is loaded if it has one
-      uint32_t mine = 0;
-      int page = -1;
-      if (lane < 4) {
-        const int j = j0 + 16 * lane;
-        const bool seen = j < sq.len && (j + 16 > sq.first || j < sq.head);
-        if (seen) page = kv_page(c, b, j, kErrAttend);
-        mine = page >= 0;
-      }
-      const uint32_t valid = __ballot_sync(0xFFFFFFFFu, mine);
-      auto groups = [&](int u) { return valid >> (u * rows_box / 16) & ((1u << rows_box / 16) - 1); };   // of box u
-      uint32_t bytes = 0;
-      for (int u = 0; u < chunks; ++u) bytes += groups(u) ? rows_box * HD * 4 : 0;
-      if (lane == 0) {
-        s_valid[stage] = valid;
-        mbar_expect_tx(&s_full[stage], bytes);
-      }
-      __syncwarp();
-      const uint32_t base = smem_u32(s_tiles) + stage * 2 * Sh::kMat;
-      for (int x0 = 0; x0 < boxes; x0 += 32) {
-        const int x = min(x0 + lane, boxes - 1);
-        const int u = x / (2 * Sh::kHalves), r = x - u * 2 * Sh::kHalves, half = r >> 1, is_v = r & 1;
-        const uint32_t here = groups(u);                     // a box lies in one page: that of its first seen group
-        const int pg = __shfl_sync(0xFFFFFFFFu, page, here ? u * rows_box / 16 + __ffs(here) - 1 : 0);
-        if (here && x0 + lane < boxes)
-          tma_load_4d(base + is_v * Sh::kMat + half * kTile * 128 + u * rows_box * 128, is_v ? &maps.v : &maps.k,
-                      64 * half, (j0 + u * rows_box) & ((1 << c.shift) - 1), kvh, pg, &s_full[stage]);
-      }
-      ++issued;
-      if (++stage == Sh::kStages) { stage = 0; phase ^= 1; }
-      if (++i == sq.nt) {
-        i = 0;
-        if (++sub == nsub && left > 1) {
-          sub = 0;
-          do sq = SeqTiles(a, ++b);
-          while (sq.nt == 0);
-        }
-      }
-    }
-    // no copy is in flight when the block ends: the last use of every stage has arrived
-    for (int k = 0; k < Sh::kStages && k < issued; ++k) {
-      if (--stage < 0) { stage = Sh::kStages - 1; phase ^= 1; }
-      mbar_wait(&s_full[stage], phase, c.err, kErrAttendWait);
-    }
-    return;
-  }
+  const int left = (int)(run_begin(total, runs, blockIdx.x + 1) - run_begin(total, runs, blockIdx.x));
+  const int nt0 = SeqTiles(a, s_plan.b).nt, sub0 = (int)(into / nt0), first = (int)(into - (long long)sub0 * nt0);
+  const uint32_t ring = smem_u32(s_raw) + warp * Sh::kRing;
+  float* s_out = reinterpret_cast<float*>(s_raw + W * Sh::kRing);
 
-  bool dead = false;
-  while (left > 0) {
-    const int kvh = sub / gblocks, h0 = kvh * G + (sub - kvh * gblocks) * kRowsMma, rows = min(kRowsMma, (kvh + 1) * G - h0);
-    // the query rows' fragments: rows lane / 4 and + 8, columns 2 (lane % 4) (+ 1, + 8, + 9) of each 16
-    uint32_t q[HD / 16][4];
+  // ---- the copies, S - 1 chunks ahead of their use; a chunk's page is looked up one chunk earlier still
+  Walk pw(a, left, s_plan.b, sub0, first);
+  int pi = first + warp, page = -1, to_slot = 0;
+  uint32_t held = 0;                              // bit x: the chunk copied x copies ago is in the ring
+  bool more = true;
+  auto find = [&] {
+    while (more && pi >= pw.i1) {
+      more = pw.next(a, nsub);
+      pi = pw.i0 + warp;
+    }
+    if (more) page = kv_page(c, pw.b, pw.sq.tile(pi) * kTile, kErrAttend);
+  };
+  auto copy = [&] {
+    held = held << 1 | (more && page >= 0);
+    if (held & 1) {
+      // piece lane % kPieces of the rows lane / kPieces, + 32 / kPieces, ..
+      constexpr int kLanes = kPieces < 32 ? kPieces : 32, kAtOnce = 32 / kLanes;
+      const int j0 = pw.sq.tile(pi) * kTile, piece = lane % kLanes, r0 = lane / kLanes, kvh = pw.sub / gblocks;
+      const int64_t from = 2 * (kv_offset(c, page, j0 + r0, kvh) + 8 * piece), step = 2 * kAtOnce * c.ss;
+      const uint32_t to = ring + to_slot * 2 * Sh::kMat;
 #pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int r = (lane >> 2) + (x & 1) * 8, col = 16 * kk + 2 * (lane & 3) + (x >> 1) * 8;
-        q[kk][x] = 0;
-        if (r < rows)
-          q[kk][x] = __ldg(reinterpret_cast<const uint32_t*>(a.q + 2 * ((int64_t)b * a.qr + (int64_t)(h0 + r) * a.qh + col)));
+      for (int x = 0; x < kTile / kAtOnce; ++x) {
+        const int r = r0 + x * kAtOnce;
+        const uint32_t at = to + r * HD * 2 + ((piece ^ (r & 7)) << 4);
+        const int bytes = pw.sq.visible(j0 + r) ? 16 : 0;     // a hidden row may hold anything: it reads as zeros
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(at), "l"(c.k + from + x * step), "r"(bytes) : "memory");
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(at + Sh::kMat), "l"(c.v + from + x * step), "r"(bytes) : "memory");
       }
-    State<HD> st;
-    st.clear();
-    const int i0 = i, n = min(left, sq.nt - i);
-    for (int k = 0; k < n; ++k, ++i) {
-      if (!dead) dead = !__all_sync(0xFFFFFFFFu, mbar_wait(&s_full[stage], phase, c.err, kErrAttendWait, a.spin));
-      if (!dead && (s_valid[stage] >> warp & 1)) {
-        const int j0 = sq.tile(i) * kTile + 16 * warp;
-        const uint32_t kt = smem_u32(s_tiles) + stage * 2 * Sh::kMat + 16 * warp * 128, vt = kt + Sh::kMat;
-        st.any = true;
-        const bool whole = j0 + 16 <= sq.len && (j0 >= sq.first || j0 + 16 <= sq.head);
-        float s[2][4] = {};
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++to_slot == S) to_slot = 0;
+    pi += W;
+    find();
+  };
+  find();
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          // matrices: slots 0-7 | 8-15 x columns 0-7 | 8-15
-          const int r = (lane & 7) + (lane >> 4) * 8, c16 = (kk & 3) * 2 + (lane >> 3 & 1);
-          uint32_t f[4];
-          ldsm4(kt + (kk >> 2) * kTile * 128 + r * 128 + ((c16 ^ (r & 7)) << 4), f);
-          mma16816<T>(s[0], q[kk], f[0], f[1]);
-          mma16816<T>(s[1], q[kk], f[2], f[3]);
+  for (int x = 0; x < S - 1; ++x) copy();
+
+  Walk w(a, left, s_plan.b, sub0, first);
+  int slot = 0;
+  do {
+    const int kvh = w.sub / gblocks, g0 = (w.sub - kvh * gblocks) * hb, h0 = kvh * G + g0, rows = min(hb, G - g0);
+    // the query rows as the MMA's second operand: head lane / 4, columns 2 (lane % 4) (+ 1, + 8, + 9) of each 16
+    uint32_t q[NB][HD / 16][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int r = 8 * nb + (lane >> 2), col = 16 * kk + 2 * (lane & 3) + 8 * x;
+          q[nb][kk][x] = 0;
+          if (r < rows)
+            q[nb][kk][x] = __ldg(reinterpret_cast<const uint32_t*>(a.q + 2 * ((int64_t)w.b * a.qr + (int64_t)(h0 + r) * a.qh + col)));
         }
-        bool show[2][2];
+    // this warp's state: rows (lane / 4, + 8) of each 16 columns of O^T, heads 2 (lane % 4) (+ 1) of each block of 8
+    float o[HD / 16][NB][4], m[NB][2], l[NB][2];
+    bool any = false;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+    for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) show[t][e] = whole || sq.visible(j0 + 8 * t + 2 * (lane & 3) + e);
+      for (int x = 0; x < HD / 16; ++x)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int e = 0; e < 4; ++e) o[x][nb][e] = 0.0f;
+      m[nb][0] = m[nb][1] = neg_inf();
+      l[nb][0] = l[nb][1] = 0.0f;
+    }
+    for (int i = w.i0 + warp; i < w.i1; i += W) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+      __syncwarp();                               // the chunk is here, and the one before it is used up
+      const uint32_t kt = ring + slot * 2 * Sh::kMat, vt = kt + Sh::kMat;
+      if (++slot == S) slot = 0;
+      copy();
+      const int j0 = w.sq.tile(i) * kTile;
+      if (!(held >> (S - 1) & 1)) continue;       // on a page outside the pool
+      any = true;
+      float s[NB][4], s2[NB][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[t][e] = show[t][e & 1] ? s[t][e] * a.scale2 : neg_inf();
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nb][e] = s2[nb][e] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        // matrices: slots 0-7, 8-15 of columns 0-7, then of columns 8-15
+        const int r = lane & 15, piece = 2 * kk + (lane >> 4);
+        uint32_t f[4];
+        ldsm4(kt + r * HD * 2 + ((piece ^ (r & 7)) << 4), f);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma16816<T>(kk & 1 ? s2[nb] : s[nb], f, q[nb][kk][0], q[nb][kk][1]);
+      }
+      const bool whole = j0 + kTile <= w.sq.len && (j0 >= w.sq.first || j0 + kTile <= w.sq.head);
+      const int r = lane >> 2;
+      const bool show[2] = {whole || w.sq.visible(j0 + r), whole || w.sq.visible(j0 + r + 8)};
+      float top[NB][2];
+      bool grow = false;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nb][e] = show[e >> 1] ? (s[nb][e] + s2[nb][e]) * a.scale2 : neg_inf();
         if (ws.scores) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int r = (lane >> 2) + 8 * y;
-            if (r < rows) {
-              float* to = ws.scores + ((int64_t)b * a.nh + h0 + r) * ws.cap + j0 + 2 * (lane & 3);
-              *reinterpret_cast<float2*>(to) = make_float2(s[0][2 * y], s[0][2 * y + 1]);
-              *reinterpret_cast<float2*>(to + 8) = make_float2(s[1][2 * y], s[1][2 * y + 1]);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const int h = 8 * nb + 2 * (lane & 3) + (e & 1);
+            if (h < rows) ws.scores[((int64_t)w.b * a.nh + h0 + h) * ws.cap + j0 + r + 8 * (e >> 1)] = s[nb][e];
           }
         }
-        if (!whole) {
-          // a hidden slot's value row may hold anything, and 0 x NaN is not 0: it is cleared here
-          for (int r = 0; r < 16; ++r)
-            if (!sq.visible(j0 + r))
-              for (int x = lane; x < HD / 8; x += 32)
-                *reinterpret_cast<uint4*>(s_tiles + stage * 2 * Sh::kMat + Sh::kMat + (x >> 3) * kTile * 128 +
-                                          (16 * warp + r) * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
-          fence_async_shared();
-          __syncwarp();
-        }
-        float m2[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          float m = fmaxf(fmaxf(s[0][2 * y], s[0][2 * y + 1]), fmaxf(s[1][2 * y], s[1][2 * y + 1]));
-          m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-          m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-          m2[y] = fmaxf(st.m[y], m);
-        }
-        if (__any_sync(0xFFFFFFFFu, m2[0] > st.m[0] || m2[1] > st.m[1])) {
-          st.scale(shrink(st.m[0], m2[0]), shrink(st.m[1], m2[1]));
-          st.m[0] = m2[0];
-          st.m[1] = m2[1];
-        }
-        const float at[2] = {m2[0] == neg_inf() ? 0.0f : m2[0], m2[1] == neg_inf() ? 0.0f : m2[1]};
-        float p[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) p[t][e] = show[t][e & 1] ? ex2(s[t][e] - at[e >> 1]) : 0.0f;
-        st.l[0] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
-        st.l[1] += (p[0][2] + p[0][3]) + (p[1][2] + p[1][3]);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float p0 = p[x >> 1][(x & 1) * 2], p1 = p[x >> 1][(x & 1) * 2 + 1];
-          hi[x] = Elem<T>::pack(p0, p1);
-          const float2 f = Elem<T>::f2(hi[x]);
-          lo[x] = Elem<T>::pack(p0 - f.x, p1 - f.y);
-        }
-#pragma unroll
-        for (int nn = 0; nn < HD / 16; ++nn) {
-          // matrices: slots 0-7 | 8-15 of columns 0-7, then of columns 8-15
-          const int r = lane & 15, c16 = (nn & 3) * 2 + (lane >> 4);
-          uint32_t f[4];
-          ldsm4t(vt + (nn >> 2) * kTile * 128 + r * 128 + ((c16 ^ (r & 7)) << 4), f);
-          mma16816<T>(st.o[2 * nn], hi, f[0], f[1]);
-          mma16816<T>(st.o[2 * nn + 1], hi, f[2], f[3]);
-          mma16816<T>(st.o[2 * nn], lo, f[0], f[1]);
-          mma16816<T>(st.o[2 * nn + 1], lo, f[2], f[3]);
+          float t = fmaxf(s[nb][y], s[nb][y + 2]);
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 4));
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 8));
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
+          top[nb][y] = fmaxf(m[nb][y], t);
+          grow |= top[nb][y] > m[nb][y];
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[stage]);
-      if (++stage == Sh::kStages) { stage = 0; phase ^= 1; }
-    }
-    // the four warps' states, joined at their common maximum: 2 into 0 and 3 into 1, then 1 into 0
+      if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      st.l[y] += __shfl_xor_sync(0xFFFFFFFFu, st.l[y], 1);
-      st.l[y] += __shfl_xor_sync(0xFFFFFFFFu, st.l[y], 2);
-      if ((lane & 3) == 0) s_ml[warp][0][(lane >> 2) + 8 * y] = st.m[y];
-    }
-    if (dead && lane == 0) s_dead = 1;
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    float m[2];
+        for (int nb = 0; nb < NB; ++nb) {
+          const float f[2] = {shrink(m[nb][0], top[nb][0]), shrink(m[nb][1], top[nb][1])};
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const int r = (lane >> 2) + 8 * y;
-      m[y] = fmaxf(fmaxf(s_ml[0][0][r], s_ml[1][0][r]), fmaxf(s_ml[2][0][r], s_ml[3][0][r]));
-    }
-    st.scale(shrink(st.m[0], m[0]), shrink(st.m[1], m[1]));
-    if ((lane & 3) == 0) {
-      s_ml[warp][1][lane >> 2] = st.any ? st.l[0] : -1.0f;
-      s_ml[warp][1][(lane >> 2) + 8] = st.any ? st.l[1] : -1.0f;
-    }
-    float4* mine = reinterpret_cast<float4*>(s_join) + (warp & 1) * (kRowsMma * HD / 4);
-    auto give = [&] {
+          for (int x = 0; x < HD / 16; ++x)
 #pragma unroll
-      for (int x = 0; x < HD / 8; ++x) mine[x * 32 + lane] = make_float4(st.o[x][0], st.o[x][1], st.o[x][2], st.o[x][3]);
-    };
-    auto take = [&](const float4* from) {
+            for (int e = 0; e < 4; ++e) o[x][nb][e] *= f[e & 1];
 #pragma unroll
-      for (int x = 0; x < HD / 8; ++x) {
-        const float4 f = from[x * 32 + lane];
-        st.o[x][0] += f.x; st.o[x][1] += f.y; st.o[x][2] += f.z; st.o[x][3] += f.w;
+          for (int y = 0; y < 2; ++y) {
+            l[nb][y] *= f[y];
+            m[nb][y] = top[nb][y];
+          }
+        }
       }
-    };
-    if (warp >= 2) give();
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (warp < 2) take(mine);
-    if (warp == 1) {
-      __syncwarp();
-      give();
+      uint32_t hi[NB][2], lo[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float base = m[nb][e & 1] == neg_inf() ? 0.0f : m[nb][e & 1];
+          p[e] = show[e >> 1] ? ex2(s[nb][e] - base) : 0.0f;
+        }
+        l[nb][0] += p[0] + p[2];
+        l[nb][1] += p[1] + p[3];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t h = Elem<T>::pack(p[2 * y], p[2 * y + 1]);
+          const float2 f = Elem<T>::f2(h);
+          hi[nb][y] = transpose8x8(h);
+          lo[nb][y] = transpose8x8(Elem<T>::pack(p[2 * y] - f.x, p[2 * y + 1] - f.y));
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < HD / 16; ++x) {
+        // matrices: slots 0-7 of columns 0-7 | 8-15, then slots 8-15
+        const int rv = (lane & 7) + (lane >> 4) * 8, piece = 2 * x + (lane >> 3 & 1);
+        uint32_t f[4];
+        ldsm4t(vt + rv * HD * 2 + ((piece ^ (rv & 7)) << 4), f);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          mma16816<T>(o[x][nb], f, hi[nb][0], hi[nb][1]);
+          mma16816<T>(o[x][nb], f, lo[nb][0], lo[nb][1]);
+        }
+      }
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (warp == 0 && !s_dead) {
-      take(mine + kRowsMma * HD / 4);
-      const bool all = i0 == 0 && n == sq.nt;
-      float* part = ws.part + ((int64_t)blockIdx.x * 2 + (i0 == 0)) * Sh::kPart;
-      bool good = true;
+
+    // ---- the warps' states at their common maximum; a warp that met no slot says so by a sum of -1
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int r = (lane >> 2) + 8 * y;
-        float l = 0.0f;
-        bool any = false;
 #pragma unroll
-        for (int w = 0; w < kConsumers; ++w) {
-          const float x = s_ml[w][1][r];
-          if (!(x < 0.0f)) {                     // (a warp that met no visible slot says -1)
-            l += x;
-            any = true;
-          }
+        for (int x = 4; x < 32; x <<= 1) l[nb][y] += __shfl_xor_sync(0xFFFFFFFFu, l[nb][y], x);
+        if (lane < 4) {
+          s_m[warp][8 * nb + 2 * lane + y] = m[nb][y];
+          s_l[warp][8 * nb + 2 * lane + y] = any ? l[nb][y] : -1.0f;
         }
-        const float inv = any ? 1.0f / l : 0.0f;
-        if (r < rows) {
-          uint8_t* to = a.out + 2 * ((int64_t)b * a.orow + (int64_t)(h0 + r) * a.oh);
+      }
+    __syncthreads();
+    const bool all = w.i0 == 0 && w.i1 == w.sq.nt;
+    float* part = ws.part + ((int64_t)blockIdx.x * 2 + (w.i0 == 0)) * Sh::kPart;
+    bool good = true;
 #pragma unroll
-          for (int x = 0; x < HD / 8; ++x) {
-            const int col = 8 * x + 2 * (lane & 3);
-            const float o0 = st.o[x][2 * y], o1 = st.o[x][2 * y + 1];
-            if (all) {
-              good &= fabsf(o0 * inv) + fabsf(o1 * inv) < __int_as_float(0x7F800000);
-              *reinterpret_cast<uint32_t*>(to + 2 * col) = Elem<T>::pack(o0 * inv, o1 * inv);
-            } else {
-              *reinterpret_cast<float2*>(part + r * HD + col) = make_float2(o0, o1);
-            }
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int h = 8 * nb + 2 * (lane & 3) + y;
+        float mm = s_m[0][h];
+#pragma unroll
+        for (int k = 1; k < W; ++k) mm = fmaxf(mm, s_m[k][h]);
+        const float f = shrink(m[nb][y], mm);
+#pragma unroll
+        for (int x = 0; x < HD / 16; ++x) {
+          float* to = s_out + warp * Sh::kSlot + (2 * (lane & 3) + y) * (HD + 4) + 16 * x + (lane >> 2);
+          to[0] = o[x][nb][y] * f;
+          to[8] = o[x][nb][y + 2] * f;
+        }
+      }
+      __syncthreads();
+      for (int u = threadIdx.x; u < 8 * HD / 4; u += Sh::kThreads) {
+        const int hh = u / (HD / 4), col = 4 * (u - hh * (HD / 4)), h = 8 * nb + hh;
+        if (h >= rows) break;
+        float mm = s_m[0][h], sum = 0.0f;
+#pragma unroll
+        for (int k = 1; k < W; ++k) mm = fmaxf(mm, s_m[k][h]);
+        bool met = false;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          const float lk = s_l[k][h];
+          if (!(lk < 0.0f)) {
+            sum = fmaf(lk, shrink(s_m[k][h], mm), sum);
+            met = true;
           }
-          if ((lane & 3) == 0) {
-            if (!all) {
-              part[kRowsMma * HD + r] = m[y];
-              part[kRowsMma * HD + kRowsMma + r] = any ? l : -1.0f;
-            } else if (ws.ml) {
-              ws.ml[(int64_t)b * a.nh + h0 + r] = make_float2(m[y], l);
-            }
+          const float4 f = *reinterpret_cast<const float4*>(s_out + k * Sh::kSlot + hh * (HD + 4) + col);
+          v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
+        }
+        if (all) {
+          const float inv = met ? 1.0f / sum : 0.0f;
+          v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
+          good &= fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < __int_as_float(0x7F800000);
+          *reinterpret_cast<uint2*>(a.out + 2 * ((int64_t)w.b * a.orow + (int64_t)(h0 + h) * a.oh + col)) =
+              make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
+          if (col == 0 && ws.ml) ws.ml[(int64_t)w.b * a.nh + h0 + h] = make_float2(mm, sum);
+        } else {
+          *reinterpret_cast<float4*>(part + h * HD + col) = v;
+          if (col == 0) {
+            part[kRowsMma * HD + h] = mm;
+            part[kRowsMma * HD + kRowsMma + h] = met ? sum : -1.0f;
           }
         }
       }
-      good = __all_sync(0xFFFFFFFFu, good);
-      if (all && lane == 0) ws.redo[(int64_t)b * nsub + sub] = !good;
+      if (nb + 1 < NB) __syncthreads();
     }
-    left -= n;
-    if (i == sq.nt) {
-      i = 0;
-      if (++sub == nsub && left > 0) {
-        sub = 0;
-        do sq = SeqTiles(a, ++b);
-        while (sq.nt == 0);
-      }
-    }
-  }
+    const int bad = __syncthreads_or(!good);
+    if (all && threadIdx.x == 0) ws.redo[(int64_t)w.b * nsub + w.sub] = bad;
+  } while (w.next(a, nsub));
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // The items whose tiles lie in several CTAs' runs: their states at the common maximum, in run order.
@@ -478,16 +441,17 @@ __global__ void __launch_bounds__(kAttendThreads, 1)
 // an infinite value would make a NaN of it.
 constexpr int kJoinThreads = 256;
 template <class T, int HD>
-__global__ void __launch_bounds__(kJoinThreads) k_join(const __grid_constant__ AttendArgs a, AttendWs ws, int grid) {
+__global__ void __launch_bounds__(kJoinThreads)
+    k_join(const __grid_constant__ AttendArgs a, AttendWs ws, int grid, int gblocks, int hb) {
   using Sh = AttendShape<HD>;
   __shared__ PlanShared s_plan;
   griddep_launch();
   const KvCache& c = a.c;
-  const int G = a.nh / c.n_kv, gblocks = (G + kRowsMma - 1) / kRowsMma, nsub = c.n_kv * gblocks;
+  const int G = a.nh / c.n_kv, nsub = c.n_kv * gblocks;
   const int b = blockIdx.x / nsub, sub = blockIdx.x - b * nsub;
-  const int kvh = sub / gblocks, h0 = kvh * G + (sub - kvh * gblocks) * kRowsMma, rows = min(kRowsMma, (kvh + 1) * G - h0);
+  const int kvh = sub / gblocks, g0 = (sub - kvh * gblocks) * hb, h0 = kvh * G + g0, rows = min(hb, G - g0);
   long long at = 0;
-  const long long total = plan(a, nsub, s_plan, b, 0, 1, &at);
+  const long long total = plan(a, nsub, s_plan, b, 0, 1, Sh::kWarps, &at);
   const int nt = SeqTiles(a, b).nt;
   griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -498,7 +462,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const __grid_constant__ A
     return;
   }
   const long long t0 = at + (long long)sub * nt;
-  const int runs = runs_of(total, grid), c0 = run_of(total, runs, t0), c1 = run_of(total, runs, t0 + nt - 1);
+  const int runs = runs_of(total, grid, Sh::kWarps), c0 = run_of(total, runs, t0), c1 = run_of(total, runs, t0 + nt - 1);
   const bool redo = c0 == c1 && ws.redo[blockIdx.x];
   if (c0 == c1 && !redo) return;
   for (int r = warp; r < rows; r += kJoinThreads / 32) {
@@ -589,19 +553,19 @@ cudaError_t attend_hd(const AttendArgs& a, cudaStream_t st) {
   const KvCache& c = a.c;
   uint64_t bytes = 0;
   const AttendWs ws = ws_of(c, a.nh, a.weight_out != nullptr, a.ws, &bytes);
-  AttendMaps maps;
-  const int rows_box = std::min(kTile, 1 << c.shift);
-  if (!make_map_pool(&maps.k, c, c.k, rows_box) || !make_map_pool(&maps.v, c, c.v, rows_box)) return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(k_attend<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+  // a group's heads in blocks of nearly equal size, of 8 or of 16 places
+  const int G = a.nh / c.n_kv, gblocks = (G + kRowsMma - 1) / kRowsMma, hb = (G + gblocks - 1) / gblocks;
+  auto kern = hb <= 8 ? k_attend<T, HD, 1> : k_attend<T, HD, 2>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
   if (e != cudaSuccess) return e;
-  // no more CTAs than the page lists can hold tiles
-  const int G = a.nh / c.n_kv, nsub = c.n_kv * ((G + kRowsMma - 1) / kRowsMma);
-  const int64_t most = (int64_t)c.batch * nsub * ((((int64_t)c.max_pages << c.shift) + kTile - 1) / kTile);
+  // no more CTAs than the page lists can hold chunks for
+  const int nsub = c.n_kv * gblocks;
+  const int64_t most = ((int64_t)c.batch * nsub * (((int64_t)c.max_pages << c.shift) / kTile) + Sh::kWarps - 1) / Sh::kWarps;
   const int grid = (int)std::min<int64_t>(kMaxGrid, most);
-  k_attend<T, HD><<<grid, kAttendThreads, Sh::kSmem, st>>>(maps, a, ws, rows_box);
+  kern<<<grid, Sh::kThreads, Sh::kSmem, st>>>(a, ws, gblocks, hb);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if ((e = launch_dependent(k_join<T, HD>, dim3(c.batch * nsub), dim3(kJoinThreads), st, a, ws, grid)) != cudaSuccess) return e;
-  if (!a.weight_out) return cudaSuccess;
+  e = launch_dependent(k_join<T, HD>, dim3(c.batch * nsub), dim3(kJoinThreads), st, a, ws, grid, gblocks, hb);
+  if (e != cudaSuccess || !a.weight_out) return e;
   const int kvrows = c.batch * c.n_kv;
   return launch_dependent(k_weights, dim3(kvrows, std::max(1, 148 * 4 / kvrows)), dim3(kWeightThreads), st, a, ws);
 }

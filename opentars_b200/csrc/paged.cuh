@@ -7,7 +7,7 @@
 
 namespace tc {
 
-enum { kErrAppend = 51, kErrAttend = 52, kErrPrompt = 53, kErrEvict = 54, kErrAttendWait = 55, kErrPromptWait = 56 };
+enum { kErrAppend = 51, kErrAttend = 52, kErrPrompt = 53, kErrEvict = 54, kErrPromptWait = 55 };
 
 __device__ __forceinline__ void kv_fail(const KvCache& c, int code) { atomicCAS(c.err, 0, code); }
 

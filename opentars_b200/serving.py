@@ -374,6 +374,6 @@ def adjust_logits(logits: torch.Tensor, token: torch.Tensor | None = None, none:
 
 def device_error(clear: bool = False) -> int:
     """The first error the current device has recorded (0: none): 51 append, 52 attend, 53
-    attend_prompt, 54 evict - a page id outside the pool or a length beyond the page list -, 55 and 56
-    a bounded wait that gave up. Waits for the device."""
+    attend_prompt, 54 evict - a page id outside the pool or a length beyond the page list -, 55 a
+    bounded wait of attend_prompt that gave up. Waits for the device."""
     return _machine_lib().tc_wait_error(int(clear))

