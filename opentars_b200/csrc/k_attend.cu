@@ -33,11 +33,12 @@ constexpr int kTile = 16, kRowsMma = 16, kMaxGrid = 148;
 
 template <int HD>
 struct AttendShape {
-  // a warp's ring: kStages chunks of keys and values
-  static constexpr int kWarps = HD == 256 ? 4 : 8, kThreads = 32 * kWarps, kStages = HD == 64 ? 5 : 3;
-  static constexpr int kMat = kTile * HD * 2, kRing = kStages * 2 * kMat;
-  static constexpr int kSlot = 8 * (HD + 4);                 // floats of a warp's outputs of 8 heads, rows padded
-  static constexpr int kSmem = kWarps * (kRing + kSlot * 4);
+  // a warp's ring: kUnits times a chunk's keys or a chunk's values
+  static constexpr int kWarps = 8, kThreads = 32 * kWarps, kUnits = HD == 64 ? 10 : HD == 128 ? 6 : 3;
+  static constexpr int kMat = kTile * HD * 2, kRing = kUnits * kMat;
+  static constexpr int kCols = HD < 128 ? HD : 128;          // columns joined in one pass
+  static constexpr int kSlot = 8 * (kCols + 4);              // floats of a warp's outputs of 8 heads, rows padded
+  static constexpr int kSmem = 512 + kWarps * (kRing + kSlot * 4);
   static constexpr int kPart = kRowsMma * HD + 2 * kRowsMma; // floats of a CTA's state of an item
 };
 
@@ -55,6 +56,7 @@ struct SeqTiles {
   }
   __device__ __forceinline__ int tile(int i) const { return i < na ? i : t0 + i - na; }
   __device__ __forceinline__ bool visible(int j) const { return j < len && (j >= first || j < head); }
+  __device__ __forceinline__ bool whole(int j0) const { return j0 + kTile <= len && (j0 >= first || j0 + kTile <= head); }
 };
 
 struct PlanShared {
@@ -180,7 +182,7 @@ template <class T, int HD, int NB>
 __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
     k_attend(const __grid_constant__ AttendArgs a, AttendWs ws, int gblocks, int hb) {
   using Sh = AttendShape<HD>;
-  constexpr int W = Sh::kWarps, S = Sh::kStages, kPieces = HD / 8;
+  constexpr int W = Sh::kWarps, U = Sh::kUnits, kPieces = HD / 8;
   extern __shared__ __align__(16) uint8_t s_raw[];
   __shared__ float s_m[W][kRowsMma], s_l[W][kRowsMma];
   __shared__ PlanShared s_plan;
@@ -194,49 +196,67 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
   if ((int)blockIdx.x >= runs) return;
   const int left = (int)(run_begin(total, runs, blockIdx.x + 1) - run_begin(total, runs, blockIdx.x));
   const int nt0 = SeqTiles(a, s_plan.b).nt, sub0 = (int)(into / nt0), first = (int)(into - (long long)sub0 * nt0);
-  const uint32_t ring = smem_u32(s_raw) + warp * Sh::kRing;
-  float* s_out = reinterpret_cast<float*>(s_raw + W * Sh::kRing);
+  const uint32_t s_at = smem_u32(s_raw), pad = (512 - (s_at & 511)) % 512, ring = s_at + pad + warp * Sh::kRing;
+  float* s_out = reinterpret_cast<float*>(s_raw + pad + W * Sh::kRing);
 
-  // ---- the copies, S - 1 chunks ahead of their use; a chunk's page is looked up one chunk earlier still
+  // ---- the copies: a chunk's keys, its values, the next chunk's keys ..., U - 1 units ahead of their
+  // use. A chunk's page id is loaded one chunk earlier still and only looked at when it is copied.
   Walk pw(a, left, s_plan.b, sub0, first);
   int pi = first + warp, page = -1, to_slot = 0;
-  uint32_t held = 0;                              // bit x: the chunk copied x copies ago is in the ring
+  uint32_t held = 0;                              // bit x: the unit copied x copies ago is in the ring
   bool more = true;
+  // A row's 16-byte piece p is kept at place p ^ (row % 8) of its 128 bytes (no bank conflicts in ldmatrix);
+  // a lane copies piece lane % kLanes of rows r0, r0 + kAtOnce, .. and r0 < kAtOnce divides 8, so the
+  // place is that of row r0 with constant bits flipped. The ring starts on a multiple of 512 bytes.
+  constexpr int kLanes = kPieces < 32 ? kPieces : 32, kAtOnce = 32 / kLanes;
+  const int r0 = lane / kLanes;
+  const uint32_t put = ring + r0 * HD * 2 + ((lane % kLanes ^ r0) << 4);
+  const int64_t step = 2 * kAtOnce * c.ss;
   auto find = [&] {
     while (more && pi >= pw.i1) {
       more = pw.next(a, nsub);
       pi = pw.i0 + warp;
     }
-    if (more) page = kv_page(c, pw.b, pw.sq.tile(pi) * kTile, kErrAttend);
+    if (more) page = __ldg(c.table + (int64_t)pw.b * c.ts + (pw.sq.tile(pi) * kTile >> c.shift));
   };
-  auto copy = [&] {
-    held = held << 1 | (more && page >= 0);
-    if (held & 1) {
-      // piece lane % kPieces of the rows lane / kPieces, + 32 / kPieces, ..
-      constexpr int kLanes = kPieces < 32 ? kPieces : 32, kAtOnce = 32 / kLanes;
-      const int j0 = pw.sq.tile(pi) * kTile, piece = lane % kLanes, r0 = lane / kLanes, kvh = pw.sub / gblocks;
-      const int64_t from = 2 * (kv_offset(c, page, j0 + r0, kvh) + 8 * piece), step = 2 * kAtOnce * c.ss;
-      const uint32_t to = ring + to_slot * 2 * Sh::kMat;
+  auto copy = [&](const uint8_t* pool, bool last) {
+    const bool good = more && (unsigned)page < (unsigned)c.n_pages;
+    if (more && !good) kv_fail(c, kErrAttend);
+    held = held << 1 | good;
+    if (good) {
+      const int j0 = pw.sq.tile(pi) * kTile;
+      const uint8_t* from = pool + 2 * ((int64_t)page * c.sp + (int64_t)((j0 & ((1 << c.shift) - 1)) + r0) * c.ss +
+                                        (int64_t)(pw.sub / gblocks) * c.sh) + 16 * (lane % kLanes);
+      const uint32_t to = put + to_slot * Sh::kMat;
+      if (pw.sq.whole(j0)) {
 #pragma unroll
-      for (int x = 0; x < kTile / kAtOnce; ++x) {
-        const int r = r0 + x * kAtOnce;
-        const uint32_t at = to + r * HD * 2 + ((piece ^ (r & 7)) << 4);
-        const int bytes = pw.sq.visible(j0 + r) ? 16 : 0;     // a hidden row may hold anything: it reads as zeros
-        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(at), "l"(c.k + from + x * step), "r"(bytes) : "memory");
-        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(at + Sh::kMat), "l"(c.v + from + x * step), "r"(bytes) : "memory");
+        for (int x = 0; x < kTile / kAtOnce; ++x)
+          asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"((to ^ (x * kAtOnce % 8 << 4)) + x * kAtOnce * HD * 2),
+                       "l"(from + x * step) : "memory");
+      } else {                                    // a hidden row may hold anything: it reads as zeros
+#pragma unroll
+        for (int x = 0; x < kTile / kAtOnce; ++x)
+          asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"((to ^ (x * kAtOnce % 8 << 4)) + x * kAtOnce * HD * 2),
+                       "l"(from + x * step), "r"(pw.sq.visible(j0 + r0 + x * kAtOnce) ? 16 : 0) : "memory");
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    if (++to_slot == S) to_slot = 0;
-    pi += W;
-    find();
+    if (++to_slot == U) to_slot = 0;
+    if (last) {
+      pi += W;
+      find();
+    }
   };
   find();
 #pragma unroll
-  for (int x = 0; x < S - 1; ++x) copy();
+  for (int x = 0; x < U - 1; ++x) copy(x & 1 ? c.v : c.k, x & 1);
 
   Walk w(a, left, s_plan.b, sub0, first);
   int slot = 0;
+  // where ldmatrix reads: keys, slots 0-15 of columns 0-7 then 8-15; values, slots 0-7 of columns 0-7 and 8-15,
+  // then slots 8-15. The next 16 columns are 32 bytes on, which flips bits of the place.
+  const uint32_t k_at = ring + (lane & 15) * HD * 2 + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_at = ring + ((lane & 7) + (lane >> 4) * 8) * HD * 2 + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
   do {
     const int kvh = w.sub / gblocks, g0 = (w.sub - kvh * gblocks) * hb, h0 = kvh * G + g0, rows = min(hb, G - g0);
     // the query rows as the MMA's second operand: head lane / 4, columns 2 (lane % 4) (+ 1, + 8, + 9) of each 16
@@ -265,14 +285,14 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
       l[nb][0] = l[nb][1] = 0.0f;
     }
     for (int i = w.i0 + warp; i < w.i1; i += W) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
-      __syncwarp();                               // the chunk is here, and the one before it is used up
-      const uint32_t kt = ring + slot * 2 * Sh::kMat, vt = kt + Sh::kMat;
-      if (++slot == S) slot = 0;
-      copy();
+      asm volatile("cp.async.wait_group %0;" ::"n"(U - 2) : "memory");
+      __syncwarp();                               // the keys are here, and the unit before them is used up
+      const uint32_t kt = k_at + slot * Sh::kMat;
+      if (++slot == U) slot = 0;
+      copy((U - 1) & 1 ? c.v : c.k, (U - 1) & 1);
       const int j0 = w.sq.tile(i) * kTile;
-      if (!(held >> (S - 1) & 1)) continue;       // on a page outside the pool
-      any = true;
+      const bool here = held >> (U - 1) & 1;      // (not on a page outside the pool)
+      any |= here;
       float s[NB][4], s2[NB][4];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
@@ -280,23 +300,21 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
         for (int e = 0; e < 4; ++e) s[nb][e] = s2[nb][e] = 0.0f;
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
-        // matrices: slots 0-7, 8-15 of columns 0-7, then of columns 8-15
-        const int r = lane & 15, piece = 2 * kk + (lane >> 4);
         uint32_t f[4];
-        ldsm4(kt + r * HD * 2 + ((piece ^ (r & 7)) << 4), f);
+        ldsm4(kt ^ (kk << 5), f);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) mma16816<T>(kk & 1 ? s2[nb] : s[nb], f, q[nb][kk][0], q[nb][kk][1]);
       }
-      const bool whole = j0 + kTile <= w.sq.len && (j0 >= w.sq.first || j0 + kTile <= w.sq.head);
+      const bool whole = w.sq.whole(j0);
       const int r = lane >> 2;
-      const bool show[2] = {whole || w.sq.visible(j0 + r), whole || w.sq.visible(j0 + r + 8)};
+      const bool show[2] = {here && (whole || w.sq.visible(j0 + r)), here && (whole || w.sq.visible(j0 + r + 8))};
       float top[NB][2];
       bool grow = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[nb][e] = show[e >> 1] ? (s[nb][e] + s2[nb][e]) * a.scale2 : neg_inf();
-        if (ws.scores) {
+        if (ws.scores && here) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int h = 8 * nb + 2 * (lane & 3) + (e & 1);
@@ -347,12 +365,16 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
           lo[nb][y] = transpose8x8(Elem<T>::pack(p[2 * y] - f.x, p[2 * y + 1] - f.y));
         }
       }
+      asm volatile("cp.async.wait_group %0;" ::"n"(U - 2) : "memory");
+      __syncwarp();                               // the values are here, and the keys are used up
+      const uint32_t vt = v_at + slot * Sh::kMat;
+      if (++slot == U) slot = 0;
+      copy(U & 1 ? c.v : c.k, U & 1);
+      if (here)
 #pragma unroll
       for (int x = 0; x < HD / 16; ++x) {
-        // matrices: slots 0-7 of columns 0-7 | 8-15, then slots 8-15
-        const int rv = (lane & 7) + (lane >> 4) * 8, piece = 2 * x + (lane >> 3 & 1);
         uint32_t f[4];
-        ldsm4t(vt + rv * HD * 2 + ((piece ^ (rv & 7)) << 4), f);
+        ldsm4t(vt ^ (x << 5), f);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           mma16816<T>(o[x][nb], f, hi[nb][0], hi[nb][1]);
@@ -379,55 +401,61 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
     bool good = true;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
+      float f[2];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const int h = 8 * nb + 2 * (lane & 3) + y;
         float mm = s_m[0][h];
 #pragma unroll
         for (int k = 1; k < W; ++k) mm = fmaxf(mm, s_m[k][h]);
-        const float f = shrink(m[nb][y], mm);
+        f[y] = shrink(m[nb][y], mm);
+      }
 #pragma unroll
-        for (int x = 0; x < HD / 16; ++x) {
-          float* to = s_out + warp * Sh::kSlot + (2 * (lane & 3) + y) * (HD + 4) + 16 * x + (lane >> 2);
-          to[0] = o[x][nb][y] * f;
-          to[8] = o[x][nb][y + 2] * f;
+      for (int c0 = 0; c0 < HD; c0 += Sh::kCols) {
+        if (nb + c0 > 0) __syncthreads();         // the pass before is read
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int x = 0; x < Sh::kCols / 16; ++x) {
+            float* to = s_out + warp * Sh::kSlot + (2 * (lane & 3) + y) * (Sh::kCols + 4) + 16 * x + (lane >> 2);
+            to[0] = o[c0 / 16 + x][nb][y] * f[y];
+            to[8] = o[c0 / 16 + x][nb][y + 2] * f[y];
+          }
+        __syncthreads();
+        for (int u = threadIdx.x; u < 8 * Sh::kCols / 4; u += Sh::kThreads) {
+          const int hh = u / (Sh::kCols / 4), at = 4 * (u - hh * (Sh::kCols / 4)), col = c0 + at, h = 8 * nb + hh;
+          if (h >= rows) break;
+          float mm = s_m[0][h], sum = 0.0f;
+#pragma unroll
+          for (int k = 1; k < W; ++k) mm = fmaxf(mm, s_m[k][h]);
+          bool met = false;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int k = 0; k < W; ++k) {
+            const float lk = s_l[k][h];
+            if (!(lk < 0.0f)) {
+              sum = fmaf(lk, shrink(s_m[k][h], mm), sum);
+              met = true;
+            }
+            const float4 g = *reinterpret_cast<const float4*>(s_out + k * Sh::kSlot + hh * (Sh::kCols + 4) + at);
+            v.x += g.x; v.y += g.y; v.z += g.z; v.w += g.w;
+          }
+          if (all) {
+            const float inv = met ? 1.0f / sum : 0.0f;
+            v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
+            good &= fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < __int_as_float(0x7F800000);
+            *reinterpret_cast<uint2*>(a.out + 2 * ((int64_t)w.b * a.orow + (int64_t)(h0 + h) * a.oh + col)) =
+                make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
+            if (col == 0 && ws.ml) ws.ml[(int64_t)w.b * a.nh + h0 + h] = make_float2(mm, sum);
+          } else {
+            *reinterpret_cast<float4*>(part + h * HD + col) = v;
+            if (col == 0) {
+              part[kRowsMma * HD + h] = mm;
+              part[kRowsMma * HD + kRowsMma + h] = met ? sum : -1.0f;
+            }
+          }
         }
       }
-      __syncthreads();
-      for (int u = threadIdx.x; u < 8 * HD / 4; u += Sh::kThreads) {
-        const int hh = u / (HD / 4), col = 4 * (u - hh * (HD / 4)), h = 8 * nb + hh;
-        if (h >= rows) break;
-        float mm = s_m[0][h], sum = 0.0f;
-#pragma unroll
-        for (int k = 1; k < W; ++k) mm = fmaxf(mm, s_m[k][h]);
-        bool met = false;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-          const float lk = s_l[k][h];
-          if (!(lk < 0.0f)) {
-            sum = fmaf(lk, shrink(s_m[k][h], mm), sum);
-            met = true;
-          }
-          const float4 f = *reinterpret_cast<const float4*>(s_out + k * Sh::kSlot + hh * (HD + 4) + col);
-          v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
-        }
-        if (all) {
-          const float inv = met ? 1.0f / sum : 0.0f;
-          v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
-          good &= fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < __int_as_float(0x7F800000);
-          *reinterpret_cast<uint2*>(a.out + 2 * ((int64_t)w.b * a.orow + (int64_t)(h0 + h) * a.oh + col)) =
-              make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
-          if (col == 0 && ws.ml) ws.ml[(int64_t)w.b * a.nh + h0 + h] = make_float2(mm, sum);
-        } else {
-          *reinterpret_cast<float4*>(part + h * HD + col) = v;
-          if (col == 0) {
-            part[kRowsMma * HD + h] = mm;
-            part[kRowsMma * HD + kRowsMma + h] = met ? sum : -1.0f;
-          }
-        }
-      }
-      if (nb + 1 < NB) __syncthreads();
     }
     const int bad = __syncthreads_or(!good);
     if (all && threadIdx.x == 0) ws.redo[(int64_t)w.b * nsub + w.sub] = bad;
@@ -466,21 +494,53 @@ __global__ void __launch_bounds__(kJoinThreads)
   const bool redo = c0 == c1 && ws.redo[blockIdx.x];
   if (c0 == c1 && !redo) return;
   for (int r = warp; r < rows; r += kJoinThreads / 32) {
-    float m = neg_inf(), l = 0.0f, o[HD / 32] = {};
+    // the pieces' statistics, a lane each (at most kMaxGrid = 148 pieces), then their outputs, independent loads
+    constexpr int kEach = (kMaxGrid + 31) / 32;
+    float m = neg_inf(), l = 0.0f, o[HD / 32] = {}, f[kEach];
+    const int pieces = redo ? 0 : c1 - c0 + 1;
     bool any = false;
-    for (int k = c0; k <= c1 && !redo; ++k) {
-      const float* part = ws.part + ((int64_t)k * 2 + (k == c0)) * Sh::kPart;
-      const float mk = part[kRowsMma * HD + r], lk = part[kRowsMma * HD + kRowsMma + r];
-      if (lk < 0.0f) continue;
-      any = true;
-      const float m2 = fmaxf(m, mk), f = shrink(m, m2), g = shrink(mk, m2);
-      m = m2;
-      l = l * f + lk * g;
+    const float* row = ws.part + (int64_t)c0 * 2 * Sh::kPart + r * HD;
 #pragma unroll
-      for (int x = 0; x < HD / 64; ++x) {
-        const float2 v = *reinterpret_cast<const float2*>(part + r * HD + 2 * (lane + 32 * x));
-        o[2 * x] = o[2 * x] * f + v.x * g;
-        o[2 * x + 1] = o[2 * x + 1] * f + v.y * g;
+    for (int x = 0; x < kEach; ++x) {
+      const int k = lane + 32 * x;
+      f[x] = neg_inf();
+      if (k < pieces) {
+        const float* st = ws.part + ((int64_t)(c0 + k) * 2 + (k == 0)) * Sh::kPart + kRowsMma * HD + r;
+        if (!(st[kRowsMma] < 0.0f)) {
+          f[x] = st[0];
+          any = true;
+        }
+      }
+      m = fmaxf(m, f[x]);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+      const int k = lane + 32 * x;
+      const float lk = k < pieces ? ws.part[((int64_t)(c0 + k) * 2 + (k == 0)) * Sh::kPart + kRowsMma * HD + kRowsMma + r] : -1.0f;
+      f[x] = lk < 0.0f ? 0.0f : shrink(f[x], m);
+      if (!(lk < 0.0f)) l = fmaf(lk, f[x], l);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
+    any = __any_sync(0xFFFFFFFFu, any);
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+      const int n = min(32, pieces - 32 * x);
+#pragma unroll 4
+      for (int y = 0; y < n; ++y) {
+        const int k = 32 * x + y;
+        const float g = __shfl_sync(0xFFFFFFFFu, f[x], y);
+        const float* from = row + ((int64_t)k * 2 + (k == 0)) * Sh::kPart;
+#pragma unroll
+        for (int z = 0; z < HD / 64; ++z) {
+          const float2 v = *reinterpret_cast<const float2*>(from + 2 * (lane + 32 * z));
+          if (g != 0.0f) {                       // (a piece without a visible slot left nothing)
+            o[2 * z] = fmaf(v.x, g, o[2 * z]);
+            o[2 * z + 1] = fmaf(v.y, g, o[2 * z + 1]);
+          }
+        }
       }
     }
     const float inv = any ? 1.0f / l : 0.0f;
