@@ -463,128 +463,145 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// The items whose tiles lie in several CTAs' runs: their states at the common maximum, in run order.
-// Sequences without a slot get zeros. One CTA per (sequence, head block), a warp per row in turn. A row
-// with a NaN or an infinity is computed again key by key: the second half of a split probability times
-// an infinite value would make a NaN of it.
-constexpr int kJoinThreads = 256;
+// The items whose tiles lie in several CTAs' runs: their states at the common maximum. One CTA per
+// (sequence, head block, row): its warps take the pieces in turn, and their sums are added in warp
+// order. Sequences without a slot get zeros. A row with a NaN or an infinity is computed again key by
+// key: the second half of a split probability times an infinite value would make a NaN of it.
+constexpr int kJoinWarps = 8, kJoinThreads = 32 * kJoinWarps;
 template <class T, int HD>
 __global__ void __launch_bounds__(kJoinThreads)
     k_join(const __grid_constant__ AttendArgs a, AttendWs ws, int grid, int gblocks, int hb) {
   using Sh = AttendShape<HD>;
   __shared__ PlanShared s_plan;
+  __shared__ float2 s_o[kJoinWarps][HD / 2];
   griddep_launch();
   const KvCache& c = a.c;
   const int G = a.nh / c.n_kv, nsub = c.n_kv * gblocks;
-  const int b = blockIdx.x / nsub, sub = blockIdx.x - b * nsub;
-  const int kvh = sub / gblocks, g0 = (sub - kvh * gblocks) * hb, h0 = kvh * G + g0, rows = min(hb, G - g0);
+  const int item = blockIdx.x / hb, r = blockIdx.x - item * hb, b = item / nsub, sub = item - b * nsub;
+  const int kvh = sub / gblocks, g0 = (sub - kvh * gblocks) * hb, h = kvh * G + g0 + r;
   long long at = 0;
   const long long total = plan(a, nsub, s_plan, b, 0, 1, Sh::kWarps, &at);
   const int nt = SeqTiles(a, b).nt;
   griddep_wait();
+  if (g0 + r >= G) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t at_out = (int64_t)b * a.orow + (int64_t)h * a.oh;
+  uint32_t* to = reinterpret_cast<uint32_t*>(a.out + 2 * at_out);
   if (nt == 0) {
-    for (int r = warp; r < rows; r += kJoinThreads / 32)
-      for (int x = lane; x < HD / 2; x += 32)
-        *reinterpret_cast<uint32_t*>(a.out + 2 * ((int64_t)b * a.orow + (int64_t)(h0 + r) * a.oh) + 4 * x) = 0;
+    for (int x = threadIdx.x; x < HD / 2; x += kJoinThreads) to[x] = 0;
     return;
   }
   const long long t0 = at + (long long)sub * nt;
   const int runs = runs_of(total, grid, Sh::kWarps), c0 = run_of(total, runs, t0), c1 = run_of(total, runs, t0 + nt - 1);
-  const bool redo = c0 == c1 && ws.redo[blockIdx.x];
-  if (c0 == c1 && !redo) return;
-  for (int r = warp; r < rows; r += kJoinThreads / 32) {
-    // the pieces' statistics, a lane each (at most kMaxGrid = 148 pieces), then their outputs, independent loads
+  bool redo = c0 == c1;
+  if (redo && !ws.redo[item]) return;
+  if (!redo) {
+    // every warp: the pieces' statistics, a lane each (at most kMaxGrid = 148 pieces)
     constexpr int kEach = (kMaxGrid + 31) / 32;
-    float m = neg_inf(), l = 0.0f, o[HD / 32] = {}, f[kEach];
-    const int pieces = redo ? 0 : c1 - c0 + 1;
-    bool any = false;
-    const float* row = ws.part + (int64_t)c0 * 2 * Sh::kPart + r * HD;
+    float m = neg_inf(), l = 0.0f, f[kEach], lk[kEach];
+    const int pieces = c1 - c0 + 1;
+    auto piece = [&](int k) { return ws.part + ((int64_t)(c0 + k) * 2 + (k == 0)) * Sh::kPart; };
 #pragma unroll
     for (int x = 0; x < kEach; ++x) {
       const int k = lane + 32 * x;
       f[x] = neg_inf();
+      lk[x] = -1.0f;                             // a piece without a visible slot
       if (k < pieces) {
-        const float* st = ws.part + ((int64_t)(c0 + k) * 2 + (k == 0)) * Sh::kPart + kRowsMma * HD + r;
-        if (!(st[kRowsMma] < 0.0f)) {
-          f[x] = st[0];
-          any = true;
-        }
+        f[x] = piece(k)[kRowsMma * HD + r];
+        lk[x] = piece(k)[kRowsMma * HD + kRowsMma + r];
       }
-      m = fmaxf(m, f[x]);
     }
 #pragma unroll
+    for (int x = 0; x < kEach; ++x) m = lk[x] < 0.0f ? m : fmaxf(m, f[x]);
+#pragma unroll
     for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
+    bool any = false;
 #pragma unroll
     for (int x = 0; x < kEach; ++x) {
-      const int k = lane + 32 * x;
-      const float lk = k < pieces ? ws.part[((int64_t)(c0 + k) * 2 + (k == 0)) * Sh::kPart + kRowsMma * HD + kRowsMma + r] : -1.0f;
-      f[x] = lk < 0.0f ? 0.0f : shrink(f[x], m);
-      if (!(lk < 0.0f)) l = fmaf(lk, f[x], l);
+      const bool met = !(lk[x] < 0.0f);
+      any |= met;
+      f[x] = met ? shrink(f[x], m) : 0.0f;
+      if (met) l = fmaf(lk[x], f[x], l);
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
     any = __any_sync(0xFFFFFFFFu, any);
+    float2 o[HD / 64];
 #pragma unroll
-    for (int x = 0; x < kEach; ++x) {
-      const int n = min(32, pieces - 32 * x);
-#pragma unroll 4
-      for (int y = 0; y < n; ++y) {
-        const int k = 32 * x + y;
-        const float g = __shfl_sync(0xFFFFFFFFu, f[x], y);
-        const float* from = row + ((int64_t)k * 2 + (k == 0)) * Sh::kPart;
+    for (int z = 0; z < HD / 64; ++z) o[z] = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int z = 0; z < HD / 64; ++z) {
-          const float2 v = *reinterpret_cast<const float2*>(from + 2 * (lane + 32 * z));
-          if (g != 0.0f) {                       // (a piece without a visible slot left nothing)
-            o[2 * z] = fmaf(v.x, g, o[2 * z]);
-            o[2 * z + 1] = fmaf(v.y, g, o[2 * z + 1]);
+    for (int x = 0; x < kEach; ++x)
+#pragma unroll
+      for (int y = 0; y < 32 / kJoinWarps; ++y) {
+        const int k = 32 * x + y * kJoinWarps + warp;
+        const float g = __shfl_sync(0xFFFFFFFFu, f[x], y * kJoinWarps + warp);
+        if (k < pieces && g != 0.0f) {
+          const float2* from = reinterpret_cast<const float2*>(piece(k) + r * HD);
+#pragma unroll
+          for (int z = 0; z < HD / 64; ++z) {
+            const float2 v = from[lane + 32 * z];
+            o[z].x = fmaf(v.x, g, o[z].x);
+            o[z].y = fmaf(v.y, g, o[z].y);
           }
         }
       }
-    }
-    const float inv = any ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int z = 0; z < HD / 64; ++z) s_o[warp][lane + 32 * z] = o[z];
+    __syncthreads();
     bool good = true;
+    const float inv = any ? 1.0f / l : 0.0f;
+    if (threadIdx.x < HD / 2) {
+      float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int x = 0; x < HD / 32; ++x) {
-      o[x] *= inv;
-      good &= fabsf(o[x]) < __int_as_float(0x7F800000);
+      for (int k = 0; k < kJoinWarps; ++k) {
+        v.x += s_o[k][threadIdx.x].x;
+        v.y += s_o[k][threadIdx.x].y;
+      }
+      v.x *= inv;
+      v.y *= inv;
+      good = fabsf(v.x) + fabsf(v.y) < __int_as_float(0x7F800000);
+      to[threadIdx.x] = Elem<T>::pack(v.x, v.y);
     }
-    const int64_t at_out = (int64_t)b * a.orow + (int64_t)(h0 + r) * a.oh;
-    if (ws.ml && lane == 0 && !redo) ws.ml[(int64_t)b * a.nh + h0 + r] = make_float2(m, l);
-    if (redo || !__all_sync(0xFFFFFFFFu, good)) {
-      float q[HD / 32];
-      row_load<T, HD>(a.q, (int64_t)b * a.qr + (int64_t)(h0 + r) * a.qh, lane, q);
-      attend_row<T, HD>(c, b, kvh, q, a.scale2, SeqTiles(a, b).len, a.window, a.sinks, kErrAttend, o);
-      row_store<T, HD>(a.out, at_out, lane, o);
-    } else {
-      uint32_t* to = reinterpret_cast<uint32_t*>(a.out + 2 * at_out);
-#pragma unroll
-      for (int x = 0; x < HD / 64; ++x) to[lane + 32 * x] = Elem<T>::pack(o[2 * x], o[2 * x + 1]);
-    }
+    if (ws.ml && threadIdx.x == 0) ws.ml[(int64_t)b * a.nh + h] = make_float2(m, l);
+    redo = __syncthreads_or(!good);
+  }
+  if (redo && warp == 0) {
+    float q[HD / 32], o[HD / 32];
+    row_load<T, HD>(a.q, (int64_t)b * a.qr + (int64_t)h * a.qh, lane, q);
+    attend_row<T, HD>(c, b, kvh, q, a.scale2, SeqTiles(a, b).len, a.window, a.sinks, kErrAttend, o);
+    row_store<T, HD>(a.out, at_out, lane, o);
   }
 }
 
 // weight_out = weight + the visible slots' probabilities, summed over the heads that share a key-value head.
-constexpr int kWeightThreads = 256;
+constexpr int kWeightThreads = 256, kWeightHeads = 64;
 __global__ void __launch_bounds__(kWeightThreads) k_weights(const __grid_constant__ AttendArgs a, AttendWs ws) {
-  griddep_wait();
+  __shared__ float2 s_ml[kWeightHeads];          // a head's maximum, and 1 / its sum
   const KvCache& c = a.c;
   const int row = blockIdx.x, b = row / c.n_kv, g = row - b * c.n_kv, G = a.nh / c.n_kv;
   const int len = kv_length(c, b, kErrAttend), first = first_in_window(len, a.window);
-  const int64_t at = (int64_t)row * c.track;
-  for (int j = blockIdx.y * kWeightThreads + threadIdx.x; j < len; j += gridDim.y * kWeightThreads) {
-    float w = c.weight[at + j];
-    if ((j < a.sinks || j >= first) && kv_page(c, b, j, kErrAttend) >= 0) {
-      float sum = 0.0f;
-      for (int i = 0; i < G; ++i) {
-        const int64_t u = (int64_t)b * a.nh + g * G + i;
-        const float2 f = ws.ml[u];
-        sum += ex2(ws.scores[u * ws.cap + j] - f.x) / f.y;
-      }
-      w += sum;
+  const int64_t at = (int64_t)row * c.track, u = (int64_t)b * a.nh + g * G;
+  griddep_wait();
+  for (int i0 = 0; i0 < G; i0 += kWeightHeads) {
+    const int n = min(kWeightHeads, G - i0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kWeightThreads) {
+      const float2 f = ws.ml[u + i0 + i];
+      s_ml[i] = make_float2(f.x, 1.0f / f.y);
     }
-    a.weight_out[at + j] = w;
+    __syncthreads();
+    for (int j = blockIdx.y * kWeightThreads + threadIdx.x; j < len; j += gridDim.y * kWeightThreads) {
+      float w = i0 ? a.weight_out[at + j] : c.weight[at + j];
+      if (j < a.sinks || j >= first) {
+        const bool here = (unsigned)__ldg(c.table + (int64_t)b * c.ts + (j >> c.shift)) < (unsigned)c.n_pages;
+        const float* from = ws.scores + (u + i0) * ws.cap + j;
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) sum = fmaf(ex2(from[i * ws.cap] - s_ml[i].x), s_ml[i].y, sum);
+        if (here) w += sum;
+      }
+      a.weight_out[at + j] = w;
+    }
   }
 }
 
@@ -624,10 +641,12 @@ cudaError_t attend_hd(const AttendArgs& a, cudaStream_t st) {
   const int grid = (int)std::min<int64_t>(kMaxGrid, most);
   kern<<<grid, Sh::kThreads, Sh::kSmem, st>>>(a, ws, gblocks, hb);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  e = launch_dependent(k_join<T, HD>, dim3(c.batch * nsub), dim3(kJoinThreads), st, a, ws, grid, gblocks, hb);
+  e = launch_dependent(k_join<T, HD>, dim3(c.batch * nsub * hb), dim3(kJoinThreads), st, a, ws, grid, gblocks, hb);
   if (e != cudaSuccess || !a.weight_out) return e;
   const int kvrows = c.batch * c.n_kv;
-  return launch_dependent(k_weights, dim3(kvrows, std::max(1, 148 * 4 / kvrows)), dim3(kWeightThreads), st, a, ws);
+  const int64_t blocks = (((int64_t)c.max_pages << c.shift) + kWeightThreads - 1) / kWeightThreads;
+  return launch_dependent(k_weights, dim3(kvrows, (unsigned)std::min<int64_t>(blocks, std::max(1, 148 * 8 / kvrows))),
+                          dim3(kWeightThreads), st, a, ws);
 }
 
 template <class T>
