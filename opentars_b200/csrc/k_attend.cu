@@ -633,7 +633,7 @@ cudaError_t attend_hd(const AttendArgs& a, cudaStream_t st) {
   // a group's heads in blocks of nearly equal size, of 8 or of 16 places
   const int G = a.nh / c.n_kv, gblocks = (G + kRowsMma - 1) / kRowsMma, hb = (G + gblocks - 1) / gblocks;
   auto kern = hb <= 8 ? k_attend<T, HD, 1> : k_attend<T, HD, 2>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+  cudaError_t e = hb <= 8 ? allow_smem<k_attend<T, HD, 1>>(Sh::kSmem) : allow_smem<k_attend<T, HD, 2>>(Sh::kSmem);
   if (e != cudaSuccess) return e;
   // no more CTAs than the page lists can hold chunks for
   const int nsub = c.n_kv * gblocks;

@@ -486,7 +486,7 @@ cudaError_t prompt_hd(const AttendArgs& a, cudaStream_t st) {
   PromptMaps maps;
   const int box = std::min(Sh::kBlock, 1 << c.shift);
   if (!make_map_pool(&maps.k, c, c.k, box) || !make_map_pool(&maps.v, c, c.v, box)) return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(k_prompt<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+  const cudaError_t e = allow_smem<k_prompt<T, HD>>(Sh::kSmem);
   if (e != cudaSuccess) return e;
   // a group's heads in blocks of nearly equal size; as many tokens as fill a tile with them
   const int G = a.nh / c.n_kv, gblocks = (G + kMaxHeads - 1) / kMaxHeads, hb = (G + gblocks - 1) / gblocks;

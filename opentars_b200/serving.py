@@ -17,6 +17,7 @@ graph. Wrong arguments raise ValueError before anything is enqueued; what only t
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -58,13 +59,12 @@ SERVE_SIGNATURES = {
 }
 
 
+@functools.lru_cache(None)
 def lib():
     L = _machine_lib()
-    if not getattr(L, "_serve_bound", False):
-        for name, (res, args) in SERVE_SIGNATURES.items():
-            fn = getattr(L, name)
-            fn.restype, fn.argtypes = res, args
-        L._serve_bound = True
+    for name, (res, args) in SERVE_SIGNATURES.items():
+        fn = getattr(L, name)
+        fn.restype, fn.argtypes = res, args
     return L
 
 
@@ -81,25 +81,23 @@ def _check(rc: int, what: str) -> None:
 
 
 def _ints(t: torch.Tensor, shape: tuple, device: torch.device, name: str) -> None:
-    _need(t.dtype == torch.int32 and tuple(t.shape) == shape and t.device == device and t.is_contiguous(),
-          f"{name}: a contiguous int32 tensor of shape {shape} on {device} is wanted")
+    if not (t.dtype is torch.int32 and t.shape == shape and t.device == device and t.is_contiguous()):
+        raise ValueError(f"{name}: a contiguous int32 tensor of shape {tuple(shape)} on {device} is wanted")
 
 
-class _On:
-    """The device of a call's tensors current, and its current stream's handle."""
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-    def __init__(self, device: torch.device):
-        self.device = device
 
-    def __enter__(self) -> int:
-        self.was = torch.cuda.current_device()
-        if self.was != self.device.index:
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.was != self.device.index:
-            torch.cuda.set_device(self.was)
+def _run(index: int, what: str, fn, *args) -> None:
+    """fn(*args, current stream) with device `index` current."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
+    if rc:
+        _check(rc, what)
 
 
 def _stride(t: torch.Tensor, d: int) -> int:
@@ -168,6 +166,15 @@ class PagedCache:
                             length.data_ptr(), ptr(weight), ptr(pos), 0 if weight is None else weight.shape[2],
                             ptr(seen))
         self.ref = ctypes.byref(self.desc)
+        self.index = k.device.index
+        self._sizes: dict = {}                                    # workspace bytes by what asks for them
+
+    def workspace(self, fn, *args) -> torch.Tensor:
+        """A workspace of its own for one call, from torch's allocator on the current stream."""
+        n = self._sizes.get((fn.__name__, args))
+        if n is None:
+            n = self._sizes[fn.__name__, args] = fn(self.ref, *args)
+        return torch.empty(n, dtype=torch.uint8, device=self.device)
 
     k = property(lambda self: self._t[0])
     v = property(lambda self: self._t[1])
@@ -192,9 +199,15 @@ class PagedCache:
         return cls(pool(), pool(), ints(batch, max_pages), ints(batch), **more)
 
 
-def _rows(t: torch.Tensor, cache: PagedCache, heads: int | None, name: str) -> None:
-    _need(t.dim() == 3 and t.shape[2] == cache.head_dim and (heads is None or t.shape[1] == heads) and
-          t.device == cache.device and t.stride(2) == 1, f"{name}: [rows, heads, {cache.head_dim}] on {cache.device}")
+def _rows(t: torch.Tensor, cache: PagedCache, heads: int, name: str) -> tuple[int, int, int]:
+    """The number of rows of t [rows, heads, head_dim] on the cache's device, its row and head strides."""
+    shape, stride = t.shape, t.stride()
+    if not (len(shape) == 3 and shape[2] == cache.head_dim and stride[2] == 1 and t.device == cache.device and
+            (shape[1] == heads if heads else shape[1] >= 1 and shape[1] % cache.n_kv == 0)):
+        raise ValueError(f"{name}: [rows, {heads or 'a multiple of %d' % cache.n_kv} heads, {cache.head_dim}] on "
+                         f"{cache.device}, a head's elements contiguous")
+    # a dimension of one entry is never stepped over: its stride may be anything
+    return shape[0], stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
 
 
 def _cu(cu: torch.Tensor, cache: PagedCache) -> int:
@@ -205,28 +218,30 @@ def _cu(cu: torch.Tensor, cache: PagedCache) -> int:
 def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor | None = None) -> None:
     """The new tokens' rows [tokens, n_kv, head_dim] (fp32, bf16 or fp16) into the cache, rounded to its
     type. Sequence b owns rows cu[b] .. cu[b+1]-1 (cu None: row b), counted in length and seen already."""
-    _rows(k, cache, cache.n_kv, "k")
-    _need(k.dtype in DTYPES and v.dtype == k.dtype and v.shape == k.shape and v.stride() == k.stride() and
-          v.device == k.device, "k and v: rows of one shape, type (fp32, bf16 or fp16) and stride")
-    _need(cu is not None or k.shape[0] <= cache.batch, "without cu there is one row per sequence")
+    n, row, head = _rows(k, cache, cache.n_kv, "k")
+    code = DTYPES.get(k.dtype)
+    if code is None or v.dtype is not k.dtype or v.shape != k.shape or v.stride() != k.stride() or v.device != k.device:
+        raise ValueError("k and v: rows of one shape, type (fp32, bf16 or fp16) and stride")
+    if cu is None:
+        _need(n <= cache.batch, "without cu there is one row per sequence")
     cu_p = None if cu is None else _cu(cu, cache)
-    if k.shape[0] == 0:
-        return
-    with _On(cache.device) as stream:
-        _check(lib().tc_kv_append(cache.ref, k.data_ptr(), v.data_ptr(), DTYPES[k.dtype], _stride(k, 0), _stride(k, 1),
-                                  cu_p, k.shape[0], stream), "append")
+    if n:
+        _run(cache.index, "append", lib().tc_kv_append, cache.ref, k.data_ptr(), v.data_ptr(), code, row, head, cu_p, n)
 
 
-def _attend_args(cache: PagedCache, q: torch.Tensor, out: torch.Tensor | None, window: int, sinks: int) -> torch.Tensor:
-    _rows(q, cache, None, "q")
-    _need(q.dtype == cache.dtype, f"q has the cache's type {cache.dtype}, not {q.dtype}")
-    _need(q.shape[1] >= 1 and q.shape[1] % cache.n_kv == 0, f"{q.shape[1]} heads over {cache.n_kv} key-value heads")
-    _need(window >= 0 and sinks >= 0, "window and sinks are not negative")
+def _attend_args(cache: PagedCache, q: torch.Tensor, out: torch.Tensor | None, window: int, sinks: int) -> tuple:
+    """The checked rows of q and out: (rows, out, (q, its strides, out, its strides, heads))."""
+    n, row, head = _rows(q, cache, 0, "q")
+    if q.dtype is not cache.dtype:
+        raise ValueError(f"q has the cache's type {cache.dtype}, not {q.dtype}")
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks are not negative")
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _rows(out, cache, q.shape[1], "out")
-    _need(out.dtype == q.dtype and out.shape == q.shape and _apart(out), "out has q's shape and type, its rows apart")
-    return out
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.dtype is not q.dtype or out.shape != q.shape or not (out.is_contiguous() or _apart(out)):
+        raise ValueError("out has q's shape and type, its rows apart")
+    _, orow, ohead = _rows(out, cache, q.shape[1], "out")
+    return n, out, (q.data_ptr(), row, head, out.data_ptr(), orow, ohead, q.shape[1])
 
 
 def attend(cache: PagedCache, q: torch.Tensor, scale: float, window: int = 0, sinks: int = 0,
@@ -234,21 +249,13 @@ def attend(cache: PagedCache, q: torch.Tensor, scale: float, window: int = 0, si
     """Attention of one query row per sequence, q [batch, heads, head_dim], over its slots: those of the
     last `window` (0: all) and the first `sinks`. weight_out (cache.weight, or a tensor like it)
     receives cache.weight plus the attention weight each slot draws. Length 0 gives zeros."""
-    out = _attend_args(cache, q, out, window, sinks)
-    _need(q.shape[0] == cache.batch, f"{q.shape[0]} query rows for {cache.batch} sequences")
-    w = None
-    if weight_out is not None:
-        _need(cache.weight is not None, "the cache keeps no weights")
-        _need(weight_out.dtype == torch.float32 and weight_out.shape == cache.weight.shape and
-              weight_out.is_contiguous() and weight_out.device == cache.device, "weight_out is laid out as cache.weight")
-        w = weight_out.data_ptr()
+    n, out, args = _attend_args(cache, q, out, window, sinks)
+    if n != cache.batch:
+        raise ValueError(f"{n} query rows for {cache.batch} sequences")
+    w = None if weight_out is None else _weight_out(cache, weight_out)
     L = lib()
-    with _On(cache.device) as stream:
-        n = L.tc_attend_workspace(cache.ref, q.shape[1], w is not None)
-        ws = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
-        _check(L.tc_attend(cache.ref, q.data_ptr(), _stride(q, 0), _stride(q, 1), out.data_ptr(),
-                           _stride(out, 0), _stride(out, 1), q.shape[1], scale, window, sinks, w, None if ws is None else ws.data_ptr(), n,
-                           stream), "attend")
+    ws = cache.workspace(L.tc_attend_workspace, args[6], int(w is not None))
+    _run(cache.index, "attend", L.tc_attend, cache.ref, *args, scale, window, sinks, w, ws.data_ptr(), ws.numel())
     return out
 
 
@@ -257,15 +264,18 @@ def attend_prompt(cache: PagedCache, q: torch.Tensor, cu: torch.Tensor, scale: f
     """Attention of the last tokens of each sequence, rows cu[b] .. cu[b+1]-1 of q [tokens, heads,
     head_dim] for sequence b, each over the slots up to its own position, of the last `window` (0: all)
     and the first `sinks`. Rows at and behind cu[batch] are left alone."""
-    out = _attend_args(cache, q, out, window, sinks)
+    n, out, args = _attend_args(cache, q, out, window, sinks)
     cu_p = _cu(cu, cache)
-    if q.shape[0] == 0:
-        return out
-    with _On(cache.device) as stream:
-        _check(lib().tc_attend_prompt(cache.ref, q.data_ptr(), _stride(q, 0), _stride(q, 1), out.data_ptr(),
-                                      _stride(out, 0), _stride(out, 1), q.shape[1], cu_p, q.shape[0], scale, window, sinks, stream),
-               "attend_prompt")
+    if n:
+        _run(cache.index, "attend_prompt", lib().tc_attend_prompt, cache.ref, *args, cu_p, n, scale, window, sinks)
     return out
+
+
+def _weight_out(cache: PagedCache, t: torch.Tensor) -> int:
+    _need(cache.weight is not None, "the cache keeps no weights")
+    if not (t.dtype is torch.float32 and t.shape == cache.weight.shape and t.is_contiguous() and t.device == cache.device):
+        raise ValueError("weight_out is laid out as cache.weight")
+    return t.data_ptr()
 
 
 def evict(cache: PagedCache, budget: int, sinks: int = 0, recent: int = 0, length_out: torch.Tensor | None = None,
@@ -277,26 +287,31 @@ def evict(cache: PagedCache, budget: int, sinks: int = 0, recent: int = 0, lengt
     _need(cache.weight is not None, "the cache keeps no weights")
     _need(budget >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= budget, "0 <= sinks + recent <= budget")
     length_out = cache.length if length_out is None else length_out
-    weight_out = cache.weight if weight_out is None else weight_out
     pos_out = cache.pos if pos_out is None else pos_out
     _ints(length_out, (cache.batch,), cache.device, "length_out")
-    _ints(pos_out, tuple(cache.pos.shape), cache.device, "pos_out")
-    _need(weight_out.dtype == torch.float32 and weight_out.shape == cache.weight.shape and weight_out.is_contiguous()
-          and weight_out.device == cache.device, "weight_out is laid out as cache.weight")
+    _ints(pos_out, cache.pos.shape, cache.device, "pos_out")
+    w = _weight_out(cache, cache.weight if weight_out is None else weight_out)
     L = lib()
-    with _On(cache.device) as stream:
-        n = L.tc_kv_evict_workspace(cache.ref, budget)
-        ws = torch.empty(n, dtype=torch.uint8, device=cache.device)
-        _check(L.tc_kv_evict(cache.ref, budget, sinks, recent, length_out.data_ptr(), weight_out.data_ptr(),
-                             pos_out.data_ptr(), ws.data_ptr(), n, stream), "evict")
+    ws = cache.workspace(L.tc_kv_evict_workspace, budget)
+    _run(cache.index, "evict", L.tc_kv_evict, cache.ref, budget, sinks, recent, length_out.data_ptr(), w,
+         pos_out.data_ptr(), ws.data_ptr(), ws.numel())
 
 
 def _per_row(t: torch.Tensor | None, dtype: torch.dtype, rows: int, device: torch.device, name: str) -> int | None:
     if t is None:
         return None
-    _need(t.dtype == dtype and tuple(t.shape) == (rows,) and t.device == device and t.is_contiguous(),
-          f"{name}: {dtype} [{rows}] on {device}")
+    if not (t.dtype is dtype and t.shape == (rows,) and t.device == device and t.is_contiguous()):
+        raise ValueError(f"{name}: {dtype} [{rows}] on {device}")
     return t.data_ptr()
+
+
+def _matrix(t: torch.Tensor, dtype: torch.dtype, rows: int, device: torch.device, name: str) -> tuple[int, int, int]:
+    """A [rows, n] matrix' pointer, row stride and n; its rows do not overlap."""
+    shape, stride = t.shape, t.stride()
+    if not (len(shape) == 2 and shape[0] == rows and t.dtype is dtype and t.device == device and
+            (stride[1] == 1 or shape[1] <= 1) and (stride[0] >= shape[1] or rows == 1)):
+        raise ValueError(f"{name}: {dtype} [{rows}, ..] on {device}, its rows contiguous and apart")
+    return t.data_ptr(), stride[0] if rows > 1 else shape[1], shape[1]
 
 
 def rules_of(logits: torch.Tensor, out: torch.Tensor | None = None, history: torch.Tensor | None = None,
@@ -306,55 +321,39 @@ def rules_of(logits: torch.Tensor, out: torch.Tensor | None = None, history: tor
              bias: torch.Tensor | None = None, mask: torch.Tensor | None = None, token: torch.Tensor | None = None,
              none: int = -1) -> Rules_t:
     """The checked C description of adjust_logits' arguments."""
-    out = logits if out is None else out
-    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.is_cuda and logits.stride(1) == 1 and
-          logits.shape[0] >= 1 and logits.shape[1] >= 1, "logits: fp32 [rows, vocab] on a CUDA device")
-    _need(out.dtype == torch.float32 and out.shape == logits.shape and out.device == logits.device and
-          out.stride(1) == 1, "out has the logits' shape, type and device")
-    rows, vocab = logits.shape
-    dev = logits.device
-    r = Rules_t()
-
-    def wide(t: torch.Tensor) -> int:
-        """A matrix' row stride; rows must not overlap (a single row's stride may be anything)."""
-        _need(t.shape[0] == 1 or t.stride(0) >= t.shape[1], "rows of logits, history, biases and masks lie apart")
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-    r.logits, r.out, r.rows, r.vocab, r.none = logits.data_ptr(), out.data_ptr(), rows, vocab, none
-    r.logits_stride, r.out_stride = wide(logits), wide(out)
-    if history is not None and history.numel() == 0:
-        _need(tuple(history.shape) == (rows, 0), "history: int32 [rows, ids]")
-        history = n_history = n_prompt = repetition = presence = frequency = None
-    if history is not None:
-        _need(history.dim() == 2 and history.shape[0] == rows and history.dtype == torch.int32 and
-              history.device == dev and (history.stride(1) == 1 or history.shape[1] <= 1), "history: int32 [rows, ids]")
-        r.history, r.history_stride, r.max_history = history.data_ptr(), wide(history), history.shape[1]
-    else:
-        _need(all(t is None for t in (n_history, n_prompt, repetition, presence, frequency)),
-              "the penalties need the history")
-    r.n_history = _per_row(n_history, torch.int32, rows, dev, "n_history")
-    r.n_prompt = _per_row(n_prompt, torch.int32, rows, dev, "n_prompt")
-    r.repetition = _per_row(repetition, torch.float32, rows, dev, "repetition")
-    r.presence = _per_row(presence, torch.float32, rows, dev, "presence")
-    r.frequency = _per_row(frequency, torch.float32, rows, dev, "frequency")
+    _need(logits.is_cuda and logits.dim() == 2 and logits.shape[0] >= 1 and logits.shape[1] >= 1,
+          "logits: fp32 [rows, vocab] on a CUDA device")
+    rows, dev = logits.shape[0], logits.device
+    x, x_stride, vocab = _matrix(logits, torch.float32, rows, dev, "logits")
+    y, y_stride, n = (x, x_stride, vocab) if out is None else _matrix(out, torch.float32, rows, dev, "out")
+    _need(n == vocab, "out has the logits' shape")
+    h, h_stride, n_h = (None, 0, 0) if history is None else _matrix(history, torch.int32, rows, dev, "history")
+    counts = (_per_row(n_history, torch.int32, rows, dev, "n_history"),
+              _per_row(n_prompt, torch.int32, rows, dev, "n_prompt"),
+              _per_row(repetition, torch.float32, rows, dev, "repetition"),
+              _per_row(presence, torch.float32, rows, dev, "presence"),
+              _per_row(frequency, torch.float32, rows, dev, "frequency"))
+    if n_h == 0:
+        _need(history is not None or counts == (None,) * 5, "the penalties need the history")
+        h, counts = None, (None,) * 5                             # an empty history has nothing to penalise
     _need((bias is None) == (bias_ids is None), "bias and bias_ids come together")
-    if bias is not None and bias.numel() == 0 == bias_ids.numel():
-        bias = bias_ids = None
+    ids = val = None
+    b_stride = n_b = 0
     if bias is not None:
-        _need(bias_ids.dim() == 2 and bias_ids.shape[0] == rows and bias_ids.dtype == torch.int32 and
-              bias.dtype == torch.float32 and bias.shape == bias_ids.shape and bias.stride() == bias_ids.stride() and
-              bias.device == dev and bias_ids.device == dev and (bias.stride(1) == 1 or bias.shape[1] <= 1),
-              "bias_ids int32 and bias fp32, [rows, entries]")
-        r.bias_ids, r.bias, r.bias_stride, r.n_bias = bias_ids.data_ptr(), bias.data_ptr(), wide(bias), bias.shape[1]
+        ids, b_stride, n_b = _matrix(bias_ids, torch.int32, rows, dev, "bias_ids")
+        val, v_stride, n = _matrix(bias, torch.float32, rows, dev, "bias")
+        _need(n == n_b and v_stride == b_stride, "bias_ids and bias have one shape and stride")
+        if n_b == 0:
+            ids = val = None
+    m, m_stride = None, 0
     if mask is not None:
-        words = (vocab + 31) // 32
-        _need(mask.dtype == torch.int32 and mask.device == dev and mask.dim() in (1, 2) and mask.shape[-1] == words and
-              mask.stride(-1) == 1 and (mask.dim() == 1 or mask.shape[0] == rows),
-              f"mask: int32 [rows, {words}], or [{words}] for all rows")
-        r.mask, r.mask_stride = mask.data_ptr(), 0 if mask.dim() == 1 else wide(mask)
-    if token is not None:
-        r.token = _per_row(token, torch.int32, rows, dev, "token")
-    return r
+        m, m_stride, n = _matrix(mask if mask.dim() == 2 else mask[None], torch.int32, rows if mask.dim() == 2 else 1, dev,
+                                 "mask")
+        _need(n == (vocab + 31) // 32, f"mask: int32 [rows, {(vocab + 31) // 32}], or one row for all")
+        if mask.dim() == 1:
+            m_stride = 0
+    return Rules_t(x, y, x_stride, y_stride, rows, vocab, h, h_stride, n_h, *counts, ids, val, b_stride, n_b, m, m_stride,
+                   _per_row(token, torch.int32, rows, dev, "token"), none)
 
 
 def adjust_logits(logits: torch.Tensor, token: torch.Tensor | None = None, none: int = -1, **rules) -> torch.Tensor:
@@ -365,10 +364,9 @@ def adjust_logits(logits: torch.Tensor, token: torch.Tensor | None = None, none:
     int32 words, bit t % 32 of word t // 32 set where token t is allowed. A row whose mask allows
     nothing picks `none`."""
     if token is None:
-        token = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
+        token = torch.empty(logits.shape[:1], dtype=torch.int32, device=logits.device)
     r = rules_of(logits, token=token, none=none, **rules)
-    with _On(logits.device) as stream:
-        _check(lib().tc_adjust_logits(ctypes.byref(r), stream), "adjust_logits")
+    _run(logits.device.index, "adjust_logits", lib().tc_adjust_logits, ctypes.byref(r))
     return token
 
 
