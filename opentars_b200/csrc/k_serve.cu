@@ -92,12 +92,15 @@ cudaError_t append_to(const AppendArgs& a, cudaStream_t st) {
 
 // ------------------------------------------------------------------------------------ evict
 // One CTA ranks the slots of one (sequence, key-value head). A slot's rank key is a 32-bit number
-// (protected slots highest, then a NaN weight, then the weight's bits made monotonic); the budget-th
-// largest key is found digit by digit from the top (8 bits a pass, counted in shared memory), and of
-// the slots with that key as many stay as are needed, from the lowest slot on. Warps own contiguous
-// runs of slots, so the lists of leaving and arriving slots come out in ascending order from
-// ballots and one scan over the warps. The rows move in a second kernel over the lists.
-constexpr int kRankThreads = 1024, kRankWarps = kRankThreads / 32;
+// (protected slots highest, then a NaN weight, then the weight's bits made monotonic), computed once
+// and kept in shared memory while it fits there. The budget-th largest key is found digit by digit
+// from the top (11, 11 and 10 bits, counted in shared memory), and of the slots with that key as many
+// stay as are needed, from the lowest slot on. Warps own contiguous runs of slots, so the lists of
+// leaving and arriving slots come out in ascending order from ballots and one scan over the warps.
+// A few rows are moved at once (a cache one slot over its budget moves one); more of them in a second
+// kernel over the lists. Bound by the chain of block-wide steps: about 1 us of loads, then three
+// counting passes and two walks of some 0.4 us each for a thousand slots.
+constexpr int kRankThreads = 1024, kRankWarps = kRankThreads / 32, kBins = 2048, kKeysMax = 49152, kFewMoves = 32;
 
 __device__ __forceinline__ uint32_t rank_key(float w, int pos, int sinks, int64_t recent_from) {
   if (pos < sinks || pos >= recent_from) return 0xFFFFFFFFu;
@@ -119,29 +122,44 @@ __host__ __device__ inline int most_moves(int capacity, int budget) {
   return capacity <= budget ? 0 : (budget < capacity - budget ? budget : capacity - budget);
 }
 
-// Exclusive sum over the warps of the CTA of each warp's x (same x in a warp's lanes); *all gets the total.
-__device__ __forceinline__ int warps_before(int x, int* s_warp, int* all) {
+// Exclusive sums over the warps of the CTA of each warp's (x, y) (the same in a warp's lanes), and the totals.
+__device__ __forceinline__ int2 warps_before(int x, int y, int2* s_warp, int2* all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __syncthreads();
-  if (lane == 0) s_warp[warp] = x;
+  if (lane == 0) s_warp[warp] = make_int2(x, y);
   __syncthreads();
-  const int mine = s_warp[lane];
-  int sum = mine;
+  const int2 mine = s_warp[lane];
+  int2 sum = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-    if (lane >= o) sum += y;
+    const int u = __shfl_up_sync(0xFFFFFFFFu, sum.x, o), v = __shfl_up_sync(0xFFFFFFFFu, sum.y, o);
+    if (lane >= o) {
+      sum.x += u;
+      sum.y += v;
+    }
   }
-  *all = __shfl_sync(0xFFFFFFFFu, sum, 31);
-  return __shfl_sync(0xFFFFFFFFu, sum - mine, warp);
+  *all = make_int2(__shfl_sync(0xFFFFFFFFu, sum.x, 31), __shfl_sync(0xFFFFFFFFu, sum.y, 31));
+  return make_int2(__shfl_sync(0xFFFFFFFFu, sum.x - mine.x, warp), __shfl_sync(0xFFFFFFFFu, sum.y - mine.y, warp));
 }
 
-__global__ void __launch_bounds__(kRankThreads) k_rank(EvictArgs a, Moves mv) {
+// One 16-byte piece of a moved row, keys and values. Sources lie at or behind the budget, destinations before it.
+__device__ __forceinline__ void move_piece(const KvCache& c, int b, int h, int2 m, int e) {
+  const int ps = kv_page(c, b, m.x, kErrEvict), pd = kv_page(c, b, m.y, kErrEvict);
+  if (ps < 0 || pd < 0) return;
+  const int64_t s = kv_offset(c, ps, m.x, h) + e, d = kv_offset(c, pd, m.y, h) + e;
+  const uint4 k = *reinterpret_cast<const uint4*>(c.k + 2 * s), v = *reinterpret_cast<const uint4*>(c.v + 2 * s);
+  *reinterpret_cast<uint4*>(c.k + 2 * d) = k;
+  *reinterpret_cast<uint4*>(c.v + 2 * d) = v;
+}
+
+__global__ void __launch_bounds__(kRankThreads) k_rank(EvictArgs a, Moves mv, int room) {
   const KvCache& c = a.c;
-  __shared__ int s_hist[256];
-  __shared__ int s_warp[kRankWarps];
-  __shared__ uint32_t s_digit;
-  __shared__ int s_left;
+  extern __shared__ uint32_t s_key[];                            // `room` keys
+  __shared__ int s_hist[kBins];
+  __shared__ int2 s_warp[kRankWarps];
+  __shared__ int2 s_few[kFewMoves];
+  __shared__ int s_digit, s_left, s_count;
+  griddep_launch();
   const int row = blockIdx.x, b = row / c.n_kv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int len = kv_length(c, b, kErrEvict);
@@ -159,81 +177,107 @@ __global__ void __launch_bounds__(kRankThreads) k_rank(EvictArgs a, Moves mv) {
     return;
   }
   const int64_t recent_from = (int64_t)__ldg(c.seen + b) - a.recent;
-  auto key = [&](int i) { return rank_key(w[i], pos[i], a.sinks, recent_from); };
+  const bool held = len <= room;
+  if (held)
+#pragma unroll 4
+    for (int i = threadIdx.x; i < len; i += kRankThreads) s_key[i] = rank_key(w[i], pos[i], a.sinks, recent_from);
+  // every slot before the budget as it is; those that are evicted are overwritten below
+  if (copy_w)
+#pragma unroll 4
+    for (int i = threadIdx.x; i < a.budget; i += kRankThreads) wo[i] = w[i];
+  if (copy_p)
+#pragma unroll 4
+    for (int i = threadIdx.x; i < a.budget; i += kRankThreads) po[i] = pos[i];
+  auto key = [&](int i) { return held ? s_key[i] : rank_key(w[i], pos[i], a.sinks, recent_from); };
   uint32_t prefix = 0, known = 0;
   int need = a.budget;                                           // slots still wanted among those with this prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kRankThreads) s_hist[i] = 0;
+#pragma unroll
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+    const uint32_t bins = digit < 2 ? 2047u : 1023u;
+    for (int i = threadIdx.x; i < kBins; i += kRankThreads) s_hist[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < len; i += kRankThreads) {
       const uint32_t k = key(i);
-      if ((k & known) == prefix) atomicAdd(&s_hist[k >> shift & 255], 1);
+      if ((k & known) == prefix) atomicAdd(&s_hist[k >> shift & bins], 1);
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      int left = need, d = 255;
-      while (d > 0 && s_hist[d] < left) left -= s_hist[d--];
-      s_digit = d;
-      s_left = left;
+    // thread t takes bins 2047 - 2t and the one below: the digit is the bin where the count from the top reaches need
+    const int hi = s_hist[kBins - 1 - 2 * threadIdx.x], lo = s_hist[kBins - 2 - 2 * threadIdx.x];
+    int sum = hi + lo;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    int2 all;
+    const int above = warps_before(__shfl_sync(0xFFFFFFFFu, sum, 31), 0, s_warp, &all).x + sum - hi - lo;
+    if (above < need && above + hi + lo >= need) {
+      const bool first = above + hi >= need;
+      s_digit = kBins - 1 - 2 * threadIdx.x - !first;
+      s_left = need - above - (first ? 0 : hi);
+      s_count = first ? hi : lo;
     }
     __syncthreads();
-    prefix |= s_digit << shift;
-    known |= 255u << shift;
+    prefix |= (uint32_t)s_digit << shift;
+    known |= bins << shift;
     need = s_left;
   }
-  // `need` slots of key `prefix` stay, from the lowest on, and every slot of a larger key
+  // every slot of a larger key than `prefix` stays, and `need` of the s_count slots with that key, from the lowest on
+  const bool some = need < s_count;
   const int run = (len + 32 * kRankWarps - 1) / (32 * kRankWarps) * 32;
   const int from = min(len, warp * run), to = min(len, from + run);
-  int ties = 0, all = 0;
-  for (int i = from + lane; i - lane < to; i += 32)
-    ties += __popc(__ballot_sync(0xFFFFFFFFu, i < to && key(i) == prefix));
-  const int ties0 = warps_before(ties, s_warp, &all);
   const uint32_t below = (1u << lane) - 1;
-  int n_out = 0, n_in = 0;
+  int2 all = make_int2(0, 0);
+  int ties0 = 0;
+  if (some) {
+    int ties = 0;
+    for (int i = from + lane; i - lane < to; i += 32) ties += __popc(__ballot_sync(0xFFFFFFFFu, i < to && key(i) == prefix));
+    ties0 = warps_before(ties, 0, s_warp, &all).x;
+  }
+  int2 at0 = make_int2(0, 0);
   for (int pass = 0; pass < 2; ++pass) {
-    int t = ties0, out0 = 0, in0 = 0;
-    if (pass) {
-      out0 = warps_before(n_out, s_warp, &all);
-      in0 = warps_before(n_in, s_warp, &all);
-      if (threadIdx.x == 0) mv.n[row] = all;
-    }
+    int t = ties0, out = at0.x, in = at0.y;
     for (int i = from + lane; i - lane < to; i += 32) {
       const bool on = i < to;
       const uint32_t k = on ? key(i) : 0;
       const uint32_t tie = __ballot_sync(0xFFFFFFFFu, on && k == prefix);
-      const bool stay = on && (k > prefix || (k == prefix && t + __popc(tie & below) < need));
+      const bool stay = on && (k > prefix || (k == prefix && (!some || t + __popc(tie & below) < need)));
       t += __popc(tie);
       const uint32_t leave = __ballot_sync(0xFFFFFFFFu, on && !stay && i < a.budget);
       const uint32_t move = __ballot_sync(0xFFFFFFFFu, stay && i >= a.budget);
       if (pass) {
-        int2* at = mv.at + (int64_t)row * mv.most;
-        if (leave >> lane & 1) at[out0 + __popc(leave & below)].y = i;
-        if (move >> lane & 1) at[in0 + __popc(move & below)].x = i;
-        if (stay && i < a.budget) {
-          if (copy_w) wo[i] = w[i];
-          if (copy_p) po[i] = pos[i];
-        }
+        int2* at = all.y <= kFewMoves ? s_few : mv.at + (int64_t)row * mv.most;
+        if (leave >> lane & 1) at[out + __popc(leave & below)].y = i;
+        if (move >> lane & 1) at[in + __popc(move & below)].x = i;
       }
-      out0 += __popc(leave);
-      in0 += __popc(move);
+      out += __popc(leave);
+      in += __popc(move);
     }
-    n_out = out0;
-    n_in = in0;
+    if (!pass) at0 = warps_before(out, in, s_warp, &all);
   }
   __syncthreads();
-  const int2* at = mv.at + (int64_t)row * mv.most;
-  for (int i = threadIdx.x; i < all; i += kRankThreads) {
+  const int n = all.y;
+  const bool few = n <= kFewMoves;
+  const int2* at = few ? s_few : mv.at + (int64_t)row * mv.most;
+  for (int i = threadIdx.x; i < n; i += kRankThreads) {
     const int2 m = at[i];
     wo[m.y] = w[m.x];
     po[m.y] = pos[m.x];
   }
+  if (few) {
+    const int pieces = c.hd / 8;
+    for (int u = threadIdx.x; u < n * pieces; u += kRankThreads)
+      move_piece(c, b, row - b * c.n_kv, s_few[u / pieces], u % pieces * 8);
+  }
+  if (threadIdx.x == 0) mv.n[row] = few ? 0 : n;
 }
 
-// The rows of the moves: a quarter of a warp's lanes (or as many as a row has 16-byte pieces) per
-// row, keys and values. Sources lie at or behind the budget, destinations before it.
+// The rows of the longer lists, 16 bytes a thread, and the new lengths (every CTA of k_rank has read the old ones).
 constexpr int kMoveThreads = 256;
 __global__ void __launch_bounds__(kMoveThreads) k_move(EvictArgs a, Moves mv) {
   const KvCache& c = a.c;
+  griddep_wait();
   const int row = blockIdx.x, b = row / c.n_kv, h = row - b * c.n_kv;
   if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
     const int len = kv_length(c, b, kErrEvict);
@@ -242,59 +286,79 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(EvictArgs a, Moves mv) {
   const int pieces = c.hd / 8, n = mv.n[row];
   const int64_t all = (int64_t)n * pieces;
   for (int64_t u = (int64_t)blockIdx.y * kMoveThreads + threadIdx.x; u < all; u += (int64_t)gridDim.y * kMoveThreads) {
-    const int i = (int)(u / pieces), e = (int)(u - (int64_t)i * pieces) * 8;
-    const int2 m = mv.at[(int64_t)row * mv.most + i];
-    const int ps = kv_page(c, b, m.x, kErrEvict), pd = kv_page(c, b, m.y, kErrEvict);
-    if (ps < 0 || pd < 0) continue;
-    const int64_t s = kv_offset(c, ps, m.x, h) + e, d = kv_offset(c, pd, m.y, h) + e;
-    const uint4 k = *reinterpret_cast<const uint4*>(c.k + 2 * s), v = *reinterpret_cast<const uint4*>(c.v + 2 * s);
-    *reinterpret_cast<uint4*>(c.k + 2 * d) = k;
-    *reinterpret_cast<uint4*>(c.v + 2 * d) = v;
+    const int i = (int)(u / pieces);
+    move_piece(c, b, h, mv.at[(int64_t)row * mv.most + i], (int)(u - (int64_t)i * pieces) * 8);
   }
 }
 
 // ------------------------------------------------------------------------------ logits rules
-// A row is spread over a cluster of kRuleCluster CTAs; a CTA takes its share in slices. A slice has one
-// word per token in shared memory: bits 0-19 how often it was generated, bit 20 that it is in the
-// prompt, bits 21-31 the last bias entry that lists it. Filling the words reads the whole history (a
-// few KB out of L2) and keeps what falls into the slice; then the logits pass once, read and
-// written, and the greedy candidates are combined over the cluster.
-constexpr int kRuleCluster = 8, kRuleThreads = 512;
+// A row is spread over a cluster of CTAs; a CTA takes its share in slices of 16 tokens a thread. The
+// slice's logits are requested first (4 x 16 bytes a thread in flight), and while they come the slice's
+// words are filled in shared memory, one per token: bits 0-19 how often it was generated, bit 20 that
+// it is in the prompt, bits 21-31 the last bias entry that lists it; the tokens met for the first time
+// go on a list. That reads the whole history (a few KB out of L2) and keeps what falls into the slice.
+// Then the logits are masked and stored as they stream, and the listed tokens, few of many, are changed
+// afterwards, a thread each: divisions and bias reads inside the stream made it three times as long.
+// Each thread keeps its best group of four; the candidates are combined over the cluster and the
+// winning group is read once more for the token. Bound by memory: 8 bytes a token and the mask.
 constexpr uint32_t kRulePrompt = 1u << 20, kRuleCount = kRulePrompt - 1;
+constexpr int kGroups = 4;                       // groups of four tokens a thread takes of a slice
+constexpr int kRuleThreadsMax = 1024;
 
 struct RowRules {
   float rep, pres, freq;
   const float* bias;
-  bool any;
 };
 __device__ __forceinline__ float rule(float x, uint32_t w, const RowRules& r) {
-  if (w) {
-    const uint32_t n = w & kRuleCount;
-    if (w & (kRulePrompt | kRuleCount)) x = x > 0.0f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
-    if (n) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.freq, (float)n)), r.pres);
-    if (w >> 21) x = __fadd_rn(x, __ldg(r.bias + (w >> 21) - 1));
-  }
+  const uint32_t n = w & kRuleCount;
+  if (w & (kRulePrompt | kRuleCount)) x = x > 0.0f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
+  if (n) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.freq, (float)n)), r.pres);
+  if (w >> 21) x = __fadd_rn(x, __ldg(r.bias + (w >> 21) - 1));
   return x;
 }
-__device__ __forceinline__ void pick_allowed(Pick& p, float v, int j, uint32_t allowed) {
-  const int vn = is_nan(v);
-  const bool take = allowed & ((p.i < 0) | (vn & !p.nan) | (!p.nan & !vn & (v > p.v)));
-  p.v = take ? v : p.v;
-  p.i = take ? j : p.i;
-  p.nan = take ? vn : p.nan;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
 }
+// The words of a slice's tokens and the list of those that are not zero.
+struct Slice {
+  uint32_t* word;
+  uint16_t* list;
+  int* listed;
+  int s0, n;
+  __device__ __forceinline__ void first(unsigned t) const { list[atomicAdd(listed, 1)] = (uint16_t)t; }
+  __device__ __forceinline__ void count(int id, bool prompt) const {
+    const unsigned t = (unsigned)id - (unsigned)s0;
+    if (t < (unsigned)n && !(prompt ? atomicOr(&word[t], kRulePrompt) : atomicAdd(&word[t], 1u))) first(t);
+  }
+  __device__ __forceinline__ void bias(int id, int entry) const {
+    const unsigned t = (unsigned)id - (unsigned)s0;
+    if (t >= (unsigned)n) return;
+    uint32_t was = word[t], now;
+    do {
+      now = was;
+      if (was >> 21 > (uint32_t)entry) return;   // a later entry is there already
+      was = atomicCAS(&word[t], now, (now & (kRulePrompt | kRuleCount)) | (uint32_t)(entry + 1) << 21);
+    } while (was != now);
+    if (!now) first(t);
+  }
+};
 
+// VEC: rows of logits and out start on 16-byte boundaries.
 template <bool VEC>
-__global__ void __launch_bounds__(kRuleThreads) k_adjust(tc_logits_rules a, int share, int slice) {
+__global__ void __launch_bounds__(kRuleThreadsMax) k_adjust(const __grid_constant__ tc_logits_rules a, int cluster, int share) {
   extern __shared__ uint32_t s_word[];
-  __shared__ Pick s_warp[kRuleThreads / 32];
-  __shared__ int s_cand[3];
-  const int row = blockIdx.x / kRuleCluster, rank = (int)cluster_rank();
-  const int lo = min(a.vocab, rank * share), hi = min(a.vocab, lo + share);
+  __shared__ Pick s_warp[kRuleThreadsMax / 32];
+  __shared__ int s_cand[3], s_listed;
+  const int row = blockIdx.x / cluster, rank = (int)cluster_rank(), threads = blockDim.x;
+  const int lo = min(a.vocab, rank * share), hi = min(a.vocab, lo + share), slice = 4 * kGroups * threads;
+  const int slice_words = min(share, slice);
   const float* x = a.logits + (int64_t)row * a.logits_stride;
   float* y = a.out + (int64_t)row * a.out_stride;
   const uint32_t* mask = a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr;
   const int* hist = a.history ? a.history + (int64_t)row * a.history_stride : nullptr;
+  const bool hist4 = ((uintptr_t)hist & 15) == 0;
   int n_all = 0, n_first = 0;
   if (hist) {
     n_all = a.n_history ? min(max(__ldg(a.n_history + row), 0), a.max_history) : a.max_history;
@@ -306,93 +370,131 @@ __global__ void __launch_bounds__(kRuleThreads) k_adjust(tc_logits_rules a, int 
   r.pres = a.presence ? __ldg(a.presence + row) : 0.0f;
   r.freq = a.frequency ? __ldg(a.frequency + row) : 0.0f;
   r.bias = ids ? a.bias + (int64_t)row * a.bias_stride : nullptr;
-  r.any = n_all > 0 || ids;
-  Pick p[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) p[u] = Pick{0.0f, -1, 0};
+  const bool any = n_all > 0 || ids;
+  const float none = __int_as_float(0xFF800000);
+  float best = none;                             // the best group's value and first token (-1: all -infinity so far)
+  int best_at = -1;
+  // of two groups of one value the first counts (a thread meets its groups out of order)
+  auto consider = [&](float v, int j) {
+    const bool take = best == best && (!(v <= best) || (v == best && best_at >= 0 && j < best_at));
+    best = take ? v : best;
+    best_at = take ? j : best_at;
+  };
   for (int s0 = lo; s0 < hi; s0 += slice) {
     const int s1 = min(hi, s0 + slice), n = s1 - s0;
-    if (r.any) {
-      for (int i = threadIdx.x; i < n; i += kRuleThreads) s_word[i] = 0;
-      __syncthreads();
-      if (ids) {
-        for (int i = threadIdx.x; i < a.n_bias; i += kRuleThreads) {
-          const unsigned t = (unsigned)__ldg(ids + i) - (unsigned)s0;
-          if (t < (unsigned)n) atomicMax(&s_word[t], (uint32_t)(i + 1) << 21);
-        }
-        __syncthreads();
-      }
-      for (int i = threadIdx.x; i < n_all; i += kRuleThreads) {
-        const unsigned t = (unsigned)__ldg(hist + i) - (unsigned)s0;
-        if (t < (unsigned)n) {
-          if (i < n_first) atomicOr(&s_word[t], kRulePrompt);
-          else atomicAdd(&s_word[t], 1u);
-        }
-      }
-      __syncthreads();
-    }
-    if (VEC) {
-      // s0 is a multiple of 32: a vector's four tokens share a mask word
-      for (int j = s0 + 4 * threadIdx.x; j < s1; j += 4 * kRuleThreads) {
-        const uint32_t bits = mask ? __ldg(mask + (j >> 5)) >> (j & 31) : 15u;
-        if (j + 4 <= s1) {
-          float4 f = *reinterpret_cast<const float4*>(x + j);
-          float e[4] = {f.x, f.y, f.z, f.w};
-          if (r.any) {
-            const uint4 w = *reinterpret_cast<const uint4*>(s_word + (j - s0));
-            e[0] = rule(e[0], w.x, r);
-            e[1] = rule(e[1], w.y, r);
-            e[2] = rule(e[2], w.z, r);
-            e[3] = rule(e[3], w.w, r);
-          }
+    float e[kGroups][4];
+    uint32_t bits[kGroups];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            pick_allowed(p[u], e[u], j + u, bits >> u & 1);
-            if (!(bits >> u & 1)) e[u] = __int_as_float(0xFF800000);
-          }
-          *reinterpret_cast<float4*>(y + j) = make_float4(e[0], e[1], e[2], e[3]);
-        } else {
-          for (int u = 0; j + u < s1; ++u) {
-            float e = x[j + u];
-            if (r.any) e = rule(e, s_word[j + u - s0], r);
-            pick_allowed(p[0], e, j + u, bits >> u & 1);
-            y[j + u] = bits >> u & 1 ? e : __int_as_float(0xFF800000);
-          }
-        }
-      }
-    } else {
-      for (int j = s0 + threadIdx.x; j < s1; j += kRuleThreads) {
-        const uint32_t ok = mask ? __ldg(mask + (j >> 5)) >> (j & 31) & 1 : 1u;
-        float e = x[j];
-        if (r.any) e = rule(e, s_word[j - s0], r);
-        pick_allowed(p[0], e, j, ok);
-        y[j] = ok ? e : __int_as_float(0xFF800000);
+    for (int g = 0; g < kGroups; ++g) {
+      const int j = s0 + 4 * (threadIdx.x + g * threads);        // s0 is a multiple of 32: one mask word a group
+      bits[g] = mask && j < s1 ? __ldg(mask + (j >> 5)) >> (j & 31) : 15u;
+      if (VEC && j + 4 <= s1) {
+        const float4 f = *reinterpret_cast<const float4*>(x + j);
+        e[g][0] = f.x; e[g][1] = f.y; e[g][2] = f.z; e[g][3] = f.w;
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) e[g][u] = j + u < s1 ? x[j + u] : none;
       }
     }
-    __syncthreads();
+    const Slice sl{s_word, reinterpret_cast<uint16_t*>(s_word + slice_words), &s_listed, s0, n};
+    if (any) {
+      for (int i = 4 * threadIdx.x; i < n; i += 4 * threads) *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
+      if (threadIdx.x == 0) s_listed = 0;
+      __syncthreads();
+      if (ids)
+        for (int i = threadIdx.x; i < a.n_bias; i += threads) sl.bias(__ldg(ids + i), i);
+      int i0 = 0;
+      if (hist4) {
+        i0 = n_all & ~3;
+#pragma unroll 2
+        for (int i = 4 * threadIdx.x; i < i0; i += 4 * threads) {
+          const int4 t = __ldg(reinterpret_cast<const int4*>(hist + i));
+          sl.count(t.x, i < n_first);
+          sl.count(t.y, i + 1 < n_first);
+          sl.count(t.z, i + 2 < n_first);
+          sl.count(t.w, i + 3 < n_first);
+        }
+      }
+#pragma unroll 4
+      for (int i = i0 + threadIdx.x; i < n_all; i += threads) sl.count(__ldg(hist + i), i < n_first);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int j = s0 + 4 * (threadIdx.x + g * threads);
+      if (j < s1) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) e[g][u] = bits[g] >> u & 1 ? e[g][u] : none;
+        if (VEC && j + 4 <= s1) {
+          *reinterpret_cast<float4*>(y + j) = make_float4(e[g][0], e[g][1], e[g][2], e[g][3]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (j + u < s1) y[j + u] = e[g][u];
+        }
+        if (any) {                               // listed tokens come below
+          const uint4 w = *reinterpret_cast<const uint4*>(s_word + (j - s0));
+          e[g][0] = w.x ? none : e[g][0];
+          e[g][1] = w.y ? none : e[g][1];
+          e[g][2] = w.z ? none : e[g][2];
+          e[g][3] = w.w ? none : e[g][3];
+        }
+        consider(max_nan(max_nan(e[g][0], e[g][1]), max_nan(e[g][2], e[g][3])), j);
+      }
+    }
+    if (any) {
+      __syncthreads();                           // the slice is stored
+      for (int i = threadIdx.x; i < s_listed; i += threads) {
+        const int t = sl.list[i], j = s0 + t;
+        if (mask && !(__ldg(mask + (j >> 5)) >> (j & 31) & 1)) continue;
+        const float v = rule(*(volatile const float*)(y + j), s_word[t], r);
+        y[j] = v;
+        consider(v, j & ~3);
+      }
+      __syncthreads();
+    }
   }
   if (!a.token) return;
-  Pick m = pick_comb(pick_comb(p[0], p[1]), pick_comb(p[2], p[3]));
+  Pick m{best, best_at, is_nan(best)};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = pick_comb(m, pick_shfl(m, o));
   if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
     Pick t = s_warp[0];
-    for (int w = 1; w < kRuleThreads / 32; ++w) t = pick_comb(t, s_warp[w]);
+    for (int w = 1; w < threads / 32; ++w) t = pick_comb(t, s_warp[w]);
     s_cand[0] = __float_as_int(t.v);
     s_cand[1] = t.i;
     s_cand[2] = t.nan;
   }
-  cluster_sync();
+  cluster_sync();                                // (orders the stores of out before the read below as well)
   if (rank == 0 && threadIdx.x == 0) {
     Pick t{__int_as_float(s_cand[0]), s_cand[1], s_cand[2]};
-    for (int q = 1; q < kRuleCluster; ++q) {
+    for (int q = 1; q < cluster; ++q) {
       const Pick u{__int_as_float(dsmem_ld_s32(smem_u32(&s_cand[0]), q)), dsmem_ld_s32(smem_u32(&s_cand[1]), q),
                    dsmem_ld_s32(smem_u32(&s_cand[2]), q)};
       t = pick_comb(t, u);
     }
-    a.token[row] = t.i < 0 ? a.none : t.i;
+    int token = a.none;
+    if (t.i >= 0) {
+      token = t.i;
+      for (int u = 3; u >= 0; --u)               // the group's first NaN, or first entry of its value
+        if (t.i + u < a.vocab) {
+          const float v = *(volatile const float*)(y + t.i + u);
+          if (t.nan ? is_nan(v) : v == t.v) token = t.i + u;
+        }
+    } else if (!mask) {
+      token = 0;                                 // a row of -infinity alone: the first token
+    } else {
+      for (int i = 0; i < (a.vocab + 31) / 32 && token == a.none; ++i) {
+        const uint32_t word = __ldg(mask + i) & (a.vocab - 32 * i >= 32 ? ~0u : (1u << (a.vocab - 32 * i)) - 1);
+        if (word) {
+          token = 32 * i + __ffs(word) - 1;      // allowed tokens that are all -infinity: the first of them
+          break;
+        }
+      }
+    }
+    a.token[row] = token;
   }
   cluster_sync();                                // no CTA leaves while its candidate is read
 }
@@ -412,23 +514,40 @@ uint64_t evict_workspace(const KvCache& c, int budget) {
 cudaError_t launch_evict(const EvictArgs& a, cudaStream_t st) {
   const int rows = a.c.batch * a.c.n_kv;
   const Moves mv = moves_of(a.ws, rows, most_moves(a.c.max_pages << a.c.shift, a.budget));
-  k_rank<<<rows, kRankThreads, 0, st>>>(a, mv);
-  cudaError_t e = cudaGetLastError();
+  const int room = std::min(a.c.max_pages << a.c.shift, kKeysMax);
+  cudaError_t e = allow_smem<k_rank>(kKeysMax * 4);
+  if (e != cudaSuccess) return e;
+  k_rank<<<rows, kRankThreads, room * 4, st>>>(a, mv, room);
+  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int64_t pieces = (int64_t)std::max(1, mv.most) * (a.c.hd / 8);
   const int blocks = (int)std::min<int64_t>((pieces + kMoveThreads - 1) / kMoveThreads, std::max(1, 148 * 8 / rows));
-  k_move<<<dim3(rows, blocks), kMoveThreads, 0, st>>>(a, mv);
-  return cudaGetLastError();
+  return launch_dependent(k_move, dim3(rows, blocks), dim3(kMoveThreads), st, a, mv);
 }
 
 cudaError_t launch_adjust(const tc_logits_rules& r, cudaStream_t st) {
-  const int share = ((r.vocab + kRuleCluster - 1) / kRuleCluster + 31) / 32 * 32;
-  // 32 KB of words leave room for several CTAs an SM, so that one fills its words while another streams
-  const int slice = std::min(share, 8192);
   const bool vec = ((uintptr_t)r.logits | (uintptr_t)r.out) % 16 == 0 && r.logits_stride % 4 == 0 && r.out_stride % 4 == 0;
+  // few rows: 16 CTAs of 1024 threads a row, whose share is one slice up to 262144 tokens; many rows: 8 CTAs of
+  // 512 threads, several to an SM, so that one fills its words while another streams
+  const bool few = r.rows * 8 <= 148;
+  const int cluster = few ? 16 : 8, threads = few ? 1024 : 512;
+  const int share = ((r.vocab + cluster - 1) / cluster + 31) / 32 * 32;
+  const int smem = std::min(share, 4 * kGroups * threads) * 6;   // a word and a list entry a token
   auto kern = vec ? k_adjust<true> : k_adjust<false>;
-  const int smem = slice * 4;
-  return launch_ex(kern, dim3(r.rows * kRuleCluster), dim3(kRuleThreads), smem, st, kRuleCluster, r, share, slice);
+  static std::atomic<uint64_t> wide{0};          // devices on which clusters of 16 and the words are allowed
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(wide.load() >> dev & 1)) {
+    for (auto k : {k_adjust<true>, k_adjust<false>}) {
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kGroups * kRuleThreadsMax * 6);
+      if (e != cudaSuccess) return e;
+    }
+    if (dev < 64) wide.fetch_or(1ull << dev);
+  }
+  return launch_ex(kern, dim3((unsigned)r.rows * cluster), dim3(threads), smem, st, cluster, r, cluster, share);
 }
 
 }  // namespace tc
