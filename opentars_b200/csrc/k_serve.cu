@@ -292,28 +292,28 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(EvictArgs a, Moves mv) {
 }
 
 // ------------------------------------------------------------------------------ logits rules
-// A row is spread over a cluster of CTAs; a CTA takes its share in slices of 16 tokens a thread. The
-// slice's logits are requested first (4 x 16 bytes a thread in flight), and while they come the slice's
-// words are filled in shared memory, one per token: bits 0-19 how often it was generated, bit 20 that
-// it is in the prompt, bits 21-31 the last bias entry that lists it; the tokens met for the first time
-// go on a list. That reads the whole history (a few KB out of L2) and keeps what falls into the slice.
-// Then the logits are masked and stored as they stream, and the listed tokens, few of many, are changed
-// afterwards, a thread each: divisions and bias reads inside the stream made it three times as long.
-// Each thread keeps its best group of four; the candidates are combined over the cluster and the
-// winning group is read once more for the token. Bound by memory: 8 bytes a token and the mask.
-constexpr uint32_t kRulePrompt = 1u << 20, kRuleCount = kRulePrompt - 1;
-constexpr int kGroups = 4;                       // groups of four tokens a thread takes of a slice
-constexpr int kRuleThreadsMax = 1024;
+// A row is spread over a cluster of CTAs. A CTA first fills, in shared memory, one word per token of its
+// share (or of a slice of it): how often it was generated, whether it is in the prompt, whether a bias
+// lists it; the tokens met for the first time go on a list. That reads the whole history (a few KB out
+// of L2) and keeps what falls into the share. Then the logits are masked and stored as they stream,
+// without a barrier, and the listed tokens, few of many, are changed afterwards, a thread each
+// (divisions and bias reads inside the stream made it three times as long). Each thread keeps its
+// best group of four; the candidates are combined over the cluster and the winning group is read once
+// more for the token. Words of 16 bits for histories below 2^14 ids, so that four CTAs share an SM.
+// Bound by memory: 8 bytes a token and the mask.
+template <class Word>
+struct Bits {
+  static constexpr uint32_t kListed = 1u << (8 * sizeof(Word) - 1), kPrompt = kListed >> 1, kCount = kPrompt - 1;
+};
 
 struct RowRules {
   float rep, pres, freq;
-  const float* bias;
 };
-__device__ __forceinline__ float rule(float x, uint32_t w, const RowRules& r) {
-  const uint32_t n = w & kRuleCount;
-  if (w & (kRulePrompt | kRuleCount)) x = x > 0.0f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
+template <class Word>
+__device__ __forceinline__ float penalties(float x, uint32_t w, const RowRules& r) {
+  const uint32_t n = w & Bits<Word>::kCount;
+  if (w & (Bits<Word>::kPrompt | Bits<Word>::kCount)) x = x > 0.0f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
   if (n) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.freq, (float)n)), r.pres);
-  if (w >> 21) x = __fadd_rn(x, __ldg(r.bias + (w >> 21) - 1));
   return x;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -321,39 +321,33 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
   return m;
 }
-// The words of a slice's tokens and the list of those that are not zero.
+// The words of a slice's tokens and the list of those that are not zero (16-bit words are changed in pairs).
+template <class Word>
 struct Slice {
   uint32_t* word;
   uint16_t* list;
   int* listed;
   int s0, n;
-  __device__ __forceinline__ void first(unsigned t) const { list[atomicAdd(listed, 1)] = (uint16_t)t; }
-  __device__ __forceinline__ void count(int id, bool prompt) const {
-    const unsigned t = (unsigned)id - (unsigned)s0;
-    if (t < (unsigned)n && !(prompt ? atomicOr(&word[t], kRulePrompt) : atomicAdd(&word[t], 1u))) first(t);
-  }
-  __device__ __forceinline__ void bias(int id, int entry) const {
+  __device__ __forceinline__ uint32_t get(int t) const { return reinterpret_cast<const Word*>(word)[t]; }
+  __device__ __forceinline__ void set(int t, uint32_t v) const { reinterpret_cast<Word*>(word)[t] = (Word)v; }
+  __device__ __forceinline__ void mark(int id, uint32_t bit, bool add) const {
     const unsigned t = (unsigned)id - (unsigned)s0;
     if (t >= (unsigned)n) return;
-    uint32_t was = word[t], now;
-    do {
-      now = was;
-      if (was >> 21 > (uint32_t)entry) return;   // a later entry is there already
-      was = atomicCAS(&word[t], now, (now & (kRulePrompt | kRuleCount)) | (uint32_t)(entry + 1) << 21);
-    } while (was != now);
-    if (!now) first(t);
+    const int at = sizeof(Word) == 2 ? t >> 1 : t, shift = sizeof(Word) == 2 ? (t & 1) * 16 : 0;
+    const uint32_t was = add ? atomicAdd(&word[at], 1u << shift) : atomicOr(&word[at], bit << shift);
+    if (!(Word)(was >> shift)) list[atomicAdd(listed, 1)] = (uint16_t)t;
   }
 };
 
-// VEC: rows of logits and out start on 16-byte boundaries.
-template <bool VEC>
-__global__ void __launch_bounds__(kRuleThreadsMax) k_adjust(const __grid_constant__ tc_logits_rules a, int cluster, int share) {
+// VEC: rows of logits and out start on 16-byte boundaries. GROUPS: groups of four tokens a thread has in flight.
+template <bool VEC, class Word, int GROUPS, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS)
+    k_adjust(const __grid_constant__ tc_logits_rules a, int cluster, int share, int slice) {
   extern __shared__ uint32_t s_word[];
-  __shared__ Pick s_warp[kRuleThreadsMax / 32];
+  __shared__ Pick s_warp[THREADS / 32];
   __shared__ int s_cand[3], s_listed;
-  const int row = blockIdx.x / cluster, rank = (int)cluster_rank(), threads = blockDim.x;
-  const int lo = min(a.vocab, rank * share), hi = min(a.vocab, lo + share), slice = 4 * kGroups * threads;
-  const int slice_words = min(share, slice);
+  const int row = blockIdx.x / cluster, rank = (int)cluster_rank(), lane = threadIdx.x & 31;
+  const int lo = min(a.vocab, rank * share), hi = min(a.vocab, lo + share);
   const float* x = a.logits + (int64_t)row * a.logits_stride;
   float* y = a.out + (int64_t)row * a.out_stride;
   const uint32_t* mask = a.mask ? a.mask + (int64_t)row * a.mask_stride : nullptr;
@@ -365,11 +359,11 @@ __global__ void __launch_bounds__(kRuleThreadsMax) k_adjust(const __grid_constan
     n_first = a.n_prompt ? min(max(__ldg(a.n_prompt + row), 0), n_all) : 0;
   }
   const int* ids = a.bias_ids ? a.bias_ids + (int64_t)row * a.bias_stride : nullptr;
+  const float* bias = ids ? a.bias + (int64_t)row * a.bias_stride : nullptr;
   RowRules r;
   r.rep = a.repetition ? __ldg(a.repetition + row) : 1.0f;
   r.pres = a.presence ? __ldg(a.presence + row) : 0.0f;
   r.freq = a.frequency ? __ldg(a.frequency + row) : 0.0f;
-  r.bias = ids ? a.bias + (int64_t)row * a.bias_stride : nullptr;
   const bool any = n_all > 0 || ids;
   const float none = __int_as_float(0xFF800000);
   float best = none;                             // the best group's value and first token (-1: all -infinity so far)
@@ -382,74 +376,110 @@ __global__ void __launch_bounds__(kRuleThreadsMax) k_adjust(const __grid_constan
   };
   for (int s0 = lo; s0 < hi; s0 += slice) {
     const int s1 = min(hi, s0 + slice), n = s1 - s0;
-    float e[kGroups][4];
-    uint32_t bits[kGroups];
+    float e[GROUPS][4];
+    uint32_t bits[GROUPS];
+    auto request = [&](int j0) {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const int j = s0 + 4 * (threadIdx.x + g * threads);        // s0 is a multiple of 32: one mask word a group
-      bits[g] = mask && j < s1 ? __ldg(mask + (j >> 5)) >> (j & 31) : 15u;
-      if (VEC && j + 4 <= s1) {
-        const float4 f = *reinterpret_cast<const float4*>(x + j);
-        e[g][0] = f.x; e[g][1] = f.y; e[g][2] = f.z; e[g][3] = f.w;
-      } else {
+      for (int g = 0; g < GROUPS; ++g) {
+        const int j = j0 + 4 * (threadIdx.x + g * THREADS);      // slices begin at multiples of 32: one mask word a group
+        bits[g] = mask && j < s1 ? __ldg(mask + (j >> 5)) : ~0u;
+        if (VEC && j + 4 <= s1) {
+          const float4 f = *reinterpret_cast<const float4*>(x + j);
+          e[g][0] = f.x; e[g][1] = f.y; e[g][2] = f.z; e[g][3] = f.w;
+        } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) e[g][u] = j + u < s1 ? x[j + u] : none;
+          for (int u = 0; u < 4; ++u) e[g][u] = j + u < s1 ? x[j + u] : none;
+        }
       }
-    }
-    const Slice sl{s_word, reinterpret_cast<uint16_t*>(s_word + slice_words), &s_listed, s0, n};
+    };
+    request(s0);                                 // on their way while the words are filled
+    int* last = reinterpret_cast<int*>(s_word) + slice * (int)sizeof(Word) / 4;     // of a listed token: its last bias entry
+    const Slice<Word> sl{s_word, reinterpret_cast<uint16_t*>(last + a.n_bias), &s_listed, s0, n};
+    int biased = 0;
     if (any) {
-      for (int i = 4 * threadIdx.x; i < n; i += 4 * threads) *reinterpret_cast<uint4*>(s_word + i) = make_uint4(0, 0, 0, 0);
+      const int words = (n * (int)sizeof(Word) + 15) / 16;       // (a slice's words are a multiple of 16 bytes)
+      for (int i = threadIdx.x; i < words; i += THREADS) reinterpret_cast<uint4*>(s_word)[i] = make_uint4(0, 0, 0, 0);
       if (threadIdx.x == 0) s_listed = 0;
       __syncthreads();
-      if (ids)
-        for (int i = threadIdx.x; i < a.n_bias; i += threads) sl.bias(__ldg(ids + i), i);
+      if (ids) {
+        // the listed tokens come first on the list; each one's last entry is found by its place there, which
+        // its word holds meanwhile
+        for (int i = threadIdx.x; i < a.n_bias; i += THREADS) sl.mark(__ldg(ids + i), Bits<Word>::kListed, false);
+        __syncthreads();
+        biased = s_listed;
+        for (int i = threadIdx.x; i < biased; i += THREADS) {
+          sl.set(sl.list[i], i);
+          last[i] = 0;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.n_bias; i += THREADS) {
+          const unsigned t = (unsigned)__ldg(ids + i) - (unsigned)s0;
+          if (t < (unsigned)n) atomicMax(&last[sl.get(t)], i);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < biased; i += THREADS) sl.set(sl.list[i], Bits<Word>::kListed);
+        __syncthreads();
+      }
       int i0 = 0;
       if (hist4) {
         i0 = n_all & ~3;
 #pragma unroll 2
-        for (int i = 4 * threadIdx.x; i < i0; i += 4 * threads) {
+        for (int i = 4 * threadIdx.x; i < i0; i += 4 * THREADS) {
           const int4 t = __ldg(reinterpret_cast<const int4*>(hist + i));
-          sl.count(t.x, i < n_first);
-          sl.count(t.y, i + 1 < n_first);
-          sl.count(t.z, i + 2 < n_first);
-          sl.count(t.w, i + 3 < n_first);
+          sl.mark(t.x, Bits<Word>::kPrompt, i >= n_first);
+          sl.mark(t.y, Bits<Word>::kPrompt, i + 1 >= n_first);
+          sl.mark(t.z, Bits<Word>::kPrompt, i + 2 >= n_first);
+          sl.mark(t.w, Bits<Word>::kPrompt, i + 3 >= n_first);
         }
       }
 #pragma unroll 4
-      for (int i = i0 + threadIdx.x; i < n_all; i += threads) sl.count(__ldg(hist + i), i < n_first);
+      for (int i = i0 + threadIdx.x; i < n_all; i += THREADS) sl.mark(__ldg(hist + i), Bits<Word>::kPrompt, i >= n_first);
       __syncthreads();
     }
+    for (int j0 = s0; j0 < s1; j0 += 4 * GROUPS * THREADS) {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const int j = s0 + 4 * (threadIdx.x + g * threads);
-      if (j < s1) {
+      for (int g = 0; g < GROUPS; ++g) {
+        const int j = j0 + 4 * (threadIdx.x + g * THREADS);
+        if (j < s1) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) e[g][u] = bits[g] >> u & 1 ? e[g][u] : none;
-        if (VEC && j + 4 <= s1) {
-          *reinterpret_cast<float4*>(y + j) = make_float4(e[g][0], e[g][1], e[g][2], e[g][3]);
-        } else {
+          for (int u = 0; u < 4; ++u) e[g][u] = bits[g] >> ((j & 31) + u) & 1 ? e[g][u] : none;
+          if (VEC && j + 4 <= s1) {
+            *reinterpret_cast<float4*>(y + j) = make_float4(e[g][0], e[g][1], e[g][2], e[g][3]);
+          } else {
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (j + u < s1) y[j + u] = e[g][u];
+            for (int u = 0; u < 4; ++u)
+              if (j + u < s1) y[j + u] = e[g][u];
+          }
+          if (any) {                             // listed tokens come below
+            uint32_t w[4];
+            if constexpr (sizeof(Word) == 2) {
+              const uint2 v = *reinterpret_cast<const uint2*>(s_word + (j - s0) / 2);
+              w[0] = v.x & 0xFFFFu; w[1] = v.x >> 16; w[2] = v.y & 0xFFFFu; w[3] = v.y >> 16;
+            } else {
+              const uint4 v = *reinterpret_cast<const uint4*>(s_word + (j - s0));
+              w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) e[g][u] = w[u] ? none : e[g][u];
+          }
+          consider(max_nan(max_nan(e[g][0], e[g][1]), max_nan(e[g][2], e[g][3])), j);
         }
-        if (any) {                               // listed tokens come below
-          const uint4 w = *reinterpret_cast<const uint4*>(s_word + (j - s0));
-          e[g][0] = w.x ? none : e[g][0];
-          e[g][1] = w.y ? none : e[g][1];
-          e[g][2] = w.z ? none : e[g][2];
-          e[g][3] = w.w ? none : e[g][3];
-        }
-        consider(max_nan(max_nan(e[g][0], e[g][1]), max_nan(e[g][2], e[g][3])), j);
       }
+      request(j0 + 4 * GROUPS * THREADS);
     }
     if (any) {
       __syncthreads();                           // the slice is stored
-      for (int i = threadIdx.x; i < s_listed; i += threads) {
+      const int listed = s_listed;
+      for (int i = threadIdx.x; i < listed; i += THREADS) {
         const int t = sl.list[i], j = s0 + t;
-        if (mask && !(__ldg(mask + (j >> 5)) >> (j & 31) & 1)) continue;
-        const float v = rule(*(volatile const float*)(y + j), s_word[t], r);
-        y[j] = v;
-        consider(v, j & ~3);
+        const float was = *(volatile const float*)(y + j);
+        const uint32_t word = mask ? __ldg(mask + (j >> 5)) : ~0u;
+        if (word >> (j & 31) & 1) {
+          float v = penalties<Word>(was, sl.get(t), r);
+          if (i < biased) v = __fadd_rn(v, __ldg(bias + last[i]));
+          y[j] = v;
+          consider(v, j & ~3);
+        }
       }
       __syncthreads();
     }
@@ -458,35 +488,35 @@ __global__ void __launch_bounds__(kRuleThreadsMax) k_adjust(const __grid_constan
   Pick m{best, best_at, is_nan(best)};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = pick_comb(m, pick_shfl(m, o));
-  if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = m;
+  if (lane == 0) s_warp[threadIdx.x >> 5] = m;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    Pick t = s_warp[0];
-    for (int w = 1; w < threads / 32; ++w) t = pick_comb(t, s_warp[w]);
-    s_cand[0] = __float_as_int(t.v);
-    s_cand[1] = t.i;
-    s_cand[2] = t.nan;
+  if (threadIdx.x < 32) {
+    Pick t = threadIdx.x < THREADS / 32 ? s_warp[threadIdx.x] : Pick{0.0f, -1, 0};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t = pick_comb(t, pick_shfl(t, o));
+    if (threadIdx.x == 0) {
+      s_cand[0] = __float_as_int(t.v);
+      s_cand[1] = t.i;
+      s_cand[2] = t.nan;
+    }
   }
   cluster_sync();                                // (orders the stores of out before the read below as well)
-  if (rank == 0 && threadIdx.x == 0) {
-    Pick t{__int_as_float(s_cand[0]), s_cand[1], s_cand[2]};
-    for (int q = 1; q < cluster; ++q) {
-      const Pick u{__int_as_float(dsmem_ld_s32(smem_u32(&s_cand[0]), q)), dsmem_ld_s32(smem_u32(&s_cand[1]), q),
-                   dsmem_ld_s32(smem_u32(&s_cand[2]), q)};
-      t = pick_comb(t, u);
-    }
+  if (rank == 0 && threadIdx.x < 32) {
+    Pick t{0.0f, -1, 0};
+    if (lane < cluster)
+      t = Pick{__int_as_float(dsmem_ld_s32(smem_u32(&s_cand[0]), lane)), dsmem_ld_s32(smem_u32(&s_cand[1]), lane),
+               dsmem_ld_s32(smem_u32(&s_cand[2]), lane)};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t = pick_comb(t, pick_shfl(t, o));
     int token = a.none;
-    if (t.i >= 0) {
-      token = t.i;
-      for (int u = 3; u >= 0; --u)               // the group's first NaN, or first entry of its value
-        if (t.i + u < a.vocab) {
-          const float v = *(volatile const float*)(y + t.i + u);
-          if (t.nan ? is_nan(v) : v == t.v) token = t.i + u;
-        }
+    if (t.i >= 0) {                              // the group's first NaN, or first entry of its value
+      const float v = lane < 4 && t.i + lane < a.vocab ? *(volatile const float*)(y + t.i + lane) : none;
+      const bool is = lane < 4 && t.i + lane < a.vocab && (t.nan ? is_nan(v) : v == t.v);
+      token = t.i + __ffs(__ballot_sync(0xFFFFFFFFu, is)) - 1;
     } else if (!mask) {
       token = 0;                                 // a row of -infinity alone: the first token
     } else {
-      for (int i = 0; i < (a.vocab + 31) / 32 && token == a.none; ++i) {
+      for (int i = 0; i < (a.vocab + 31) / 32; ++i) {
         const uint32_t word = __ldg(mask + i) & (a.vocab - 32 * i >= 32 ? ~0u : (1u << (a.vocab - 32 * i)) - 1);
         if (word) {
           token = 32 * i + __ffs(word) - 1;      // allowed tokens that are all -infinity: the first of them
@@ -494,7 +524,7 @@ __global__ void __launch_bounds__(kRuleThreadsMax) k_adjust(const __grid_constan
         }
       }
     }
-    a.token[row] = token;
+    if (lane == 0) a.token[row] = token;
   }
   cluster_sync();                                // no CTA leaves while its candidate is read
 }
@@ -525,29 +555,42 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t st) {
   return launch_dependent(k_move, dim3(rows, blocks), dim3(kMoveThreads), st, a, mv);
 }
 
-cudaError_t launch_adjust(const tc_logits_rules& r, cudaStream_t st) {
-  const bool vec = ((uintptr_t)r.logits | (uintptr_t)r.out) % 16 == 0 && r.logits_stride % 4 == 0 && r.out_stride % 4 == 0;
-  // few rows: 16 CTAs of 1024 threads a row, whose share is one slice up to 262144 tokens; many rows: 8 CTAs of
-  // 512 threads, several to an SM, so that one fills its words while another streams
-  const bool few = r.rows * 8 <= 148;
-  const int cluster = few ? 16 : 8, threads = few ? 1024 : 512;
+namespace {
+template <bool VEC, class Word, int GROUPS, int THREADS, int CTAS>
+cudaError_t adjust(const tc_logits_rules& r, int cluster, int slice_bytes, cudaStream_t st) {
+  constexpr auto kern = k_adjust<VEC, Word, GROUPS, THREADS, CTAS>;
   const int share = ((r.vocab + cluster - 1) / cluster + 31) / 32 * 32;
-  const int smem = std::min(share, 4 * kGroups * threads) * 6;   // a word and a list entry a token
-  auto kern = vec ? k_adjust<true> : k_adjust<false>;
-  static std::atomic<uint64_t> wide{0};          // devices on which clusters of 16 and the words are allowed
+  const int slice = std::min(share, slice_bytes / (int)sizeof(Word));
+  // a word a token, a place a bias entry, and list entries for as many tokens as the history and the biases can name
+  const int n_bias = r.bias ? r.n_bias : 0;
+  const int64_t names = (r.history ? r.max_history : 0) + (int64_t)n_bias;
+  const int smem = slice * (int)sizeof(Word) + 4 * n_bias + 2 * (int)std::min<int64_t>(slice, names);
+  static std::atomic<uint64_t> ready{0};         // devices on which clusters of 16 and the shared memory are allowed
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !(wide.load() >> dev & 1)) {
-    for (auto k : {k_adjust<true>, k_adjust<false>}) {
-      e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kGroups * kRuleThreadsMax * 6);
-      if (e != cudaSuccess) return e;
-    }
-    if (dev < 64) wide.fetch_or(1ull << dev);
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * slice_bytes + 8192);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  return launch_ex(kern, dim3((unsigned)r.rows * cluster), dim3(threads), smem, st, cluster, r, cluster, share);
+  tc_logits_rules a = r;
+  a.n_bias = n_bias;
+  return launch_ex(kern, dim3((unsigned)r.rows * cluster), dim3(THREADS), smem, st, cluster, a, cluster, share, slice);
+}
+template <bool VEC, class Word>
+cudaError_t adjust_of(const tc_logits_rules& r, cudaStream_t st) {
+  // few rows: 16 CTAs of 1024 threads a row; many: 8 CTAs of 256, four to an SM
+  return r.rows * 8 <= 148 ? adjust<VEC, Word, 4, 1024, 1>(r, 16, 65536, st) : adjust<VEC, Word, 4, 256, 4>(r, 8, 32768, st);
+}
+}  // namespace
+
+cudaError_t launch_adjust(const tc_logits_rules& r, cudaStream_t st) {
+  const bool vec = ((uintptr_t)r.logits | (uintptr_t)r.out) % 16 == 0 && r.logits_stride % 4 == 0 && r.out_stride % 4 == 0;
+  if (r.history && r.max_history > (int)Bits<uint16_t>::kCount)
+    return vec ? adjust_of<true, uint32_t>(r, st) : adjust_of<false, uint32_t>(r, st);
+  return vec ? adjust_of<true, uint16_t>(r, st) : adjust_of<false, uint16_t>(r, st);
 }
 
 }  // namespace tc
