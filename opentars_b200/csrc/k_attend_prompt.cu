@@ -38,6 +38,7 @@ struct PromptShape {
   static constexpr int kTiles = HD == 256 ? 1 : 2;           // query tiles of a CTA
   static constexpr int kBlock = HD == 256 ? 64 : 128;        // key slots of a block
   static constexpr int kQ = kRows * HD * 2, kMat = kBlock * HD * 2;
+  static constexpr int kParts = kTiles;                      // a block's probabilities are handed over in parts
   static constexpr int kSlots = HD == 64 ? 8 : 5;            // ring of key / value blocks
   static constexpr int kThreads = kTiles == 2 ? 384 : 192;   // (whole warpgroups where registers are split)
   static constexpr int kSmem = 1024 + kTiles * kQ + kSlots * kMat;
@@ -64,6 +65,72 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return m;
 }
 
+// Two fp32 values in a register pair, one instruction for both.
+__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t pair(float a) { return pair(__float_as_uint(a), __float_as_uint(a)); }
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+// 2^x of two values <= 9 on the FMA units: x = n + f with n the nearest integer (added to 1.5 x 2^23, n stands in
+// the sum's low bits) and f in [-1/2, 1/2]; 2^f by a polynomial fitted to least relative error (2.6e-6), n added
+// to its exponent. Below 2^-126 the result is 2^-126; a NaN stays one.
+__device__ __forceinline__ uint64_t ex2_fma(uint64_t x2) {
+  const float2 x = halves(x2);
+  x2 = pair(__float_as_uint(max_nan(x.x, -126.0f)), __float_as_uint(max_nan(x.y, -126.0f)));
+  const uint64_t t = add2(x2, pair(12582912.0f)), f = add2(x2, fma2(t, pair(-1.0f), pair(12582912.0f)));
+  uint64_t p = fma2(f, pair(0.009570101276040077f), pair(0.05591785907745361f));
+  p = fma2(p, f, pair(0.240247443318367f));
+  p = fma2(p, f, pair(0.6931217908859253f));
+  p = fma2(p, f, pair(0.9999992847442627f));
+  const float2 n = halves(t), y = halves(p);
+  return pair(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23), __float_as_uint(y.y) + (__float_as_uint(n.y) << 23));
+}
+// v[i] = 2^(v[i] scale - base) for N scores, rounded to T two by two into out; their sum (of the unrounded values).
+// MIX: every fourth pair goes to the FMA units, which are idle while the others wait for the special function
+// unit (8 cycles a warp and instruction); not where masked scores of -infinity have to become 0.
+template <class T, int N, bool MIX>
+__device__ __forceinline__ float exponentials(const uint32_t* v, uint32_t* out, float scale2, float base) {
+  const uint64_t s2 = pair(scale2), b2 = pair(-base);
+  uint64_t sum[2] = {0, 0};
+#pragma unroll
+  for (int x = 0; x < N; x += 2) {
+    const uint64_t y = fma2(pair(v[x], v[x + 1]), s2, b2);
+    uint64_t p;
+    if (MIX && (x >> 1 & 3) == 3) {
+      p = ex2_fma(y);
+    } else {
+      const float2 f = halves(y);
+      p = pair(__float_as_uint(ex2(f.x)), __float_as_uint(ex2(f.y)));
+    }
+    sum[x >> 1 & 1] = add2(sum[x >> 1 & 1], p);
+    const float2 f = halves(p);
+    out[x >> 1] = Elem<T>::pack(f.x, f.y);
+  }
+  const float2 f = halves(add2(sum[0], sum[1]));
+  return f.x + f.y;
+}
+
 template <class T, int HD>
 __device__ __noinline__ void redo_row(const AttendArgs& a, int b, int kvh, int64_t row, int h, int end) {
   float q[HD / 32], o[HD / 32];
@@ -79,7 +146,7 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   using Sh = PromptShape<HD>;
   constexpr int NT = Sh::kTiles, BN = Sh::kBlock;
   extern __shared__ uint8_t s_raw[];
-  __shared__ __align__(8) uint64_t s_full[Sh::kSlots], s_free[Sh::kSlots], s_sfull[2], s_pfull[2], s_odone[2], s_fix, s_end;
+  __shared__ __align__(8) uint64_t s_full[Sh::kSlots], s_free[Sh::kSlots], s_sfull[2], s_pfull[4], s_odone[2], s_fix, s_end;
   __shared__ uint32_t s_tmem;
   __shared__ int s_scan[16], s_found[2], s_bad, s_dead;
   const KvCache& c = a.c;
@@ -150,7 +217,8 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_sfull[i], 1);
-      mbar_init(&s_pfull[i], 4);
+      mbar_init(&s_pfull[2 * i], 4);
+      mbar_init(&s_pfull[2 * i + 1], 4);
       mbar_init(&s_odone[i], 1);
     }
     mbar_init(&s_fix, 1);
@@ -232,85 +300,91 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
     } else if (warp == kMma) {
       asm volatile("bar.sync 1, %0;" ::"n"(128 * NT + 32) : "memory");       // Q is in shared memory
       tc_fence_after();
-      if (lane == 0) {
-        constexpr bool bf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
-        constexpr uint32_t id_s = idesc_f16(kRows, BN, bf16, false), id_o = idesc_f16(kRows, HD, bf16, true);
-        int slot = 0, phase = 0;
-        bool ok = true;
-        auto wait = [&](uint64_t* bar, int parity) { return ok = ok && mbar_wait(bar, parity, c.err, kErrPromptWait, a.spin); };
-        auto next = [&] {
-          if (++slot == Sh::kSlots) { slot = 0; phase ^= 1; }
-        };
-        // S = Q K^T of tile t with the keys in `at`, into buffer `buf`
-        auto scores = [&](int t, int at, int buf) {
-          const uint32_t q = smem_u32(s_q) + t * Sh::kQ, k = smem_u32(s_kv) + at * Sh::kMat;
+      constexpr bool bf16 = __is_same(T, __nv_bfloat16);
+      constexpr uint32_t id_s = idesc_f16(kRows, BN, bf16, false), id_o = idesc_f16(kRows, HD, bf16, true);
+      constexpr uint32_t kGroup = kRows * 128 / 16, kKeys = BN * 128 / 16;   // a 64-column group's bytes in descriptor units
+      // (the whole warp runs this part: the elected lane issues, and commits what it issued)
+      const uint32_t leader = elect_one();
+      const uint64_t q_desc = sdesc_k128(smem_u32(s_q)), k_desc = sdesc_k128(smem_u32(s_kv)),
+                     v_desc = sdesc_mn128(smem_u32(s_kv), BN * 128);
+      int slot = 0, phase = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int parity) {
+        return ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, c.err, kErrPromptWait, a.spin));
+      };
+      auto next = [&] {
+        if (++slot == Sh::kSlots) { slot = 0; phase ^= 1; }
+      };
+      // S = Q K^T of tile t with the keys in `at`, into buffer `buf`
+      auto scores = [&](int t, int at, int buf) {
+        const uint64_t q = q_desc + t * (Sh::kQ / 16), k = k_desc + at * (Sh::kMat / 16);
 #pragma unroll
-          for (int x = 0; x < HD / 16; ++x)
-            mma_f16(tmem + Sh::kS + buf * BN, sdesc_k128(q + (x >> 2) * kRows * 128) + 2 * (x & 3),
-                    sdesc_k128(k + (x >> 2) * BN * 128) + 2 * (x & 3), id_s, x > 0);
-          mma_commit(&s_sfull[buf]);
-        };
-        auto values = [&](int t, int at, int buf, bool more) {
-          const uint32_t v = smem_u32(s_kv) + at * Sh::kMat;
+        for (int x = 0; x < HD / 16; ++x)
+          mma_f16(tmem + Sh::kS + buf * BN, q + (x >> 2) * kGroup + 2 * (x & 3), k + (x >> 2) * kKeys + 2 * (x & 3), id_s,
+                  x > 0, leader);
+        mma_commit_if(&s_sfull[buf], leader);
+      };
+      // part h of O += P V: the probabilities come in kParts, so that the first can be multiplied while the
+      // rest is still being exponentiated
+      auto values = [&](int t, int at, int buf, bool more, int h) {
+        const uint64_t v = v_desc + at * (Sh::kMat / 16);
 #pragma unroll
-          for (int x = 0; x < BN / 16; ++x)
-            mma_f16_ta(tmem + Sh::kO + t * HD, tmem + Sh::kS + buf * BN + 8 * x, sdesc_mn128(v + x * 2048, BN * 128), id_o,
-                       more || x > 0);
-          mma_commit(&s_odone[t]);
-        };
-        if (w.nmax && wait(&s_full[0], 0)) {
-          tc_fence_after();
+        for (int x = h * (BN / 16 / Sh::kParts); x < (h + 1) * (BN / 16 / Sh::kParts); ++x)
+          mma_f16_ta(tmem + Sh::kO + t * HD, tmem + Sh::kS + buf * BN + 8 * x, v + x * 128, id_o, more || x > 0, leader);
+        if (h == Sh::kParts - 1) mma_commit_if(&s_odone[t], leader);
+      };
+      if (w.nmax && wait(&s_full[0], 0)) {
+        tc_fence_after();
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-            if (w.nb[t]) scores(t, 0, t);
-          mma_commit(&s_free[0]);
+        for (int t = 0; t < NT; ++t)
+          if (w.nb[t]) scores(t, 0, t);
+        mma_commit_if(&s_free[0], leader);
+        next();
+      }
+      for (int j = 0; ok && j < w.nmax; ++j) {
+        if constexpr (NT == 2) {
+          const int vs = slot, vph = phase;
           next();
-        }
-        for (int j = 0; ok && j < w.nmax; ++j) {
-          if constexpr (NT == 2) {
-            const int vs = slot, vph = phase;
-            next();
-            const int ks = slot, kph = phase;
-            const bool more = j + 1 < w.nmax;
-            if (more) next();
-            bool have_v = false, have_k = false;
+          const int ks = slot, kph = phase;
+          const bool more = j + 1 < w.nmax;
+          if (more) next();
+          bool have_v = false, have_k = false;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (j >= w.nb[t]) continue;
-              if (!have_v && !wait(&s_full[vs], vph)) break;
-              have_v = true;
-              if (!wait(&s_pfull[t], j & 1)) break;
-              tc_fence_after();
-              values(t, vs, t, j > 0);
-              if (t == 1 || j >= w.nb[1]) mma_commit(&s_free[vs]);       // the last tile that reads it
-              if (j + 1 < w.nb[t]) {
-                if (!have_k && !wait(&s_full[ks], kph)) break;
-                have_k = true;
-                scores(t, ks, t);
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || j >= w.nb[t]) continue;
+            if (!have_v && !wait(&s_full[vs], vph)) continue;
+            have_v = true;
+#pragma unroll
+            for (int h = 0; h < Sh::kParts; ++h)
+              if (wait(&s_pfull[2 * t + h], j & 1)) {
+                tc_fence_after();
+                values(t, vs, t, j > 0, h);
               }
+            if (t == 1 || j >= w.nb[1]) mma_commit_if(&s_free[vs], leader);       // the last tile that reads it
+            if (ok && j + 1 < w.nb[t] && (have_k || wait(&s_full[ks], kph))) {
+              have_k = true;
+              scores(t, ks, t);
             }
-            if (!ok) break;
-            if (more) mma_commit(&s_free[ks]);
-          } else {
-            if (j + 1 < w.nmax) {
-              if (!wait(&s_full[slot], phase)) break;
-              tc_fence_after();
-              scores(0, slot, (j + 1) & 1);
-              mma_commit(&s_free[slot]);
-              next();
-            }
-            if (!wait(&s_full[slot], phase) || !wait(&s_pfull[j & 1], j >> 1 & 1)) break;
+          }
+          if (more) mma_commit_if(&s_free[ks], leader);
+        } else {
+          if (j + 1 < w.nmax) {
+            if (!wait(&s_full[slot], phase)) break;
             tc_fence_after();
-            values(0, slot, j & 1, j > 0);
-            mma_commit(&s_free[slot]);
+            scores(0, slot, (j + 1) & 1);
+            mma_commit_if(&s_free[slot], leader);
             next();
           }
+          if (!wait(&s_full[slot], phase) || !wait(&s_pfull[2 * (j & 1)], j >> 1 & 1)) break;
+          tc_fence_after();
+          values(0, slot, j & 1, j > 0, 0);
+          mma_commit_if(&s_free[slot], leader);
+          next();
         }
-        if (!ok) s_dead = 1;
-        mma_commit(&s_end);                          // nothing this thread issued is still running when the block ends
-        mbar_wait(&s_end, 0, c.err, kErrPromptWait);
       }
-      __syncwarp();
+      if (!ok) s_dead = 1;
+      mma_commit_if(&s_end, leader);               // nothing this warp issued is still running when the block ends
+      mbar_wait(&s_end, 0, c.err, kErrPromptWait);
     }
     __syncthreads();
     __syncthreads();                               // the outputs are out of TMEM
@@ -373,7 +447,8 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
 #pragma unroll
     for (int x = 0; x < BN; ++x) asm volatile("" : "+r"(v[x]));        // no use moves before the wait
     const int j0 = w.block(j) * BN;
-    if (j0 + BN - 1 > pmin || (pmax - j0 >= a.window && j0 + BN > a.sinks)) {
+    const bool masked = j0 + BN - 1 > pmin || (pmax - j0 >= a.window && j0 + BN > a.sinks);
+    if (masked) {
       const int hi = p + 1 - j0, lo = from - j0, sk = a.sinks - j0;
 #pragma unroll
       for (int x = 0; x < BN; ++x)
@@ -408,20 +483,17 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
       }
     }
     const float base = m == neg_inf() ? 0.0f : m;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kN = BN / Sh::kParts;
 #pragma unroll
-    for (int x = 0; x < BN; x += 2) {
-      const float p0 = ex2(fmaf(__uint_as_float(v[x]), scale2, -base)), p1 = ex2(fmaf(__uint_as_float(v[x + 1]), scale2, -base));
-      sum[x >> 1 & 3] += p0 + p1;
-      v[x >> 1] = Elem<T>::pack(p0, p1);
+    for (int h = 0; h < Sh::kParts; ++h) {
+      l += masked ? exponentials<T, kN, false>(v + h * kN, v + h * kN / 2, scale2, base)
+                  : exponentials<T, kN, true>(v + h * kN, v + h * kN / 2, scale2, base);
+      tmem_st32(st + h * kN / 2, v + h * kN / 2);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_pfull[2 * buf + h]);
     }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-    for (int x = 0; x < BN / 2; x += 32) tmem_st32(st + x, v + x);
-    tmem_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&s_pfull[buf]);
   }
   if (ok && n) ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_odone[t], (n - 1) & 1, c.err, kErrPromptWait, a.spin));
   if (!ok) s_dead = 1;
