@@ -5,9 +5,13 @@
 // consecutive tokens, so a group's heads share every key and value tile that is staged. A CTA takes
 // two tiles (one for head dim 256, whose output alone fills half of TMEM) of one sequence and walks
 // the blocks of key slots that any of its rows sees: the sinks' blocks, then those of the windows.
-//   producer   one warp: a block's keys and values page by page by TMA (64 columns x page rows
-//              boxes, 128-byte swizzle) into a ring; value rows behind the sequence's end, which
-//              may hold anything, are cleared there (0 x NaN is not 0)
+//   loaders    a block's keys and values into a ring, rows behind the sequence's end, which may hold
+//              anything, as zeros (0 x NaN is not 0). Pages of 64 slots and more: one warp, by TMA (64
+//              columns x page rows boxes, 128-byte swizzle). Smaller pages: three warps, by cp.async
+//              (16-byte pieces, eight slots of one page at a time, placed as the swizzle wants them),
+//              because boxes of 2 or 4 KB are TMA's limit: 16000 tokens of a window of 512 at head dim
+//              256 take 131 us by TMA against 101 over 16-slot pages, and 92 against 99 over 64-slot
+//              ones; three prompts of up to 8192 tokens at head dim 128 364 against 413 over the latter
 //   MMA        one thread: S = Q K^T into TMEM (tcgen05 kind::f16), then O += P V with P as the
 //              TMEM operand where S was; with two tiles one is multiplied while the other is
 //              exponentiated, with one tile S is double-buffered
@@ -40,7 +44,7 @@ struct PromptShape {
   static constexpr int kQ = kRows * HD * 2, kMat = kBlock * HD * 2;
   static constexpr int kParts = kTiles;                      // a block's probabilities are handed over in parts
   static constexpr int kSlots = HD == 64 ? 8 : 5;            // ring of key / value blocks
-  static constexpr int kThreads = kTiles == 2 ? 384 : 192;   // (whole warpgroups where registers are split)
+  static constexpr int kThreads = 128 * kTiles + 128;        // softmax, MMA, loaders
   static constexpr int kSmem = 1024 + kTiles * kQ + kSlots * kMat;
   static constexpr uint32_t kS = 0, kO = 256;                // TMEM columns: two S (and P) buffers, the outputs
 };
@@ -48,6 +52,7 @@ struct PromptShape {
 struct PromptMaps {
   CUtensorMap k, v;
 };
+constexpr int kLoaders = 3, kTmaPage = 64;       // loader warps without TMA; the smallest page it takes
 
 // What a CTA works on, the same in every thread.
 struct Work {
@@ -140,7 +145,7 @@ __device__ __noinline__ void redo_row(const AttendArgs& a, int b, int kvh, int64
   row_store<T, HD>(a.out, row * a.orow + (int64_t)h * a.oh, lane, o);
 }
 
-template <class T, int HD>
+template <class T, int HD, bool TMA>
 __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
     k_prompt(const __grid_constant__ PromptMaps maps, const __grid_constant__ AttendArgs a, int gblocks, int hb, int tokens) {
   using Sh = PromptShape<HD>;
@@ -153,7 +158,7 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   uint8_t* s_q = s_raw + (1024 - (smem_u32(s_raw) & 1023)) % 1024;
   uint8_t* s_kv = s_q + NT * Sh::kQ;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kProducer = 4 * NT, kMma = kProducer + 1;
+  constexpr int kMma = 4 * NT;                    // warps 0 .. 4 NT - 1 softmax, then the MMA's, then the loaders
 
   // ---- which rows: pairs of tiles, sequence by sequence; the last pairs (the longest rows) go first
   Work w;
@@ -212,7 +217,7 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < Sh::kSlots; ++i) {
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[i], TMA ? 1 : kLoaders);
       mbar_init(&s_free[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -233,9 +238,10 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   const uint32_t tmem = s_tmem;
 
   // With two tiles the launch's 168 registers a thread (3 warpgroups) are split 208 + 208 + 88, their sum unchanged
-  if (warp >= kProducer) {
+  if (warp >= kMma) {
     if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == kProducer) {
+    if (TMA && warp == kMma + 1) {
+      // one loader: a block page by page in boxes of 64 columns, a lane a box
       int slot = 0, phase = 0, issued = 0, fixes = 0;
       const int end = max(w.end[0], w.end[1]), box = min(BN, 1 << c.shift), per = box / 16;
       auto load = [&](int j, bool is_v) {
@@ -297,6 +303,67 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
         if (--slot < 0) { slot = Sh::kSlots - 1; phase ^= 1; }
         mbar_wait(&s_full[slot], phase, c.err, kErrPromptWait);
       }
+    } else if (!TMA && warp > kMma) {
+      // A loader takes every kLoaders-th unit of 8 slots of a block; a lane copies piece lane % kLanes of rows r0,
+      // r0 + kAtOnce, ..: row r of a 64-column group is 128 bytes, its piece p at place p ^ (r % 8)
+      constexpr int kPieces = HD / 8, kLanes = kPieces < 32 ? kPieces : 32, kAtOnce = 32 / kLanes, kLag = 2;
+      const int piece = lane % kLanes, r0 = lane / kLanes, me = warp - kMma - 1;
+      const uint32_t put = smem_u32(s_kv) + (piece >> 3) * BN * 128 + r0 * 128 + (((piece & 7) ^ r0) << 4);
+      const int64_t step = 2 * kAtOnce * c.ss;
+      const int end = max(w.end[0], w.end[1]);
+      int slot = 0, phase = 0, issued = 0, full = 0;
+      auto arrive = [&] {                          // the oldest block still on its way is here
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_full[full]);
+        if (++full == Sh::kSlots) full = 0;
+      };
+      auto load = [&](int j, const uint8_t* pool) {
+        if (issued >= Sh::kSlots &&
+            !__all_sync(0xFFFFFFFFu, mbar_wait(&s_free[slot], phase ^ 1, c.err, kErrPromptWait, a.spin)))
+          return false;
+        const int j0 = w.block(j) * BN;
+        int page = -1;                             // lane u: of unit u
+        if (lane < BN / 8 && j0 + 8 * lane < end) {
+          const int js = j0 + 8 * lane;
+          page = __ldg(c.table + (int64_t)w.b * c.ts + (js >> c.shift));
+          if ((unsigned)page >= (unsigned)c.n_pages) {
+            page = -1;
+            if (js + 8 > w.first || js < w.head) { // (a page that no row sees may be gone)
+              kv_fail(c, kErrPrompt);
+              s_bad = 1;
+            }
+          }
+        }
+        for (int u = me; u < BN / 8; u += kLoaders) {
+          const int pg = __shfl_sync(0xFFFFFFFFu, page, u), js = j0 + 8 * u + r0;
+          const uint8_t* from = pool + 2 * (kv_offset(c, max(pg, 0), js, w.kvh) + 8 * piece);
+          const uint32_t to = put + slot * Sh::kMat + u * 1024;
+          const int rows = pg >= 0 ? w.len - js : 0;         // of them exist, counted from this lane's first
+#pragma unroll
+          for (int x = 0; x < 8 / kAtOnce; ++x)
+            asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"((to ^ (x * kAtOnce << 4)) + x * kAtOnce * 128),
+                         "l"(from + x * step), "r"(x * kAtOnce < rows ? 16 : 0)
+                         : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (++issued > kLag) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+          arrive();
+        }
+        if (++slot == Sh::kSlots) { slot = 0; phase ^= 1; }
+        return true;
+      };
+      bool ok = w.nmax == 0 || load(0, c.k);
+      for (int j = 0; ok && j < w.nmax; ++j) {
+        // in the order of use: with two tiles V(j), K(j + 1); with one K(j + 1), V(j)
+        if (NT == 2) ok = load(j, c.v) && (j + 1 == w.nmax || load(j + 1, c.k));
+        else ok = (j + 1 == w.nmax || load(j + 1, c.k)) && load(j, c.v);
+      }
+      if (!ok) s_dead = 1;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (ok)
+        for (int x = min(issued, kLag); x > 0; --x) arrive();
     } else if (warp == kMma) {
       asm volatile("bar.sync 1, %0;" ::"n"(128 * NT + 32) : "memory");       // Q is in shared memory
       tc_fence_after();
@@ -551,14 +618,14 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   __syncthreads();
 }
 
-template <class T, int HD>
+template <class T, int HD, bool TMA>
 cudaError_t prompt_hd(const AttendArgs& a, cudaStream_t st) {
   using Sh = PromptShape<HD>;
   const KvCache& c = a.c;
-  PromptMaps maps;
+  PromptMaps maps{};
   const int box = std::min(Sh::kBlock, 1 << c.shift);
-  if (!make_map_pool(&maps.k, c, c.k, box) || !make_map_pool(&maps.v, c, c.v, box)) return cudaErrorInvalidValue;
-  const cudaError_t e = allow_smem<k_prompt<T, HD>>(Sh::kSmem);
+  if (TMA && (!make_map_pool(&maps.k, c, c.k, box) || !make_map_pool(&maps.v, c, c.v, box))) return cudaErrorInvalidValue;
+  const cudaError_t e = allow_smem<k_prompt<T, HD, TMA>>(Sh::kSmem);
   if (e != cudaSuccess) return e;
   // a group's heads in blocks of nearly equal size; as many tokens as fill a tile with them
   const int G = a.nh / c.n_kv, gblocks = (G + kMaxHeads - 1) / kMaxHeads, hb = (G + gblocks - 1) / gblocks;
@@ -567,16 +634,17 @@ cudaError_t prompt_hd(const AttendArgs& a, cudaStream_t st) {
   const int64_t pairs = std::min<int64_t>(a.tokens, a.tokens / span + std::min(a.tokens, c.batch));
   const int64_t grid = pairs * c.n_kv * gblocks;
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
-  k_prompt<T, HD><<<(unsigned)grid, Sh::kThreads, Sh::kSmem, st>>>(maps, a, gblocks, hb, tokens);
+  k_prompt<T, HD, TMA><<<(unsigned)grid, Sh::kThreads, Sh::kSmem, st>>>(maps, a, gblocks, hb, tokens);
   return cudaGetLastError();
 }
 
 template <class T>
 cudaError_t prompt_of(const AttendArgs& a, cudaStream_t st) {
+  const bool tma = 1 << a.c.shift >= kTmaPage;
   switch (a.c.hd) {
-    case 64: return prompt_hd<T, 64>(a, st);
-    case 128: return prompt_hd<T, 128>(a, st);
-    default: return prompt_hd<T, 256>(a, st);
+    case 64: return tma ? prompt_hd<T, 64, true>(a, st) : prompt_hd<T, 64, false>(a, st);
+    case 128: return tma ? prompt_hd<T, 128, true>(a, st) : prompt_hd<T, 128, false>(a, st);
+    default: return tma ? prompt_hd<T, 256, true>(a, st) : prompt_hd<T, 256, false>(a, st);
   }
 }
 
