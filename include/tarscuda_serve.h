@@ -80,10 +80,14 @@ uint64_t tc_attend_workspace(const tc_kv_cache* c, int32_t n_heads, int32_t weig
 /* Attention of the tokens of a prompt, or of a chunk of one, whose key and value rows are in the
  * cache already: rows cu[b] .. cu[b+1] - 1 of q are the last tokens of sequence b, row i of n at
  * position p = length[b] - n + i. It sees slot j if j <= p and (p - j < window or j < sinks; window
- * 0: all). Rows at a negative position get zeros; rows at and behind cu[batch] are left alone. */
+ * 0: all). Rows at a negative position get zeros; rows at and behind cu[batch] are left alone.
+ * ws: tc_attend_prompt_workspace bytes, 256-byte aligned (0 bytes, and NULL, for calls of many
+ * rows). */
 int tc_attend_prompt(const tc_kv_cache* c, const void* q, int64_t q_row_stride, int64_t q_head_stride, void* out,
                      int64_t out_row_stride, int64_t out_head_stride, int32_t n_heads, const int32_t* cu,
-                     int32_t tokens, float scale, int32_t window, int32_t sinks, void* stream);
+                     int32_t tokens, float scale, int32_t window, int32_t sinks, void* ws, uint64_t ws_bytes,
+                     void* stream);
+uint64_t tc_attend_prompt_workspace(const tc_kv_cache* c, int32_t n_heads, int32_t tokens, int32_t window, int32_t sinks);
 
 /* Cuts every sequence longer than `budget` slots to budget, separately for each key-value head. The
  * slots whose position is below `sinks` or at least seen[b] - recent stay first (sinks + recent <=

@@ -1,18 +1,21 @@
-// Attention of one query row per sequence over the paged cache (tc_attend).
+// Attention of few query rows per sequence over the paged cache: one token each (tc_attend), or short
+// chunks of a prompt (tc_attend_prompt takes longer ones to the tensor cores, k_attend_prompt.cu).
 //
-// The G = n_heads / n_kv heads of a key-value head read the same rows, so they are the columns of one
-// warp MMA (m16n8k16: 16 slots x 8 heads; blocks of 8 or 16 heads): each key and value row crosses HBM
-// once and the kernel is bound by that stream. The work of a call is one list of chunks of 16 slots -
-// sequence by sequence, key-value head by key-value head, only chunks with a visible slot - cut into
-// equal runs, one per CTA and one CTA per SM: ragged batches and a single long sequence fill the GPU
-// alike. Every CTA derives its run from the lengths (a scan of the batch); nothing is planned on the
-// host. The warps of a CTA take the chunks of its run in turn, each with a ring of its own that it fills
-// by cp.async (16-byte pieces, hidden rows as zeros: 0 x NaN is not 0) and a running maximum, sum and
-// output of its own, so no warp waits for another within an item:
+// The G = n_heads / n_kv heads of a key-value head read the same rows, so the heads of a token, or of a
+// block of consecutive tokens, are the columns of one warp MMA (m16n8k16: 16 slots x 8 rows of q; blocks
+// of at most 8 or 16 rows): each key and value row crosses HBM once and the kernel is bound by that
+// stream. The work of a call is one list of chunks of 16 slots - sequence by sequence, block by block,
+// key-value head by key-value head, only chunks with a visible slot - cut into equal runs, one per CTA
+// and one CTA per SM: ragged batches and a single long sequence fill the GPU alike. Every CTA derives
+// its run from the lengths (a scan of the batch); nothing is planned on the host. The warps of a CTA
+// take the chunks of its run in turn, each with a ring of its own that it fills by cp.async (16-byte
+// pieces, hidden rows as zeros: 0 x NaN is not 0) and a running maximum, sum and output of its own, so
+// no warp waits for another within an item:
 //   S^T = K Q^T (ldmatrix), p = 2^(s - m), O^T += V^T P^T (ldmatrix.trans) with P split in two 16-bit
 //   parts: the probabilities keep 16 bits and more at the price of MMAs that the memory bound hides
 // (Boxes of TMA over 16-slot pages were tried in place of cp.async: 3.46 against 4.84 TB/s with
-// 64-slot pages, the boxes of 2 KB being the limit.)
+// 64-slot pages, the boxes of 2 KB being the limit.) 64 ragged conversations of up to 8192 slots, 16
+// heads on 8 of 128, bf16: 204 us over 16-slot pages, 190 us over 64-slot ones (5.4 and 5.75 TB/s).
 // At an item's end the warps' states are joined through shared memory. An item that lies in one
 // CTA's run is stored at once; of the others every CTA writes its state (maximum, sum, 16 x HD fp32)
 // to the workspace, and k_join, launched early as a dependent, combines them in run order: no atomics,
@@ -20,6 +23,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "attend_row.cuh"
 #include "mma.h"
@@ -42,76 +46,156 @@ struct AttendShape {
   static constexpr int kPart = kRowsMma * HD + 2 * kRowsMma; // floats of a CTA's state of an item
 };
 
-// Where one sequence's visible slots lie: [0, head) and [first, len), in nt tiles: tiles 0 .. na - 1,
-// then from t0 on.
-struct SeqTiles {
-  int len, first, head, na, t0, nt;
-  __device__ __forceinline__ SeqTiles(const AttendArgs& a, int b) {
-    len = kv_length(a.c, b, kErrAttend);
-    first = first_in_window(len, a.window);
+// ONE in what follows: one token per sequence (tc_attend); what chunks need besides is then left out of the code.
+// A sequence's query tokens in blocks of a.block: rows row0 .. row0 + rows - 1 of q are the last n of its
+// len tokens (rows < n where q ends before them).
+template <bool ONE>
+struct Seq {
+  int b, len, n, row0, rows, nblk;
+  __device__ __forceinline__ Seq(const AttendArgs& a, int b_) : b(b_) {
+    len = kv_length(a.c, b, a.code);
+    n = 1;
+    row0 = b;
+    rows = 1;
+    if (!ONE) {
+      row0 = __ldg(a.cu + b);
+      n = max(__ldg(a.cu + b + 1) - row0, 0);
+      rows = row0 < 0 ? 0 : max(min(n, a.tokens - row0), 0);
+    }
+    nblk = ONE ? 1 : a.block == 1 ? rows : (rows + a.block - 1) / a.block;
+  }
+};
+// A block of tokens: the first one's position, how many, and the slots that any of them sees, [0, head) and
+// [first, end), in nt chunks: chunks 0 .. na - 1, then from t0 on.
+template <bool ONE>
+struct Block {
+  int tb, pos, ntok, end, first, head, na, t0, nt;
+  __device__ __forceinline__ Block(const AttendArgs& a, const Seq<ONE>& q, int tb_) : tb(tb_) {
+    pos = ONE ? q.len - 1 : q.len - q.n + tb * a.block;
+    ntok = ONE ? 1 : min(a.block, q.rows - tb * a.block);
+    end = max(pos + ntok, 0);
+    first = pos >= 0 ? first_in_window(pos + 1, a.window) : 0;
     head = min(a.sinks, first);
     t0 = first / kTile;
     na = min((head + kTile - 1) / kTile, t0);
-    nt = len ? na + (len + kTile - 1) / kTile - t0 : 0;
+    nt = ntok > 0 && end > 0 ? na + (end + kTile - 1) / kTile - t0 : 0;
   }
   __device__ __forceinline__ int tile(int i) const { return i < na ? i : t0 + i - na; }
-  __device__ __forceinline__ bool visible(int j) const { return j < len && (j >= first || j < head); }
-  __device__ __forceinline__ bool whole(int j0) const { return j0 + kTile <= len && (j0 >= first || j0 + kTile <= head); }
+  __device__ __forceinline__ bool visible(int j) const { return j < end && (j >= first || j < head); }
+  // every row sees all slots of the chunk
+  __device__ __forceinline__ bool whole(const AttendArgs& a, int j0) const {
+    return j0 + kTile <= pos + 1 && (j0 >= (ONE ? first : first_in_window(end, a.window)) || j0 + kTile <= a.sinks);
+  }
 };
 
-struct PlanShared {
-  long long warp[8];
-  long long into;
-  int b;
-};
-// The tiles of the whole call are cut into runs of total / runs (rounded down) or one more; there are
-// no more runs than leave every warp of a CTA a tile, so none is empty.
+// x * i / n rounded down, i <= n, n at most a few hundred: 32-bit arithmetic (a quarter of the time) while it serves.
+__device__ __forceinline__ long long part_of(long long x, int i, int n) {
+  return x < (1 << 22) ? (long long)((uint32_t)x * (uint32_t)i / (uint32_t)n) : x * i / n;
+}
+// The chunks of the whole call are cut into runs of total / runs (rounded down) or one more; there are
+// no more runs than leave every warp of a CTA a chunk, so none is empty.
 __device__ __forceinline__ int runs_of(long long total, int grid, int warps) {
   return (int)min((total + warps - 1) / warps, (long long)grid);
 }
-__device__ __forceinline__ long long run_begin(long long total, int runs, int i) { return total * i / runs; }
-// The run that holds tile t: the last one that begins at or before it.
-__device__ __forceinline__ int run_of(long long total, int runs, long long t) { return (int)(((t + 1) * runs - 1) / total); }
+__device__ __forceinline__ long long run_begin(long long total, int runs, int i) { return part_of(total, i, runs); }
+// The run that holds chunk t: the last one that begins at or before it.
+__device__ __forceinline__ int run_of(long long total, int runs, long long t) {
+  const long long x = (t + 1) * runs - 1;
+  return max(x, total) <= 0x7FFFFFFF ? (int)((uint32_t)x / (uint32_t)total) : (int)(x / total);
+}
 
-// The tiles of the whole call (every thread of the CTA calls it; at most 256 threads), and *before: the
-// tiles before sequence `want`; or, want < 0, s.b = the sequence that holds the first tile of run
-// `run` and the tiles of it before that one.
-__device__ __forceinline__ long long plan(const AttendArgs& a, int nsub, PlanShared& s, int want, int run, int grid,
-                                          int warps, long long* before) {
-  const int T = blockDim.x, t = threadIdx.x, B = a.c.batch, per = (B + T - 1) / T;
-  const int lo = min(B, t * per), hi = min(B, lo + per), warp = t >> 5, lane = t & 31;
+// What plan() finds: the chunks of the whole call, a block of tokens by its number in the batch, its sequence
+// (-1: there is none) and its place in that, and a number of chunks before something.
+struct Plan {
+  long long total, before;
+  int b, tb, group;
+};
+struct PlanShared {
+  long long warp[8];
+  int groups[8];
+  Plan found;
+};
+constexpr int kSolo = 64;            // up to this many sequences every warp scans the batch for itself, without a barrier
+// Every thread of the CTA calls it (at most 256 threads). Finds block number `want` and the chunks before it; or,
+// want < 0, the block that holds the first chunk of run `run` and the chunks of it before that one.
+template <bool ONE>
+__device__ __forceinline__ Plan plan(const AttendArgs& a, int nsub, PlanShared& s, int want, int run, int grid, int warps) {
+  const int B = a.c.batch, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool solo = B <= kSolo;
+  const int T = solo ? 32 : blockDim.x, t = solo ? lane : threadIdx.x, per = (B + T - 1) / T;
+  const int lo = min(B, t * per), hi = min(B, lo + per);
   long long mine = 0;
-  for (int b = lo; b < hi; ++b) mine += (long long)SeqTiles(a, b).nt * nsub;
+  int groups = 0;
+  for (int b = lo; b < hi; ++b) {
+    const Seq<ONE> q(a, b);
+    groups += q.nblk;
+    for (int tb = 0; tb < q.nblk; ++tb) mine += (long long)Block<ONE>(a, q, tb).nt * nsub;
+  }
   long long sum = mine;
+  int gsum = groups;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-    if (lane >= o) sum += y;
-  }
-  if (lane == 31) s.warp[warp] = sum;
-  __syncthreads();
-  long long base = 0, total = 0;
-  for (int w = 0; w < T / 32; ++w) {
-    if (w < warp) base += s.warp[w];
-    total += s.warp[w];
-  }
-  long long at = base + sum - mine;                          // tiles before this thread's sequences
-  const int runs = runs_of(total, grid, warps);
-  const long long find = want < 0 && run < runs ? run_begin(total, runs, run) : total;
-  if (want < 0 ? mine && find >= at && find < at + mine : want >= lo && want < hi) {
-    int b = lo;
-    for (;; ++b) {
-      if (b == want) break;
-      const long long n = (long long)SeqTiles(a, b).nt * nsub;
-      if (want < 0 && find < at + n) break;
-      at += n;
+    const int z = __shfl_up_sync(0xFFFFFFFFu, gsum, o);
+    if (lane >= o) {
+      sum += y;
+      gsum += z;
     }
-    s.b = b;
-    s.into = want < 0 ? find - at : at;
   }
-  __syncthreads();
-  *before = s.into;
-  return total;
+  Plan p{0, 0, -1, 0, 0};
+  long long at = sum - mine;                                 // chunks and blocks before this thread's sequences
+  int group = gsum - groups;
+  if (solo) {
+    p.total = __shfl_sync(0xFFFFFFFFu, sum, 31);
+  } else {
+    if (lane == 31) {
+      s.warp[warp] = sum;
+      s.groups[warp] = gsum;
+    }
+    if (t == 0) s.found.b = -1;
+    __syncthreads();
+    for (int w = 0; w < T / 32; ++w) {
+      if (w < warp) {
+        at += s.warp[w];
+        group += s.groups[w];
+      }
+      p.total += s.warp[w];
+    }
+  }
+  const int runs = runs_of(p.total, grid, warps);
+  const long long find = want < 0 && run < runs ? run_begin(p.total, runs, run) : p.total;
+  if (want < 0 ? mine && find >= at && find < at + mine : want >= group && want < group + groups) {
+    for (int b = lo; b < hi && p.b < 0; ++b) {
+      const Seq<ONE> q(a, b);
+      for (int tb = 0; tb < q.nblk && p.b < 0; ++tb) {
+        const long long n = (long long)Block<ONE>(a, q, tb).nt * nsub;
+        if (want < 0 ? find < at + n : group == want) {
+          p.b = b;
+          p.tb = tb;
+          p.group = group;
+          p.before = want < 0 ? find - at : at;
+        }
+        at += n;
+        ++group;
+      }
+    }
+  }
+  if (solo) {
+    const uint32_t who = __ballot_sync(0xFFFFFFFFu, p.b >= 0);
+    const int from = who ? __ffs(who) - 1 : 0;
+    p.b = __shfl_sync(0xFFFFFFFFu, p.b, from);
+    p.tb = __shfl_sync(0xFFFFFFFFu, p.tb, from);
+    p.group = __shfl_sync(0xFFFFFFFFu, p.group, from);
+    p.before = __shfl_sync(0xFFFFFFFFu, p.before, from);
+  } else {
+    if (p.b >= 0) s.found = p;
+    __syncthreads();
+    p.b = s.found.b;
+    p.tb = s.found.tb;
+    p.group = s.found.group;
+    p.before = s.found.before;
+  }
+  return p;
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -145,6 +229,7 @@ __device__ __forceinline__ float shrink(float m, float m2) { return m2 == neg_in
 struct AttendWs {
   float* part;
   int* redo;                         // per item that one CTA holds whole: an output is not finite
+  int64_t items;
   float2* ml;
   float* scores;
   int64_t cap;                       // slots a row of scores holds
@@ -157,20 +242,32 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 
 // The parts of items that a CTA's run consists of, one after the other: chunks [i0, i1) of an item.
+template <bool ONE>
 struct Walk {
-  int left, b, sub, i0, i1;          // left: chunks of the run from this part on
-  SeqTiles sq;
-  __device__ __forceinline__ Walk(const AttendArgs& a, int left_, int b_, int sub_, int first)
-      : left(left_), b(b_), sub(sub_), i0(first), i1(0), sq(a, b_) {
-    i1 = min(sq.nt, first + left);
+  int left, group, sub, i0, i1;      // left: chunks of the run from this part on
+  Seq<ONE> q;
+  Block<ONE> sq;
+  __device__ __forceinline__ Walk(const AttendArgs& a, int left_, const Plan& p)
+      : left(left_), group(p.group), sub(0), i0(0), i1(0), q(a, p.b), sq(a, q, p.tb) {
+    sub = p.before <= 0x7FFFFFFF ? (int)((uint32_t)p.before / (uint32_t)sq.nt) : (int)(p.before / sq.nt);
+    i0 = (int)(p.before - (long long)sub * sq.nt);
+    i1 = min(sq.nt, i0 + left);
   }
   __device__ __forceinline__ bool next(const AttendArgs& a, int nsub) {
     left -= i1 - i0;
     if (left <= 0) return false;
     if (++sub == nsub) {
       sub = 0;
-      do sq = SeqTiles(a, ++b);
-      while (sq.nt == 0);
+      do {                                        // (a sequence without rows has no block to count)
+        int tb = sq.tb + 1;
+        if (q.nblk > 0) ++group;
+        if (tb >= q.nblk) {
+          if (q.b + 1 >= a.c.batch) return false;  // (only if the lengths changed under the call)
+          q = Seq<ONE>(a, q.b + 1);
+          tb = 0;
+        }
+        sq = Block<ONE>(a, q, tb);
+      } while (sq.nt == 0);
     }
     i0 = 0;
     i1 = min(sq.nt, left);
@@ -178,7 +275,7 @@ struct Walk {
   }
 };
 
-template <class T, int HD, int NB>
+template <class T, int HD, int NB, bool ONE>
 __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
     k_attend(const __grid_constant__ AttendArgs a, AttendWs ws, int gblocks, int hb) {
   using Sh = AttendShape<HD>;
@@ -190,19 +287,17 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
   const KvCache& c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.nh / c.n_kv, nsub = c.n_kv * gblocks;
-  long long into = 0;
-  const long long total = plan(a, nsub, s_plan, -1, blockIdx.x, gridDim.x, W, &into);
-  const int runs = runs_of(total, gridDim.x, W);
+  const Plan p = plan<ONE>(a, nsub, s_plan, -1, blockIdx.x, gridDim.x, W);
+  const int runs = runs_of(p.total, gridDim.x, W);
   if ((int)blockIdx.x >= runs) return;
-  const int left = (int)(run_begin(total, runs, blockIdx.x + 1) - run_begin(total, runs, blockIdx.x));
-  const int nt0 = SeqTiles(a, s_plan.b).nt, sub0 = (int)(into / nt0), first = (int)(into - (long long)sub0 * nt0);
+  Walk<ONE> w(a, (int)(run_begin(p.total, runs, blockIdx.x + 1) - run_begin(p.total, runs, blockIdx.x)), p);
   const uint32_t s_at = smem_u32(s_raw), pad = (512 - (s_at & 511)) % 512, ring = s_at + pad + warp * Sh::kRing;
   float* s_out = reinterpret_cast<float*>(s_raw + pad + W * Sh::kRing);
 
   // ---- the copies: a chunk's keys, its values, the next chunk's keys ..., U - 1 units ahead of their
   // use. A chunk's page id is loaded one chunk earlier still and only looked at when it is copied.
-  Walk pw(a, left, s_plan.b, sub0, first);
-  int pi = first + warp, page = -1, to_slot = 0;
+  Walk<ONE> pw = w;
+  int pi = w.i0 + warp, page = -1, to_slot = 0;
   uint32_t held = 0;                              // bit x: the unit copied x copies ago is in the ring
   bool more = true;
   // A row's 16-byte piece p is kept at place p ^ (row % 8) of its 128 bytes (no bank conflicts in ldmatrix);
@@ -217,18 +312,18 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
       more = pw.next(a, nsub);
       pi = pw.i0 + warp;
     }
-    if (more) page = __ldg(c.table + (int64_t)pw.b * c.ts + (pw.sq.tile(pi) * kTile >> c.shift));
+    if (more) page = __ldg(c.table + (int64_t)pw.q.b * c.ts + (pw.sq.tile(pi) * kTile >> c.shift));
   };
   auto copy = [&](const uint8_t* pool, bool last) {
     const bool good = more && (unsigned)page < (unsigned)c.n_pages;
-    if (more && !good) kv_fail(c, kErrAttend);
+    if (more && !good) kv_fail(c, a.code);
     held = held << 1 | good;
     if (good) {
       const int j0 = pw.sq.tile(pi) * kTile;
       const uint8_t* from = pool + 2 * ((int64_t)page * c.sp + (int64_t)((j0 & ((1 << c.shift) - 1)) + r0) * c.ss +
                                         (int64_t)(pw.sub / gblocks) * c.sh) + 16 * (lane % kLanes);
       const uint32_t to = put + to_slot * Sh::kMat;
-      if (pw.sq.whole(j0)) {
+      if (j0 + kTile <= pw.sq.end && (j0 >= pw.sq.first || j0 + kTile <= pw.sq.head)) {
 #pragma unroll
         for (int x = 0; x < kTile / kAtOnce; ++x)
           asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"((to ^ (x * kAtOnce % 8 << 4)) + x * kAtOnce * HD * 2),
@@ -251,28 +346,41 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
 #pragma unroll
   for (int x = 0; x < U - 1; ++x) copy(x & 1 ? c.v : c.k, x & 1);
 
-  Walk w(a, left, s_plan.b, sub0, first);
   int slot = 0;
   // where ldmatrix reads: keys, slots 0-15 of columns 0-7 then 8-15; values, slots 0-7 of columns 0-7 and 8-15,
   // then slots 8-15. The next 16 columns are 32 bytes on, which flips bits of the place.
   const uint32_t k_at = ring + (lane & 15) * HD * 2 + (((lane >> 4) ^ (lane & 7)) << 4);
   const uint32_t v_at = ring + ((lane & 7) + (lane >> 4) * 8) * HD * 2 + (((lane >> 3 & 1) ^ (lane & 7)) << 4);
   do {
-    const int kvh = w.sub / gblocks, g0 = (w.sub - kvh * gblocks) * hb, h0 = kvh * G + g0, rows = min(hb, G - g0);
-    // the query rows as the MMA's second operand: head lane / 4, columns 2 (lane % 4) (+ 1, + 8, + 9) of each 16
+    // row r of the item is head h0 + r % heads of token r / heads of the block
+    const int kvh = w.sub / gblocks, g0 = (w.sub - kvh * gblocks) * hb, h0 = kvh * G + g0, heads = min(hb, G - g0),
+              rows = heads * w.sq.ntok, row0 = w.q.row0 + w.sq.tb * a.block;
+    // the query rows as the MMA's second operand: row lane / 4, columns 2 (lane % 4) (+ 1, + 8, + 9) of each 16
     uint32_t q[NB][HD / 16][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int nb = 0; nb < NB; ++nb) {
+      const int r = 8 * nb + (lane >> 2), rr = min(r, rows - 1), tok = ONE ? 0 : rr / heads;
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(
+          a.q + 2 * ((int64_t)(row0 + tok) * a.qr + (int64_t)(h0 + rr - tok * heads) * a.qh + 2 * (lane & 3)));
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int r = 8 * nb + (lane >> 2), col = 16 * kk + 2 * (lane & 3) + 8 * x;
-          q[nb][kk][x] = 0;
-          if (r < rows)
-            q[nb][kk][x] = __ldg(reinterpret_cast<const uint32_t*>(a.q + 2 * ((int64_t)w.b * a.qr + (int64_t)(h0 + r) * a.qh + col)));
-        }
-    // this warp's state: rows (lane / 4, + 8) of each 16 columns of O^T, heads 2 (lane % 4) (+ 1) of each block of 8
+        for (int x = 0; x < 2; ++x) q[nb][kk][x] = __ldg(from + 8 * kk + 4 * x);
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) q[nb][kk][x] = r < rows ? q[nb][kk][x] : 0;
+    }
+    // rows 2 (lane % 4) (+ 1) of each block of 8 are this lane's in the scores and outputs: what they see
+    int last[NB][2], from[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        last[nb][y] = w.sq.pos + (ONE ? 0 : (8 * nb + 2 * (lane & 3) + y) / heads);
+        from[nb][y] = ONE ? w.sq.first : first_in_window(last[nb][y] + 1, a.window);
+      }
+    // this warp's state: rows (lane / 4, + 8) of each 16 columns of O^T, those two rows of q in each block of 8
     float o[HD / 16][NB][4], m[NB][2], l[NB][2];
     bool any = false;
 #pragma unroll
@@ -305,20 +413,33 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) mma16816<T>(kk & 1 ? s2[nb] : s[nb], f, q[nb][kk][0], q[nb][kk][1]);
       }
-      const bool whole = w.sq.whole(j0);
+      const bool whole = w.sq.whole(a, j0);
       const int r = lane >> 2;
-      const bool show[2] = {here && (whole || w.sq.visible(j0 + r)), here && (whole || w.sq.visible(j0 + r + 8))};
+      // bit 4 nb + e: element e of block nb is visible (with one token the same bits for every block and row)
+      constexpr int kShow = ONE ? 1 : NB;
+      uint32_t show = here ? ~0u : 0;
+      if (here && !whole) {
+        show = 0;
+#pragma unroll
+        for (int nb = 0; nb < kShow; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = j0 + r + 8 * (e >> 1);
+            if (j <= last[nb][e & 1] && (j >= from[nb][e & 1] || j < a.sinks)) show |= 1u << (4 * nb + e);
+          }
+      }
+      auto seen = [&](int nb, int e) { return show >> (4 * (ONE ? 0 : nb) + (ONE ? e & 2 : e)) & 1; };
       float top[NB][2];
       bool grow = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nb][e] = show[e >> 1] ? (s[nb][e] + s2[nb][e]) * a.scale2 : neg_inf();
+        for (int e = 0; e < 4; ++e) s[nb][e] = seen(nb, e) ? (s[nb][e] + s2[nb][e]) * a.scale2 : neg_inf();
         if (ws.scores && here) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int h = 8 * nb + 2 * (lane & 3) + (e & 1);
-            if (h < rows) ws.scores[((int64_t)w.b * a.nh + h0 + h) * ws.cap + j0 + r + 8 * (e >> 1)] = s[nb][e];
+            const int h = 8 * nb + 2 * (lane & 3) + (e & 1);  // (scores are kept for one token a sequence: row = head)
+            if (h < rows) ws.scores[((int64_t)w.q.b * a.nh + h0 + h) * ws.cap + j0 + r + 8 * (e >> 1)] = s[nb][e];
           }
         }
 #pragma unroll
@@ -353,7 +474,7 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float base = m[nb][e & 1] == neg_inf() ? 0.0f : m[nb][e & 1];
-          p[e] = show[e >> 1] ? ex2(s[nb][e] - base) : 0.0f;
+          p[e] = seen(nb, e) ? ex2(s[nb][e] - base) : 0.0f;
         }
         l[nb][0] += p[0] + p[2];
         l[nb][1] += p[1] + p[3];
@@ -444,9 +565,10 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
             const float inv = met ? 1.0f / sum : 0.0f;
             v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
             good &= fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < __int_as_float(0x7F800000);
-            *reinterpret_cast<uint2*>(a.out + 2 * ((int64_t)w.b * a.orow + (int64_t)(h0 + h) * a.oh + col)) =
-                make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
-            if (col == 0 && ws.ml) ws.ml[(int64_t)w.b * a.nh + h0 + h] = make_float2(mm, sum);
+            const int tok = ONE ? 0 : h / heads;
+            *reinterpret_cast<uint2*>(a.out + 2 * ((int64_t)(row0 + tok) * a.orow + (int64_t)(h0 + h - tok * heads) * a.oh +
+                                                   col)) = make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
+            if (col == 0 && ws.ml) ws.ml[(int64_t)w.q.b * a.nh + h0 + h] = make_float2(mm, sum);
           } else {
             *reinterpret_cast<float4*>(part + h * HD + col) = v;
             if (col == 0) {
@@ -458,17 +580,18 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
       }
     }
     const int bad = __syncthreads_or(!good);
-    if (all && threadIdx.x == 0) ws.redo[(int64_t)w.b * nsub + w.sub] = bad;
+    const int64_t item = (int64_t)w.group * nsub + w.sub;         // (beyond the workspace only if cu is not ascending)
+    if (all && threadIdx.x == 0 && item < ws.items) ws.redo[item] = bad;
   } while (w.next(a, nsub));
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // The items whose tiles lie in several CTAs' runs: their states at the common maximum. One CTA per
-// (sequence, head block, row): its warps take the pieces in turn, and their sums are added in warp
-// order. Sequences without a slot get zeros. A row with a NaN or an infinity is computed again key by
+// (block, head block, row): its warps take the pieces in turn, and their sums are added in warp
+// order. Blocks that see no slot get zeros. A row with a NaN or an infinity is computed again key by
 // key: the second half of a split probability times an infinite value would make a NaN of it.
 constexpr int kJoinWarps = 8, kJoinThreads = 32 * kJoinWarps;
-template <class T, int HD>
+template <class T, int HD, bool ONE>
 __global__ void __launch_bounds__(kJoinThreads)
     k_join(const __grid_constant__ AttendArgs a, AttendWs ws, int grid, int gblocks, int hb) {
   using Sh = AttendShape<HD>;
@@ -477,21 +600,24 @@ __global__ void __launch_bounds__(kJoinThreads)
   griddep_launch();
   const KvCache& c = a.c;
   const int G = a.nh / c.n_kv, nsub = c.n_kv * gblocks;
-  const int item = blockIdx.x / hb, r = blockIdx.x - item * hb, b = item / nsub, sub = item - b * nsub;
-  const int kvh = sub / gblocks, g0 = (sub - kvh * gblocks) * hb, h = kvh * G + g0 + r;
-  long long at = 0;
-  const long long total = plan(a, nsub, s_plan, b, 0, 1, Sh::kWarps, &at);
-  const int nt = SeqTiles(a, b).nt;
-  griddep_wait();
-  if (g0 + r >= G) return;
+  const int most = ONE ? hb : hb * a.block, item = blockIdx.x / most, r = blockIdx.x - item * most, sub = item % nsub;
+  const int kvh = sub / gblocks, g0 = (sub - kvh * gblocks) * hb, heads = min(hb, G - g0);
+  const Plan p = plan<ONE>(a, nsub, s_plan, item / nsub, 0, 1, Sh::kWarps);
+  const long long total = p.total;
+  griddep_wait();                                // (before any return: what follows in the stream counts on it)
+  if (p.b < 0) return;
+  const Seq<ONE> q(a, p.b);
+  const Block<ONE> sq(a, q, p.tb);
+  const int nt = sq.nt, tok = ONE ? r >= heads : r / heads, h = kvh * G + g0 + r - tok * heads, row = q.row0 + sq.tb * a.block + tok;
+  if (tok >= sq.ntok) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t at_out = (int64_t)b * a.orow + (int64_t)h * a.oh;
+  const int64_t at_out = (int64_t)row * a.orow + (int64_t)h * a.oh;
   uint32_t* to = reinterpret_cast<uint32_t*>(a.out + 2 * at_out);
   if (nt == 0) {
     for (int x = threadIdx.x; x < HD / 2; x += kJoinThreads) to[x] = 0;
     return;
   }
-  const long long t0 = at + (long long)sub * nt;
+  const long long t0 = p.before + (long long)sub * nt;
   const int runs = runs_of(total, grid, Sh::kWarps), c0 = run_of(total, runs, t0), c1 = run_of(total, runs, t0 + nt - 1);
   bool redo = c0 == c1;
   if (redo && !ws.redo[item]) return;
@@ -562,13 +688,13 @@ __global__ void __launch_bounds__(kJoinThreads)
       good = fabsf(v.x) + fabsf(v.y) < __int_as_float(0x7F800000);
       to[threadIdx.x] = Elem<T>::pack(v.x, v.y);
     }
-    if (ws.ml && threadIdx.x == 0) ws.ml[(int64_t)b * a.nh + h] = make_float2(m, l);
+    if (ws.ml && threadIdx.x == 0) ws.ml[(int64_t)q.b * a.nh + h] = make_float2(m, l);
     redo = __syncthreads_or(!good);
   }
   if (redo && warp == 0) {
-    float q[HD / 32], o[HD / 32];
-    row_load<T, HD>(a.q, (int64_t)b * a.qr + (int64_t)h * a.qh, lane, q);
-    attend_row<T, HD>(c, b, kvh, q, a.scale2, SeqTiles(a, b).len, a.window, a.sinks, kErrAttend, o);
+    float x[HD / 32], o[HD / 32];
+    row_load<T, HD>(a.q, (int64_t)row * a.qr + (int64_t)h * a.qh, lane, x);
+    attend_row<T, HD>(c, q.b, kvh, x, a.scale2, max(sq.pos + tok + 1, 0), a.window, a.sinks, a.code, o);
     row_store<T, HD>(a.out, at_out, lane, o);
   }
 }
@@ -606,13 +732,25 @@ __global__ void __launch_bounds__(kWeightThreads) k_weights(const __grid_constan
 }
 
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
-AttendWs ws_of(const KvCache& c, int nh, bool weights, uint8_t* ws, uint64_t* bytes) {
+// A group's heads in blocks of nearly equal size (at most 16), and the blocks of tokens a call may have.
+struct Shape {
+  int gblocks, hb, nsub;
+  int64_t groups;
+};
+Shape shape_of(const KvCache& c, int nh, int block, int tokens) {
+  const int G = nh / c.n_kv, gblocks = (G + kRowsMma - 1) / kRowsMma;
+  // (every sequence ends in at most one block that is not full; tokens < 0: one token a sequence)
+  const int64_t groups = tokens < 0 ? c.batch : std::min<int64_t>(tokens, tokens / block + std::min(tokens, c.batch));
+  return Shape{gblocks, (G + gblocks - 1) / gblocks, c.n_kv * gblocks, groups};
+}
+AttendWs ws_of(const KvCache& c, int nh, int64_t items, bool weights, uint8_t* ws, uint64_t* bytes) {
   AttendWs w{};
   int64_t at = 0;
   w.part = reinterpret_cast<float*>(ws);
   at += up256((int64_t)kMaxGrid * 2 * (kRowsMma * c.hd + 2 * kRowsMma) * 4);
   w.redo = reinterpret_cast<int*>(ws + at);
-  at += up256((int64_t)c.batch * c.n_kv * ((nh / c.n_kv + kRowsMma - 1) / kRowsMma) * 4);
+  w.items = items;
+  at += up256(items * 4);
   if (weights) {
     w.ml = reinterpret_cast<float2*>(ws + at);
     at += up256((int64_t)c.batch * nh * 8);
@@ -624,24 +762,25 @@ AttendWs ws_of(const KvCache& c, int nh, bool weights, uint8_t* ws, uint64_t* by
   return w;
 }
 
-template <class T, int HD>
+template <class T, int HD, bool ONE>
 cudaError_t attend_hd(const AttendArgs& a, cudaStream_t st) {
   using Sh = AttendShape<HD>;
   const KvCache& c = a.c;
+  const Shape sh = shape_of(c, a.nh, a.block, ONE ? -1 : a.tokens);
   uint64_t bytes = 0;
-  const AttendWs ws = ws_of(c, a.nh, a.weight_out != nullptr, a.ws, &bytes);
-  // a group's heads in blocks of nearly equal size, of 8 or of 16 places
-  const int G = a.nh / c.n_kv, gblocks = (G + kRowsMma - 1) / kRowsMma, hb = (G + gblocks - 1) / gblocks;
-  auto kern = hb <= 8 ? k_attend<T, HD, 1> : k_attend<T, HD, 2>;
-  cudaError_t e = hb <= 8 ? allow_smem<k_attend<T, HD, 1>>(Sh::kSmem) : allow_smem<k_attend<T, HD, 2>>(Sh::kSmem);
+  const AttendWs ws = ws_of(c, a.nh, sh.groups * sh.nsub, a.weight_out != nullptr, a.ws, &bytes);
+  const bool one = sh.hb * a.block <= 8;         // rows of an item
+  auto kern = one ? k_attend<T, HD, 1, ONE> : k_attend<T, HD, 2, ONE>;
+  cudaError_t e = one ? allow_smem<k_attend<T, HD, 1, ONE>>(Sh::kSmem) : allow_smem<k_attend<T, HD, 2, ONE>>(Sh::kSmem);
   if (e != cudaSuccess) return e;
   // no more CTAs than the page lists can hold chunks for
-  const int nsub = c.n_kv * gblocks;
-  const int64_t most = ((int64_t)c.batch * nsub * (((int64_t)c.max_pages << c.shift) / kTile) + Sh::kWarps - 1) / Sh::kWarps;
-  const int grid = (int)std::min<int64_t>(kMaxGrid, most);
-  kern<<<grid, Sh::kThreads, Sh::kSmem, st>>>(a, ws, gblocks, hb);
+  const int64_t chunks = ((int64_t)c.max_pages << c.shift) / kTile;
+  const int grid = (int)std::min<int64_t>(kMaxGrid, (sh.groups * sh.nsub * chunks + Sh::kWarps - 1) / Sh::kWarps);
+  const int64_t joins = sh.groups * sh.nsub * sh.hb * a.block;
+  if (joins > INT32_MAX) return cudaErrorInvalidValue;
+  kern<<<grid, Sh::kThreads, Sh::kSmem, st>>>(a, ws, sh.gblocks, sh.hb);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  e = launch_dependent(k_join<T, HD>, dim3(c.batch * nsub * hb), dim3(kJoinThreads), st, a, ws, grid, gblocks, hb);
+  e = launch_dependent(k_join<T, HD, ONE>, dim3((unsigned)joins), dim3(kJoinThreads), st, a, ws, grid, sh.gblocks, sh.hb);
   if (e != cudaSuccess || !a.weight_out) return e;
   const int kvrows = c.batch * c.n_kv;
   const int64_t blocks = (((int64_t)c.max_pages << c.shift) + kWeightThreads - 1) / kWeightThreads;
@@ -649,24 +788,59 @@ cudaError_t attend_hd(const AttendArgs& a, cudaStream_t st) {
                           dim3(kWeightThreads), st, a, ws);
 }
 
-template <class T>
+template <class T, bool ONE>
 cudaError_t attend_of(const AttendArgs& a, cudaStream_t st) {
   switch (a.c.hd) {
-    case 64: return attend_hd<T, 64>(a, st);
-    case 128: return attend_hd<T, 128>(a, st);
-    default: return attend_hd<T, 256>(a, st);
+    case 64: return attend_hd<T, 64, ONE>(a, st);
+    case 128: return attend_hd<T, 128, ONE>(a, st);
+    default: return attend_hd<T, 256, ONE>(a, st);
   }
 }
 
 }  // namespace
 
 uint64_t attend_workspace(const KvCache& c, int nh, bool weights) {
+  const Shape sh = shape_of(c, nh, 1, -1);
   uint64_t bytes = 0;
-  ws_of(c, nh, weights, nullptr, &bytes);
+  ws_of(c, nh, sh.groups * sh.nsub, weights, nullptr, &bytes);
   return bytes;
 }
-cudaError_t launch_attend(const AttendArgs& a, cudaStream_t st) {
-  return a.dtype == TC_BF16 ? attend_of<__nv_bfloat16>(a, st) : attend_of<__half>(a, st);
+cudaError_t launch_attend(AttendArgs a, cudaStream_t st) {
+  a.block = 1;
+  a.code = kErrAttend;
+  return a.dtype == TC_BF16 ? attend_of<__nv_bfloat16, true>(a, st) : attend_of<__half, true>(a, st);
+}
+
+// Which of the two kernels takes a chunk of a prompt, by their times on a B200 in microseconds, fitted to
+// measurements at 1 to 128 tokens of 1, 8 and 32 sequences behind 1000 and 16000 slots (16 heads on 8 of 128,
+// 4 on 1 of 256). This one passes over a sequence's slots once for each block of rows and head block
+// (8 x 4 tokens behind 1000 slots, 16 heads on 8: 20 us against 24; 8 x 16: 49 against 25; behind 16000
+// slots 95 against 251 and 200 against 252); the prompt kernel's time is that of its blocks of 128 (64) slots
+// one after the other while its CTAs fit on the SMs. The lengths are the device's: the page lists' room
+// stands in for them.
+int chunk_block(const KvCache& c, int nh, int tokens, int window, int sinks) {
+  const Shape sh = shape_of(c, nh, 1, tokens);
+  const int each = (tokens + c.batch - 1) / c.batch, rows = sh.hb * each;
+  const int block = std::max(1, (rows <= 8 ? 8 : kRowsMma) / sh.hb);
+  const double keys = std::min((double)((int64_t)c.max_pages << c.shift), (double)window + sinks + each);
+  const double items = (double)std::min(tokens, c.batch) * sh.nsub, passes = items * ((each + block - 1) / block);
+  const double few = 10 + passes * ((rows <= 8 ? 0.12 : 0.2) + keys * c.hd * (rows <= 8 ? 0.6e-6 : 0.7e-6));
+  const double spans = items * ((each * sh.hb + 255) / 256), waves = std::ceil(spans / kMaxGrid);
+  const double many = 8 + waves * keys * (c.hd == 256 ? 24e-3 : 15e-3);
+  return few < many ? block : 0;
+}
+uint64_t chunk_workspace(const KvCache& c, int nh, int tokens, int window, int sinks) {
+  const int block = chunk_block(c, nh, tokens, window, sinks);
+  if (!block) return 0;
+  const Shape sh = shape_of(c, nh, block, tokens);
+  uint64_t bytes = 0;
+  ws_of(c, nh, sh.groups * sh.nsub, false, nullptr, &bytes);
+  return bytes;
+}
+cudaError_t launch_attend_chunk(AttendArgs a, cudaStream_t st) {
+  a.block = chunk_block(a.c, a.nh, a.tokens, a.window, a.sinks);
+  a.code = kErrPrompt;
+  return a.dtype == TC_BF16 ? attend_of<__nv_bfloat16, false>(a, st) : attend_of<__half, false>(a, st);
 }
 
 }  // namespace tc

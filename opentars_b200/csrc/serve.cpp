@@ -109,17 +109,31 @@ int tc_attend(const tc_kv_cache* c, const void* q, int64_t q_row_stride, int64_t
 
 int tc_attend_prompt(const tc_kv_cache* c, const void* q, int64_t q_row_stride, int64_t q_head_stride, void* out,
                      int64_t out_row_stride, int64_t out_head_stride, int32_t n_heads, const int32_t* cu,
-                     int32_t tokens, float scale, int32_t window, int32_t sinks, void* stream) {
+                     int32_t tokens, float scale, int32_t window, int32_t sinks, void* ws, uint64_t ws_bytes,
+                     void* stream) {
   AttendArgs a{};
   if (tokens < 0 || tokens > (1 << 28) || !cu) return TC_ERR_ARG;
   if (tokens == 0) return take_cache(c, &a.c) ? TC_OK : TC_ERR_ARG;
   if (!take_attend(c, q, q_row_stride, q_head_stride, out, out_row_stride, out_head_stride, n_heads, scale, window,
                    sinks, &a))
     return TC_ERR_ARG;
+  const uint64_t need = chunk_workspace(a.c, n_heads, tokens, a.window, a.sinks);
+  if (need && (!ws || (uintptr_t)ws % 256 || ws_bytes < need)) return TC_ERR_ARG;
   a.cu = cu;
   a.tokens = tokens;
+  a.ws = static_cast<uint8_t*>(ws);
   if (!take_error(&a.c)) return TC_ERR_CUDA;
-  return done(launch_attend_prompt(a, static_cast<cudaStream_t>(stream)));
+  return done(need ? launch_attend_chunk(a, static_cast<cudaStream_t>(stream))
+                   : launch_attend_prompt(a, static_cast<cudaStream_t>(stream)));
+}
+
+uint64_t tc_attend_prompt_workspace(const tc_kv_cache* c, int32_t n_heads, int32_t tokens, int32_t window,
+                                    int32_t sinks) {
+  KvCache o{};
+  if (!take_cache(c, &o) || n_heads < 1 || n_heads % c->n_kv || n_heads > (1 << 16) || tokens < 1 ||
+      tokens > (1 << 28) || window < 0 || sinks < 0)
+    return 0;
+  return chunk_workspace(o, n_heads, tokens, window ? window : INT_MAX, sinks);
 }
 
 uint64_t tc_kv_evict_workspace(const tc_kv_cache* c, int32_t budget) {

@@ -48,10 +48,15 @@ struct AttendArgs {
   uint8_t* ws;
   const int* cu;                     // prompt only
   int tokens;
-  uint32_t spin;                     // poll limit of the bounded waits (set by the launcher)
+  uint32_t spin;                     // poll limit of the bounded waits
+  int block, code;                   // set by the launchers: tokens of an MMA, the error code of bad pages
 };
 uint64_t attend_workspace(const KvCache& c, int nh, bool weights);
-cudaError_t launch_attend(const AttendArgs& a, cudaStream_t st);
+cudaError_t launch_attend(AttendArgs a, cudaStream_t st);
+// Chunks of few rows: the tokens of an MMA's block, or 0 where the prompt kernel takes the call.
+int chunk_block(const KvCache& c, int nh, int tokens, int window, int sinks);
+uint64_t chunk_workspace(const KvCache& c, int nh, int tokens, int window, int sinks);
+cudaError_t launch_attend_chunk(AttendArgs a, cudaStream_t st);
 cudaError_t launch_attend_prompt(const AttendArgs& a, cudaStream_t st);
 
 struct EvictArgs {

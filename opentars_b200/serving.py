@@ -52,7 +52,9 @@ SERVE_SIGNATURES = {
     "tc_attend": (ctypes.c_int, [_C, P, I64, I64, P, I64, I64, I32, ctypes.c_float, I32, I32, P, P, ctypes.c_uint64,
                                  P]),
     "tc_attend_workspace": (ctypes.c_uint64, [_C, I32, I32]),
-    "tc_attend_prompt": (ctypes.c_int, [_C, P, I64, I64, P, I64, I64, I32, P, I32, ctypes.c_float, I32, I32, P]),
+    "tc_attend_prompt": (ctypes.c_int, [_C, P, I64, I64, P, I64, I64, I32, P, I32, ctypes.c_float, I32, I32, P,
+                                        ctypes.c_uint64, P]),
+    "tc_attend_prompt_workspace": (ctypes.c_uint64, [_C, I32, I32, I32, I32]),
     "tc_kv_evict": (ctypes.c_int, [_C, I32, I32, I32, P, P, P, P, ctypes.c_uint64, P]),
     "tc_kv_evict_workspace": (ctypes.c_uint64, [_C, I32]),
     "tc_adjust_logits": (ctypes.c_int, [_R, P]),
@@ -169,12 +171,18 @@ class PagedCache:
         self.index = k.device.index
         self._sizes: dict = {}                                    # workspace bytes by what asks for them
 
-    def workspace(self, fn, *args) -> torch.Tensor:
-        """A workspace of its own for one call, from torch's allocator on the current stream."""
+    def workspace(self, fn, *args) -> tuple:
+        """A workspace of its own for one call, from torch's allocator on the current stream: the tensor, its
+        address and its size."""
         n = self._sizes.get((fn.__name__, args))
         if n is None:
+            if len(self._sizes) >= 1024:
+                self._sizes.clear()
             n = self._sizes[fn.__name__, args] = fn(self.ref, *args)
-        return torch.empty(n, dtype=torch.uint8, device=self.device)
+        if n == 0:
+            return None, None, 0
+        t = torch.empty(n, dtype=torch.uint8, device=self.device)
+        return t, t.data_ptr(), n
 
     k = property(lambda self: self._t[0])
     v = property(lambda self: self._t[1])
@@ -254,8 +262,8 @@ def attend(cache: PagedCache, q: torch.Tensor, scale: float, window: int = 0, si
         raise ValueError(f"{n} query rows for {cache.batch} sequences")
     w = None if weight_out is None else _weight_out(cache, weight_out)
     L = lib()
-    ws = cache.workspace(L.tc_attend_workspace, args[6], int(w is not None))
-    _run(cache.index, "attend", L.tc_attend, cache.ref, *args, scale, window, sinks, w, ws.data_ptr(), ws.numel())
+    ws, ws_p, ws_n = cache.workspace(L.tc_attend_workspace, args[6], int(w is not None))
+    _run(cache.index, "attend", L.tc_attend, cache.ref, *args, scale, window, sinks, w, ws_p, ws_n)
     return out
 
 
@@ -267,7 +275,9 @@ def attend_prompt(cache: PagedCache, q: torch.Tensor, cu: torch.Tensor, scale: f
     n, out, args = _attend_args(cache, q, out, window, sinks)
     cu_p = _cu(cu, cache)
     if n:
-        _run(cache.index, "attend_prompt", lib().tc_attend_prompt, cache.ref, *args, cu_p, n, scale, window, sinks)
+        L = lib()
+        ws, ws_p, ws_n = cache.workspace(L.tc_attend_prompt_workspace, args[6], n, window, sinks)
+        _run(cache.index, "attend_prompt", L.tc_attend_prompt, cache.ref, *args, cu_p, n, scale, window, sinks, ws_p, ws_n)
     return out
 
 
@@ -292,9 +302,9 @@ def evict(cache: PagedCache, budget: int, sinks: int = 0, recent: int = 0, lengt
     _ints(pos_out, cache.pos.shape, cache.device, "pos_out")
     w = _weight_out(cache, cache.weight if weight_out is None else weight_out)
     L = lib()
-    ws = cache.workspace(L.tc_kv_evict_workspace, budget)
+    ws, ws_p, ws_n = cache.workspace(L.tc_kv_evict_workspace, budget)
     _run(cache.index, "evict", L.tc_kv_evict, cache.ref, budget, sinks, recent, length_out.data_ptr(), w,
-         pos_out.data_ptr(), ws.data_ptr(), ws.numel())
+         pos_out.data_ptr(), ws_p, ws_n)
 
 
 def _per_row(t: torch.Tensor | None, dtype: torch.dtype, rows: int, device: torch.device, name: str) -> int | None:

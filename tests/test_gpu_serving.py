@@ -190,6 +190,15 @@ PROMPT = [
     (torch.float16, 64, 16, 1, 33, [(3, 21)], 10, 2, "slots"),
     (torch.bfloat16, 128, 64, 1, 4, [(700, 170)], 2 ** 31 - 1, 2 ** 31 - 1, "heads"),
     (torch.bfloat16, 128, 32, 1, 2, [(2000, 4), (10, 4), (0, 4)], 300, 40, "slots"),
+    # few rows a sequence
+    (torch.bfloat16, 128, 16, 2, 2, [(1000, 4), (3, 4), (0, 0), (0, 1), (64, 7)], 0, 0, "heads"),
+    (torch.float16, 256, 64, 1, 4, [(600, 8), (0, 3)], 512, 4, "heads"),
+    (torch.bfloat16, 64, 16, 3, 1, [(5, 31), (500, 33), (15, 1)], 20, 3, "slots"),
+    (torch.float16, 128, 16, 1, 7, [(100, 2), (0, 5), (333, 1)], 0, 0, "heads"),
+    (torch.bfloat16, 256, 16, 1, 16, [(40, 2)], 1, 0, "heads"),
+    (torch.float16, 64, 256, 1, 20, [(300, 1), (0, 2)], 50, 260, "slots"),
+    (torch.bfloat16, 128, 16, 1, 2, [(9000, 5)], 0, 0, "heads"),
+    (torch.float16, 128, 64, 2, 3, [(1, 1)] * 40 + [(0, 60)], 0, 0, "heads"),
 ]
 
 
@@ -240,35 +249,38 @@ def test_attend_prompt_keeps_later_tokens_out():
     _close(out, ref, _tolerance(ref, q, k, v, 0.09, torch.bfloat16))
 
 
-def test_attend_prompt_rows_at_negative_positions_get_zeros():
+@pytest.mark.parametrize("n", [9, 300])
+def test_attend_prompt_rows_at_negative_positions_get_zeros(n):
     from opentars_b200 import serving as S
     g = torch.Generator().manual_seed(9)
     k, v, table = _pools([5], 1, 64, 16, torch.bfloat16, g)
-    q = torch.randn(9, 1, 64, generator=g).bfloat16()
-    cu = torch.tensor([0, 9], dtype=torch.int32)
+    q = torch.randn(n, 1, 64, generator=g).bfloat16()
+    cu = torch.tensor([0, n], dtype=torch.int32)
     out = S.attend_prompt(_cache(k, v, table, [5]), q.cuda(), cu.cuda(), 0.125)
     _no_error()
-    assert (out[:4] == 0).all() and (out[4:] != 0).any()
+    assert (out[:n - 5] == 0).all() and (out[n - 5:] != 0).any()
     ref = R.attend_prompt(k, v, table, [5], q, cu, 0.125, 0, 0, 16)
     _close(out, ref, _tolerance(ref, q, k, v, 0.125, torch.bfloat16))
 
 
-@pytest.mark.parametrize("op", ["attend", "prompt"])
-def test_bad_pages_and_lengths_are_left_out_and_recorded(op):
+@pytest.mark.parametrize("op,n,room", [("attend", 1, 0), ("prompt", 1, 0), ("prompt", 1, 600), ("prompt", 50, 0)])
+def test_bad_pages_and_lengths_are_left_out_and_recorded(op, n, room):
     """Ids outside the pool inside the used slots, and a length beyond the page list: the kernels check
-    every id against the pool and clamp the length before they read."""
+    every id against the pool and clamp the length before they read. (Room in the page list for many more
+    slots takes a chunk of few rows to the kernel that splits the length.)"""
     from opentars_b200 import serving as S
     g = torch.Generator().manual_seed(10)
     lens, hd, page = [100, 70, 64], 128, 16
     k, v, table = _pools(lens, 2, hd, page, torch.bfloat16, g)
     table[0, 2], table[1, 4], table[1, 0] = -1, k.shape[0], 2 ** 31 - 1
-    q = torch.randn(3, 4, hd, generator=g).bfloat16()
+    table = torch.cat([table, torch.full((3, room), -3, dtype=torch.int32)], 1)
+    q = torch.randn(3 * n, 4, hd, generator=g).bfloat16()
     cache = _cache(k, v, table, lens)
     if op == "attend":
         out, code = S.attend(cache, q.cuda(), 0.09), 52
         ref, _ = R.attend(k, v, table, lens, q, 0.09, 0, 0, page)
     else:
-        cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32)
+        cu = torch.tensor([0, n, 2 * n, 3 * n], dtype=torch.int32)
         out, code = S.attend_prompt(cache, q.cuda(), cu.cuda(), 0.09), 53
         ref = R.attend_prompt(k, v, table, lens, q, cu, 0.09, 0, 0, page)
     torch.cuda.synchronize()
@@ -277,15 +289,16 @@ def test_bad_pages_and_lengths_are_left_out_and_recorded(op):
     table[2, 4] = int(table[2, 3])                             # all pages of sequence 2's list are real now
     cache = _cache(k, v, table[2:, :5].contiguous(), [10 ** 6])
     ref_len = [80]
+    cu = torch.tensor([0, n], dtype=torch.int32)
     if op == "attend":
         out = S.attend(cache, q[2:].cuda(), 0.09, window=16)
+        ref, _ = R.attend(k, v, table[2:, :5], ref_len, q[2:], 0.09, 16, 0, page)
     else:
-        out = S.attend_prompt(cache, q[2:].cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda(), 0.09, window=16)
+        out = S.attend_prompt(cache, q[2 * n:].cuda(), cu.cuda(), 0.09, window=16)
+        ref = R.attend_prompt(k, v, table[2:, :5], ref_len, q[2 * n:], cu, 0.09, 16, 0, page)
     torch.cuda.synchronize()
     assert S.device_error(clear=True) == code
-    if op == "attend":
-        ref, _ = R.attend(k, v, table[2:, :5], ref_len, q[2:], 0.09, 16, 0, page)
-        _close(out, ref, _tolerance(ref, q, k, v, 0.09, torch.bfloat16))
+    _close(out, ref, _tolerance(ref, q, k, v, 0.09, torch.bfloat16))       # (slots 64 .. 79 lie on page 3 again)
 
 
 def test_attend_offsets_past_32_bits():
@@ -307,8 +320,11 @@ def test_attend_offsets_past_32_bits():
     ref, _ = R.attend(ks, vs, small, lens, q, 0.06, 0, 0, page)
     tol = _tolerance(ref, q, ks, vs, 0.06, torch.bfloat16)
     _close(S.attend(cache, q.cuda(), 0.06), ref, tol)
-    cu = torch.tensor([0, 1], dtype=torch.int32).cuda()
-    _close(S.attend_prompt(cache, q.cuda(), cu, 0.06), ref, tol)
+    for n in (1, 40):                                          # few rows, and many
+        rows = torch.randn(n, 2, hd, generator=g).bfloat16()
+        cu = torch.tensor([0, n], dtype=torch.int32)
+        want = R.attend_prompt(ks, vs, small, lens, rows, cu, 0.06, 0, 0, page)
+        _close(S.attend_prompt(cache, rows.cuda(), cu.cuda(), 0.06), want, _tolerance(want, rows, ks, vs, 0.06, torch.bfloat16))
     S.append(cache, torch.ones(1, 1, hd, device="cuda"), torch.full((1, 1, hd), 2.0, device="cuda"))
     _no_error()
     assert (k[n_pages - 30, 43, 0] == 1).all() and (v[n_pages - 30, 43, 0] == 2).all()
@@ -732,8 +748,8 @@ def test_waits_that_run_out_are_recorded():
     lens = [500, 0, 90]
     k, v, table = _pools(lens, 2, 128, 16, torch.bfloat16, g)
     cache = _cache(k, v, table, lens)
-    q = torch.randn(3, 4, 128, generator=g).bfloat16().cuda()
-    cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32).cuda()
+    q = torch.randn(150, 4, 128, generator=g).bfloat16().cuda()
+    cu = torch.tensor([0, 80, 80, 150], dtype=torch.int32).cuda()
     call = lambda: S.attend_prompt(cache, q, cu, 0.09)  # noqa: E731
     want = call().clone()
     _no_error()

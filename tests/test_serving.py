@@ -71,9 +71,10 @@ def test_bad_caches_are_refused(L, bad):
     p = 1 << 20
     assert L.tc_kv_append(c, p, p, 1, 128, 128, None, 1, None) == -2
     assert L.tc_attend(c, p, 256, 128, p, 256, 128, 2, 1.0, 0, 0, None, None, 0, None) == -2
-    assert L.tc_attend_prompt(c, p, 256, 128, p, 256, 128, 2, p, 1, 1.0, 0, 0, None) == -2
+    assert L.tc_attend_prompt(c, p, 256, 128, p, 256, 128, 2, p, 1, 1.0, 0, 0, p, 1 << 30, None) == -2
     assert L.tc_kv_evict(c, 16, 0, 0, p, p, p, p, 1 << 30, None) == -2
     assert L.tc_attend_workspace(c, 2, 1) == 0 and L.tc_kv_evict_workspace(c, 16) == 0
+    assert L.tc_attend_prompt_workspace(c, 2, 1, 0, 0) == 0
 
 
 def test_bad_calls_are_refused(L):
@@ -99,8 +100,14 @@ def test_bad_calls_are_refused(L):
     assert L.tc_attend(ctypes.byref(_cache()), *(ok[k] for k in ok), None) == -2  # weights of a cache without them
     prompt = [(None, p, 1), (p, None, 1), (p, p, -1), (p, p, (1 << 28) + 1)]
     for q, cu, n in prompt:
-        assert L.tc_attend_prompt(c, q, 256, 128, p, 256, 128, 2, cu, n, 1.0, 0, 0, None) == -2, (q, cu, n)
-    assert L.tc_attend_prompt(c, None, 0, 0, None, 0, 0, 2, p, 0, 1.0, 0, 0, None) == 0
+        assert L.tc_attend_prompt(c, q, 256, 128, p, 256, 128, 2, cu, n, 1.0, 0, 0, p, 1 << 30, None) == -2, (q, cu, n)
+    assert L.tc_attend_prompt(c, None, 0, 0, None, 0, 0, 2, p, 0, 1.0, 0, 0, None, 0, None) == 0
+    long = ctypes.byref(_cache(n_pages=1000, max_pages=1000, table_stride=1000))
+    n = L.tc_attend_prompt_workspace(long, 2, 3, 0, 0)
+    assert n > 0 and L.tc_attend_prompt_workspace(long, 2, 5000, 0, 0) == 0    # few rows, many rows
+    assert L.tc_attend_prompt_workspace(long, 2, 3, -1, 0) == 0 and L.tc_attend_prompt_workspace(long, 2, 3, 0, -1) == 0
+    for ws, size in ((None, n), (p + 16, n), (p, n - 1)):
+        assert L.tc_attend_prompt(long, p, 256, 128, p, 256, 128, 2, p, 3, 1.0, 0, 0, ws, size, None) == -2
     n = L.tc_kv_evict_workspace(c, 16)
     assert n > 0
     evict = [(0, 0, 0, p, p, p, p, n), (16, -1, 0, p, p, p, p, n), (16, 0, -1, p, p, p, p, n), (16, 9, 8, p, p, p, p, n),
