@@ -14,6 +14,7 @@
 #include <stdint.h>
 
 #include "tarscuda.h"
+#include "tarscuda_serve.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -77,6 +78,13 @@ int tc_engine_profile(tc_engine* e, float* ms, int32_t* kind, uint64_t* bytes, u
 int tc_engine_reset_seq(tc_engine* e, int32_t b);
 /* Each sequence's position (its next token's index) [batch] into the host. */
 int tc_engine_positions(tc_engine* e, int32_t* pos_host);
+/* Rules on the logits of the last step before its picks are used (tc_adjust_logits, tarscuda_serve.h, in
+ * place on the engine's stream): the history, penalties, biases and mask of r; its logits, out, rows,
+ * vocab, token and strides of the two are the engine's own and not read. Each sequence's pick becomes
+ * the rules' pick: tc_engine_tokens returns it, and a following step without host tokens feeds it.
+ * `none`, the pick where a mask allows nothing, must be a token of the vocabulary when there is a mask.
+ * tc_engine_logits then returns the changed logits. No counterpart in the reference. */
+int tc_engine_adjust(tc_engine* e, const tc_logits_rules* r);
 /* The fused decode step: one-token steps run as one cooperative kernel over every SM (all layers,
  * the final norm and the head; then the greedy pick) when the model and batch fit it (batch <= 64,
  * every K a multiple of 128, head dim 64 / 128 / 256); otherwise, and for chunks of more tokens, as

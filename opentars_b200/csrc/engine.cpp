@@ -16,6 +16,7 @@
 
 #include "../../include/tarscuda.h"
 #include "../../include/tarscuda_engine.h"
+#include "../../include/tarscuda_serve.h"
 #include "engine.h"
 #include "pdl.cuh"
 #include "mma.h"
@@ -677,6 +678,22 @@ int tc_engine_logits(tc_engine* e, float* logits_host) {
 int tc_engine_sync(tc_engine* e) {
   TRY(cudaStreamSynchronize(e->st));
   return TC_OK;
+}
+
+int tc_engine_adjust(tc_engine* e, const tc_logits_rules* r) {
+  if (!e || !r) return TC_ERR_ARG;
+  tc_logits_rules a = *r;
+  a.logits = a.out = e->logits;
+  a.logits_stride = a.out_stride = a.vocab = e->md.vocab;
+  a.rows = e->B;
+  a.token = e->next;
+  if (a.mask && (a.none < 0 || a.none >= e->md.vocab)) {
+    e->err = "none is not a token of the vocabulary";
+    return TC_ERR_ARG;
+  }
+  const int rc = tc_adjust_logits(&a, e->st);
+  if (rc != TC_OK) e->err = rc == TC_ERR_ARG ? "a rule's argument is out of range" : "adjust: launch failed";
+  return rc;
 }
 
 int tc_argmax(const float* logits, int32_t vocab, int32_t rows, int32_t* tok_out, void* stream) {

@@ -61,6 +61,7 @@ ENGINE_SIGNATURES = {
     "tc_engine_fused": (ctypes.c_int, [P, ctypes.c_int32]),
     "tc_engine_fused_why": (ctypes.c_char_p, [P]),
     "tc_engine_fused_diag": (ctypes.c_int, [P, P]),
+    "tc_engine_adjust": (ctypes.c_int, [P, P]),
     "tc_engine_phase_times": (ctypes.c_int, [P, P, ctypes.c_uint32]),
 }
 # the fused step's phases, in the order of tc_engine_phase_times' stamps (per layer, then the tail)
@@ -181,6 +182,23 @@ class DecodeEngine:
         out = np.empty((self.B, self.vocab), F32)
         self._check(lib().tc_engine_logits(self.h, out.ctypes.data_as(ctypes.c_void_p)), "logits")
         return out
+
+    def adjust(self, none: int = 0, **rules) -> None:
+        """Rules on the last step's logits before its picks are used (serving.adjust_logits' keywords
+        history, n_history, n_prompt, repetition, presence, frequency, bias_ids, bias and mask: torch
+        tensors on the engine's device, a row per sequence): logits() and tokens() then return the changed
+        logits and their picks, and step(None) feeds those. A sequence whose mask allows nothing picks
+        `none`. Ordered after the work that torch's current stream holds, and before what it gets next."""
+        import torch
+
+        from .serving import rules_of
+        with torch.cuda.device(self.device):
+            own = torch.cuda.ExternalStream(lib().tc_engine_stream(self.h), device=self.device)
+            now = torch.cuda.current_stream(self.device)
+            own.wait_stream(now)
+            r = rules_of(None, shape=(self.B, self.vocab), device=torch.device("cuda", self.device), none=none, **rules)
+            self._check(lib().tc_engine_adjust(self.h, ctypes.byref(r)), "adjust")
+            now.wait_stream(own)
 
     def sync(self):
         self._check(lib().tc_engine_sync(self.h), "sync")

@@ -324,19 +324,25 @@ def _matrix(t: torch.Tensor, dtype: torch.dtype, rows: int, device: torch.device
     return t.data_ptr(), stride[0] if rows > 1 else shape[1], shape[1]
 
 
-def rules_of(logits: torch.Tensor, out: torch.Tensor | None = None, history: torch.Tensor | None = None,
+def rules_of(logits: torch.Tensor | None, out: torch.Tensor | None = None, history: torch.Tensor | None = None,
              n_history: torch.Tensor | None = None, n_prompt: torch.Tensor | None = None,
              repetition: torch.Tensor | None = None, presence: torch.Tensor | None = None,
              frequency: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
              bias: torch.Tensor | None = None, mask: torch.Tensor | None = None, token: torch.Tensor | None = None,
-             none: int = -1) -> Rules_t:
-    """The checked C description of adjust_logits' arguments."""
-    _need(logits.is_cuda and logits.dim() == 2 and logits.shape[0] >= 1 and logits.shape[1] >= 1,
-          "logits: fp32 [rows, vocab] on a CUDA device")
-    rows, dev = logits.shape[0], logits.device
-    x, x_stride, vocab = _matrix(logits, torch.float32, rows, dev, "logits")
-    y, y_stride, n = (x, x_stride, vocab) if out is None else _matrix(out, torch.float32, rows, dev, "out")
-    _need(n == vocab, "out has the logits' shape")
+             none: int = -1, shape: tuple | None = None, device: torch.device | None = None) -> Rules_t:
+    """The checked C description of adjust_logits' arguments; without logits, of rules on a decode engine's
+    own logits of this shape and device."""
+    if logits is None:
+        (rows, vocab), dev = shape, device
+        x = y = None
+        x_stride = y_stride = vocab
+    else:
+        _need(logits.is_cuda and logits.dim() == 2 and logits.shape[0] >= 1 and logits.shape[1] >= 1,
+              "logits: fp32 [rows, vocab] on a CUDA device")
+        rows, dev = logits.shape[0], logits.device
+        x, x_stride, vocab = _matrix(logits, torch.float32, rows, dev, "logits")
+        y, y_stride, n = (x, x_stride, vocab) if out is None else _matrix(out, torch.float32, rows, dev, "out")
+        _need(n == vocab, "out has the logits' shape")
     h, h_stride, n_h = (None, 0, 0) if history is None else _matrix(history, torch.int32, rows, dev, "history")
     counts = (_per_row(n_history, torch.int32, rows, dev, "n_history"),
               _per_row(n_prompt, torch.int32, rows, dev, "n_prompt"),

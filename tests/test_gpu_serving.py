@@ -762,3 +762,56 @@ def test_waits_that_run_out_are_recorded():
         lib().tc_set_spin_limit(was)
     assert torch.equal(call(), want)
     _no_error()
+
+
+@pytest.mark.parametrize("name", ["qwen3_small", "gemma3_small"])
+def test_the_decode_engine_takes_rules_before_its_picks(name):
+    """DecodeEngine.adjust after every step: the changed logits and picks are the rules' on the step's own
+    logits, and the following step feeds the changed picks (as a second engine that is given them)."""
+    import numpy as np
+
+    from opentars_b200.engine import DecodeEngine
+    from tests import fixtures as FX
+    from tests.model_runs import build_image
+    fx = FX.engine_models()[name]
+    rng = np.random.default_rng(3)
+    B, V = 3, fx["vocab"]
+    prompts = rng.integers(0, V, (B, 4))
+    eng, twin = DecodeEngine(build_image(fx), batch=B), DecodeEngine(build_image(fx), batch=B)
+    for e in (eng, twin):
+        e.reset()
+        e.step(prompts, 4)
+    hist = torch.zeros(B, 16, dtype=torch.int32, device="cuda")
+    hist[:, :4] = torch.from_numpy(prompts).int().cuda()
+    n = torch.full((B,), 4, dtype=torch.int32, device="cuda")
+    first = n.clone()
+    rep, freq = torch.full((B,), 1.7, device="cuda"), torch.full((B,), 0.3, device="cuda")
+    for step in range(4):
+        plain = twin.logits()
+        mask = torch.full((B, (V + 31) // 32), -1, dtype=torch.int32, device="cuda")
+        top = plain.argmax(1)
+        for b in range(B - 1):                                 # the greedy pick of two sequences is forbidden
+            mask[b, top[b] // 32] = ~(1 << int(top[b] % 32)) if top[b] % 32 < 31 else 2 ** 31 - 1
+        mask[B - 1] = 0                                        # and everything for the third
+        eng.adjust(none=7, history=hist, n_history=n, n_prompt=first, repetition=rep, frequency=freq, mask=mask)
+        got, picks = eng.logits(), eng.tokens()
+        for b in range(B):
+            allowed = torch.ones(V, dtype=torch.bool) if b < B - 1 else torch.zeros(V, dtype=torch.bool)
+            allowed[top[b]] = False
+            want, pick = R.adjust(torch.from_numpy(plain[b]), hist[b].cpu(), int(n[b]), 4, float(rep[b]), 0.0, float(freq[b]),
+                                  [], [], allowed)
+            assert np.allclose(got[b], want.numpy(), rtol=1e-6, atol=1e-5)
+            assert picks[b] == (7 if pick is None else int(np.argmax(got[b])))
+        hist[torch.arange(B), n.long()] = torch.from_numpy(picks).cuda()
+        n += 1
+        eng.step(None)
+        twin.step(picks.reshape(B, 1), 1)
+        assert np.array_equal(eng.logits().view(np.uint32), twin.logits().view(np.uint32)), step
+    with pytest.raises(RuntimeError, match="none"):
+        eng.adjust(none=V, mask=mask)
+    with pytest.raises(ValueError):
+        eng.adjust(repetition=rep)
+    with pytest.raises(ValueError):
+        eng.adjust(history=hist[:2], repetition=rep)
+    eng.close()
+    twin.close()
