@@ -95,11 +95,10 @@ cudaError_t append_to(const AppendArgs& a, cudaStream_t st) {
 // (protected slots highest, then a NaN weight, then the weight's bits made monotonic), computed once
 // and kept in shared memory while it fits there. The budget-th largest key is found digit by digit
 // from the top (11, 11 and 10 bits, counted in shared memory), and of the slots with that key as many
-// stay as are needed, from the lowest slot on. Warps own contiguous runs of slots, so the lists of
-// leaving and arriving slots come out in ascending order from ballots and one scan over the warps.
+// stay as are needed, from the lowest slot on. Threads own contiguous runs of slots, so the lists of
+// leaving and arriving slots come out in ascending order from one scan over the threads.
 // A few rows are moved at once (a cache one slot over its budget moves one); more of them in a second
-// kernel over the lists. Bound by the chain of block-wide steps: about 1 us of loads, then three
-// counting passes and two walks of some 0.4 us each for a thousand slots.
+// kernel over the lists. Bound by the chain of block-wide steps; the rows' move by memory.
 constexpr int kRankThreads = 1024, kRankWarps = kRankThreads / 32, kBins = 2048, kKeysMax = 49152, kFewMoves = 32;
 
 __device__ __forceinline__ uint32_t rank_key(float w, int pos, int sinks, int64_t recent_from) {
@@ -122,14 +121,10 @@ __host__ __device__ inline int most_moves(int capacity, int budget) {
   return capacity <= budget ? 0 : (budget < capacity - budget ? budget : capacity - budget);
 }
 
-// Exclusive sums over the warps of the CTA of each warp's (x, y) (the same in a warp's lanes), and the totals.
-__device__ __forceinline__ int2 warps_before(int x, int y, int2* s_warp, int2* all) {
+// Exclusive sums over the threads of the CTA of (x, y), and the totals. s_warp is not reused before a barrier.
+__device__ __forceinline__ int2 threads_before(int x, int y, int2* s_warp, int2* all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncthreads();
-  if (lane == 0) s_warp[warp] = make_int2(x, y);
-  __syncthreads();
-  const int2 mine = s_warp[lane];
-  int2 sum = mine;
+  int2 sum = make_int2(x, y);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xFFFFFFFFu, sum.x, o), v = __shfl_up_sync(0xFFFFFFFFu, sum.y, o);
@@ -138,8 +133,20 @@ __device__ __forceinline__ int2 warps_before(int x, int y, int2* s_warp, int2* a
       sum.y += v;
     }
   }
-  *all = make_int2(__shfl_sync(0xFFFFFFFFu, sum.x, 31), __shfl_sync(0xFFFFFFFFu, sum.y, 31));
-  return make_int2(__shfl_sync(0xFFFFFFFFu, sum.x - mine.x, warp), __shfl_sync(0xFFFFFFFFu, sum.y - mine.y, warp));
+  if (lane == 31) s_warp[warp] = sum;
+  __syncthreads();
+  int2 w = s_warp[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xFFFFFFFFu, w.x, o), v = __shfl_up_sync(0xFFFFFFFFu, w.y, o);
+    if (lane >= o) {
+      w.x += u;
+      w.y += v;
+    }
+  }
+  *all = make_int2(__shfl_sync(0xFFFFFFFFu, w.x, 31), __shfl_sync(0xFFFFFFFFu, w.y, 31));
+  const int bx = __shfl_sync(0xFFFFFFFFu, w.x, (warp + 31) & 31), by = __shfl_sync(0xFFFFFFFFu, w.y, (warp + 31) & 31);
+  return make_int2((warp ? bx : 0) + sum.x - x, (warp ? by : 0) + sum.y - y);
 }
 
 // One 16-byte piece of a moved row, keys and values. Sources lie at or behind the budget, destinations before it.
@@ -154,14 +161,13 @@ __device__ __forceinline__ void move_piece(const KvCache& c, int b, int h, int2 
 
 __global__ void __launch_bounds__(kRankThreads) k_rank(EvictArgs a, Moves mv, int room) {
   const KvCache& c = a.c;
-  extern __shared__ uint32_t s_key[];                            // `room` keys
-  __shared__ int s_hist[kBins];
-  __shared__ int2 s_warp[kRankWarps];
+  extern __shared__ __align__(16) uint32_t s_key[];              // `room` keys, a multiple of four
+  __shared__ int s_hist[2][kBins];
+  __shared__ int2 s_warp[2][kRankWarps];
   __shared__ int2 s_few[kFewMoves];
-  __shared__ int s_digit, s_left, s_count;
+  __shared__ int s_digit[3], s_left[3], s_count;
   griddep_launch();
   const int row = blockIdx.x, b = row / c.n_kv;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int len = kv_length(c, b, kErrEvict);
   const float* w = c.weight + (int64_t)row * c.track;
   const int* pos = c.pos + (int64_t)row * c.track;
@@ -178,6 +184,7 @@ __global__ void __launch_bounds__(kRankThreads) k_rank(EvictArgs a, Moves mv, in
   }
   const int64_t recent_from = (int64_t)__ldg(c.seen + b) - a.recent;
   const bool held = len <= room;
+  for (int i = threadIdx.x; i < kBins; i += kRankThreads) s_hist[0][i] = 0;
   if (held)
 #pragma unroll 4
     for (int i = threadIdx.x; i < len; i += kRankThreads) s_key[i] = rank_key(w[i], pos[i], a.sinks, recent_from);
@@ -188,78 +195,80 @@ __global__ void __launch_bounds__(kRankThreads) k_rank(EvictArgs a, Moves mv, in
   if (copy_p)
 #pragma unroll 4
     for (int i = threadIdx.x; i < a.budget; i += kRankThreads) po[i] = pos[i];
-  auto key = [&](int i) { return held ? s_key[i] : rank_key(w[i], pos[i], a.sinks, recent_from); };
+  __syncthreads();
+  // this thread's run of slots, four at a time: f(slot, key)
+  const int run = ((len + kRankThreads - 1) / kRankThreads + 3) / 4 * 4;
+  const int from = min(len, (int)threadIdx.x * run), to = min(len, from + run);
+  auto each = [&](auto f) {
+    for (int i = from; i < to; i += 4) {
+      uint4 k;
+      if (held) {
+        k = *reinterpret_cast<const uint4*>(s_key + i);
+      } else {
+        auto at = [&](int j) { return j < len ? rank_key(w[j], pos[j], a.sinks, recent_from) : 0; };
+        k = make_uint4(at(i), at(i + 1), at(i + 2), at(i + 3));
+      }
+      f(i, k.x);
+      if (i + 1 < to) f(i + 1, k.y);
+      if (i + 2 < to) f(i + 2, k.z);
+      if (i + 3 < to) f(i + 3, k.w);
+    }
+  };
   uint32_t prefix = 0, known = 0;
   int need = a.budget;                                           // slots still wanted among those with this prefix
+  int2 all = make_int2(0, 0);
 #pragma unroll
   for (int digit = 0; digit < 3; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
     const uint32_t bins = digit < 2 ? 2047u : 1023u;
-    for (int i = threadIdx.x; i < kBins; i += kRankThreads) s_hist[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < len; i += kRankThreads) {
-      const uint32_t k = key(i);
-      if ((k & known) == prefix) atomicAdd(&s_hist[k >> shift & bins], 1);
-    }
+    int* hist = s_hist[digit & 1];
+    each([&](int, uint32_t k) {
+      if ((k & known) == prefix) atomicAdd(&hist[k >> shift & bins], 1);
+    });
+    if (digit < 2)
+      for (int i = threadIdx.x; i < kBins; i += kRankThreads) s_hist[~digit & 1][i] = 0;
     __syncthreads();
     // thread t takes bins 2047 - 2t and the one below: the digit is the bin where the count from the top reaches need
-    const int hi = s_hist[kBins - 1 - 2 * threadIdx.x], lo = s_hist[kBins - 2 - 2 * threadIdx.x];
-    int sum = hi + lo;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-      if (lane >= o) sum += y;
-    }
-    int2 all;
-    const int above = warps_before(__shfl_sync(0xFFFFFFFFu, sum, 31), 0, s_warp, &all).x + sum - hi - lo;
+    const int hi = hist[kBins - 1 - 2 * threadIdx.x], lo = hist[kBins - 2 - 2 * threadIdx.x];
+    const int above = threads_before(hi + lo, 0, s_warp[digit & 1], &all).x;
     if (above < need && above + hi + lo >= need) {
       const bool first = above + hi >= need;
-      s_digit = kBins - 1 - 2 * threadIdx.x - !first;
-      s_left = need - above - (first ? 0 : hi);
-      s_count = first ? hi : lo;
+      s_digit[digit] = kBins - 1 - 2 * threadIdx.x - !first;
+      s_left[digit] = need - above - (first ? 0 : hi);
+      if (digit == 2) s_count = first ? hi : lo;
     }
     __syncthreads();
-    prefix |= (uint32_t)s_digit << shift;
+    prefix |= (uint32_t)s_digit[digit] << shift;
     known |= bins << shift;
-    need = s_left;
+    need = s_left[digit];
   }
   // every slot of a larger key than `prefix` stays, and `need` of the s_count slots with that key, from the lowest on
-  const bool some = need < s_count;
-  const int run = (len + 32 * kRankWarps - 1) / (32 * kRankWarps) * 32;
-  const int from = min(len, warp * run), to = min(len, from + run);
-  const uint32_t below = (1u << lane) - 1;
-  int2 all = make_int2(0, 0);
   int ties0 = 0;
-  if (some) {
+  if (need < s_count) {
     int ties = 0;
-    for (int i = from + lane; i - lane < to; i += 32) ties += __popc(__ballot_sync(0xFFFFFFFFu, i < to && key(i) == prefix));
-    ties0 = warps_before(ties, 0, s_warp, &all).x;
+    each([&](int, uint32_t k) { ties += k == prefix; });
+    ties0 = threads_before(ties, 0, s_warp[1], &all).x;
   }
-  int2 at0 = make_int2(0, 0);
-  for (int pass = 0; pass < 2; ++pass) {
-    int t = ties0, out = at0.x, in = at0.y;
-    for (int i = from + lane; i - lane < to; i += 32) {
-      const bool on = i < to;
-      const uint32_t k = on ? key(i) : 0;
-      const uint32_t tie = __ballot_sync(0xFFFFFFFFu, on && k == prefix);
-      const bool stay = on && (k > prefix || (k == prefix && (!some || t + __popc(tie & below) < need)));
-      t += __popc(tie);
-      const uint32_t leave = __ballot_sync(0xFFFFFFFFu, on && !stay && i < a.budget);
-      const uint32_t move = __ballot_sync(0xFFFFFFFFu, stay && i >= a.budget);
-      if (pass) {
-        int2* at = all.y <= kFewMoves ? s_few : mv.at + (int64_t)row * mv.most;
-        if (leave >> lane & 1) at[out + __popc(leave & below)].y = i;
-        if (move >> lane & 1) at[in + __popc(move & below)].x = i;
-      }
-      out += __popc(leave);
-      in += __popc(move);
-    }
-    if (!pass) at0 = warps_before(out, in, s_warp, &all);
-  }
-  __syncthreads();
+  int t = ties0, out = 0, in = 0;
+  each([&](int i, uint32_t k) {
+    const bool stay = k > prefix || (k == prefix && t++ < need);
+    out += !stay && i < a.budget;
+    in += stay && i >= a.budget;
+  });
+  // (s_warp[0] was last read before the last digit's second barrier)
+  const int2 at0 = threads_before(out, in, s_warp[0], &all);
   const int n = all.y;
   const bool few = n <= kFewMoves;
-  const int2* at = few ? s_few : mv.at + (int64_t)row * mv.most;
+  int2* at = few ? s_few : mv.at + (int64_t)row * mv.most;
+  t = ties0;
+  out = at0.x;
+  in = at0.y;
+  each([&](int i, uint32_t k) {
+    const bool stay = k > prefix || (k == prefix && t++ < need);
+    if (!stay && i < a.budget) at[out++].y = i;
+    if (stay && i >= a.budget) at[in++].x = i;
+  });
+  __syncthreads();
   for (int i = threadIdx.x; i < n; i += kRankThreads) {
     const int2 m = at[i];
     wo[m.y] = w[m.x];
