@@ -815,3 +815,97 @@ def test_the_decode_engine_takes_rules_before_its_picks(name):
         eng.adjust(history=hist[:2], repetition=rep)
     eng.close()
     twin.close()
+
+
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+@pytest.mark.parametrize("n,room", [(2, 700), (130, 0)], ids=["chunk", "tiles"])
+def test_negative_and_zero_scales(scale, n, room):
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(15)
+    lens, hd, page = [200, n], 64, 16
+    k, v, table = _pools(lens, 1, hd, page, torch.float16, g)
+    table = torch.cat([table, torch.full((2, room), -1, dtype=torch.int32)], 1)
+    q = torch.randn(2 * n, 2, hd, generator=g).half()
+    cu = torch.tensor([0, n, 2 * n], dtype=torch.int32)
+    cache = _cache(k, v, table, lens)
+    ref = R.attend_prompt(k, v, table, lens, q, cu, scale, 50, 2, page)
+    _close(S.attend_prompt(cache, q.cuda(), cu.cuda(), scale, window=50, sinks=2), ref,
+           _tolerance(ref, q, k, v, scale, torch.float16))
+    ref, _ = R.attend(k, v, table, lens, q[:2], scale, 50, 2, page)
+    _close(S.attend(cache, q[:2].cuda(), scale, window=50, sinks=2), ref, _tolerance(ref, q, k, v, scale, torch.float16))
+    _no_error()
+
+
+@pytest.mark.parametrize("batch", [65, 300, 700])
+@pytest.mark.parametrize("n,room", [(0, 0), (1, 900), (3, 900), (40, 0)], ids=["attend", "chunk1", "chunk3", "tiles"])
+def test_large_batches(batch, n, room):
+    """More sequences than lanes, than threads of a CTA, and several a thread; some are empty."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(batch + n)
+    hd, page = 64, 16
+    lens = [0 if b % 7 == 3 else max(n, 1) + int(torch.randint(0, 40, (1,), generator=g)) for b in range(batch)]
+    lens[batch // 2] = 500
+    new = [min(n, x) for x in lens]
+    k, v, table = _pools(lens, 1, hd, page, torch.bfloat16, g)
+    table = torch.cat([table, torch.full((batch, room), -1, dtype=torch.int32)], 1)
+    cache = _cache(k, v, table, lens)
+    if n == 0:
+        q = torch.randn(batch, 2, hd, generator=g).bfloat16()
+        ref, _ = R.attend(k, v, table, lens, q, 0.125, 0, 0, page)
+        out = S.attend(cache, q.cuda(), 0.125)
+    else:
+        cu = torch.tensor([0] + new).cumsum(0).int()
+        q = torch.randn(int(cu[-1]), 2, hd, generator=g).bfloat16()
+        ref = R.attend_prompt(k, v, table, lens, q, cu, 0.125, 0, 0, page)
+        out = S.attend_prompt(cache, q.cuda(), cu.cuda(), 0.125)
+    _no_error()
+    _close(out, ref, _tolerance(ref, q, k, v, 0.125, torch.bfloat16))
+
+
+@pytest.mark.parametrize("vocab", [140000, 140001])
+@pytest.mark.parametrize("ids", [3000, 20000], ids=["words16", "words32"])
+def test_adjust_logits_of_many_rows(vocab, ids):
+    """Enough rows for the smaller clusters, a vocabulary of several slices a CTA, and histories on both sides of
+    the 16-bit words' limit with tokens counted thousands of times; every value against 64 bits."""
+    import numpy as np
+
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(ids)
+    rows, nb = 20, 2047
+    x = torch.randn(rows, vocab, generator=g) * 4
+    x[3, 77], x[3, vocab - 3] = NAN, NAN
+    x[4] = -math.inf
+    hist = torch.randint(0, vocab, (rows, ids), generator=g, dtype=torch.int32)
+    hist[:, ::2] = vocab - 1                                   # one token half of the time
+    n = torch.randint(ids // 2, ids + 1, (rows,), generator=g, dtype=torch.int32)
+    first = (n // 3).int()
+    rep, pres, freq = 1 + torch.rand(rows, generator=g), torch.rand(rows, generator=g), torch.rand(rows, generator=g) * 0.01
+    bid = torch.randint(0, vocab, (rows, nb), generator=g, dtype=torch.int32)
+    bid[:, 1::3] = vocab // 2
+    bias = torch.randn(rows, nb, generator=g)
+    words = (vocab + 31) // 32
+    mask = torch.randint(-2 ** 31, 2 ** 31, (words,), generator=g).int()
+    c = lambda t: t.cuda()  # noqa: E731
+    out = torch.empty(rows, vocab, device="cuda")
+    token = S.adjust_logits(c(x), history=c(hist), n_history=c(n), n_prompt=c(first), repetition=c(rep), presence=c(pres),
+                            frequency=c(freq), bias_ids=c(bid), bias=c(bias), mask=c(mask), out=out, none=-9)
+    _no_error()
+    got = out.cpu()
+    t = torch.arange(vocab)
+    allowed = (mask[t // 32] >> (t % 32).int()) & 1 == 1
+    for r in range(rows):
+        want = x[r].double()
+        seen = torch.bincount(hist[r, :int(n[r])].long(), minlength=vocab) > 0
+        made = torch.bincount(hist[r, int(first[r]):int(n[r])].long(), minlength=vocab).double()
+        want = torch.where(seen, torch.where(want > 0, want / rep[r].double(), want * rep[r].double()), want)
+        want = want - freq[r].double() * made - torch.where(made > 0, pres[r].double(), 0.0)
+        last = {int(i): float(b) for i, b in zip(bid[r], bias[r])}
+        want[list(last)] += torch.tensor(list(last.values()), dtype=torch.float64)
+        want[~allowed] = -math.inf
+        fin = torch.isfinite(want)
+        # five roundings of numbers no larger than these
+        size = x[r].abs().double() * 2 + made + 1 + bias[r].abs().max()
+        assert torch.equal(torch.isnan(got[r]), torch.isnan(want)) and (got[r][~fin & ~torch.isnan(want)] == -math.inf).all()
+        assert ((got[r].double() - want).abs()[fin] <= 5 * 2.0 ** -24 * size[fin]).all(), r
+        ok = torch.nonzero(allowed)[:, 0]
+        assert int(token[r]) == int(ok[int(np.argmax(got[r][ok].numpy()))]), r
