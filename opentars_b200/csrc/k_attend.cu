@@ -699,7 +699,8 @@ __global__ void __launch_bounds__(kJoinThreads)
   }
 }
 
-// weight_out = weight + the visible slots' probabilities, summed over the heads that share a key-value head.
+// weight_out = weight + the visible slots' probabilities, summed over the heads that share a key-value head, a
+// slot a thread: the scores of k_attend once more (4 bytes a head and slot) and the final statistics.
 constexpr int kWeightThreads = 256, kWeightHeads = 64;
 __global__ void __launch_bounds__(kWeightThreads) k_weights(const __grid_constant__ AttendArgs a, AttendWs ws) {
   __shared__ float2 s_ml[kWeightHeads];          // a head's maximum, and 1 / its sum

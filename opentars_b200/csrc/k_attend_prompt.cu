@@ -19,6 +19,11 @@
 //              running maximum is only moved (and O rescaled) when it grows by more than 2^8, and
 //              P is rounded to the cache's type, whose range holds 2^8; the row's sum is of the
 //              unrounded fp32 values
+// Three prompts of up to 8192 tokens, 16 heads on 8 of 128, bf16: 365 us (1005 TFLOP/s; 430 us in long runs under
+// the power limit). A pair of tiles takes 3400 cycles for 128 slots, of which its MMAs are 2048: the rest is the
+// way of one tile's scores to its softmax and of its probabilities back (some 1500 cycles besides the work).
+// Parts of 64 slots, which put twice as many tiles' steps in flight, took 432 us: S at N = 64 is bound by the
+// reads of Q from shared memory.
 // A row whose output is not finite, and every row of a CTA that met a page id outside the pool, is
 // computed again by attend_row over its visible slots alone: a NaN or an infinity in a slot that the
 // mask hides from this row but not from its tile reaches it as 0 x inf.
