@@ -311,9 +311,10 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(EvictArgs a, Moves mv) {
 // without a barrier, and the listed tokens, few of many, are changed afterwards, a thread each
 // (divisions and bias reads inside the stream made it three times as long). Each thread keeps its
 // best group of four; the candidates are combined over the cluster and the winning group is read once
-// more for the token. Words of 16 bits for histories below 2^14 ids, so that four CTAs share an SM.
-// Bound by memory, 8 bytes a token and the mask: 64 rows of 262144 with histories of up to 4000 ids, 43 us
-// (3.2 TB/s; the words' filling is the rest); one row of 151936, 10 us (a chain of latencies).
+// more for the token. Words of 16 bits for histories below 2^14 ids: 32768 tokens in 64 KB.
+// Bound by memory, 8 bytes a token and the mask: 64 rows of 262144 with histories of up to 4000 ids, 40 us
+// (3.4 TB/s; the words' filling is the rest); one row of 151936, 9.5 us (a chain of latencies). Tried and not
+// kept: a prefetch of the share to L2 (48 us), eight groups in flight (109 us, with the penalties in the stream).
 template <class Word>
 struct Bits {
   static constexpr uint32_t kListed = 1u << (8 * sizeof(Word) - 1), kPrompt = kListed >> 1, kCount = kPrompt - 1;
@@ -352,12 +353,14 @@ struct Slice {
   }
 };
 
-// VEC: rows of logits and out start on 16-byte boundaries. GROUPS: groups of four tokens a thread has in flight.
-template <bool VEC, class Word, int GROUPS, int THREADS, int CTAS>
-__global__ void __launch_bounds__(THREADS, CTAS)
+// VEC: rows of logits and out start on 16-byte boundaries.
+constexpr int kRuleThreads = 512, kGroups = 4;         // a thread has kGroups groups of four tokens in flight
+constexpr int kSliceBytes = 65536;               // of words
+template <bool VEC, class Word>
+__global__ void __launch_bounds__(kRuleThreads, 2)
     k_adjust(const __grid_constant__ tc_logits_rules a, int cluster, int share, int slice) {
   extern __shared__ uint32_t s_word[];
-  __shared__ Pick s_warp[THREADS / 32];
+  __shared__ Pick s_warp[kRuleThreads / 32];
   __shared__ int s_cand[3], s_listed;
   const int row = blockIdx.x / cluster, rank = (int)cluster_rank(), lane = threadIdx.x & 31;
   const int lo = min(a.vocab, rank * share), hi = min(a.vocab, lo + share);
@@ -389,12 +392,12 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   };
   for (int s0 = lo; s0 < hi; s0 += slice) {
     const int s1 = min(hi, s0 + slice), n = s1 - s0;
-    float e[GROUPS][4];
-    uint32_t bits[GROUPS];
+    float e[kGroups][4];
+    uint32_t bits[kGroups];
     auto request = [&](int j0) {
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        const int j = j0 + 4 * (threadIdx.x + g * THREADS);      // slices begin at multiples of 32: one mask word a group
+      for (int g = 0; g < kGroups; ++g) {
+        const int j = j0 + 4 * (threadIdx.x + g * kRuleThreads);      // slices begin at multiples of 32: one mask word a group
         bits[g] = mask && j < s1 ? __ldg(mask + (j >> 5)) : ~0u;
         if (VEC && j + 4 <= s1) {
           const float4 f = *reinterpret_cast<const float4*>(x + j);
@@ -411,33 +414,33 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     int biased = 0;
     if (any) {
       const int words = (n * (int)sizeof(Word) + 15) / 16;       // (a slice's words are a multiple of 16 bytes)
-      for (int i = threadIdx.x; i < words; i += THREADS) reinterpret_cast<uint4*>(s_word)[i] = make_uint4(0, 0, 0, 0);
+      for (int i = threadIdx.x; i < words; i += kRuleThreads) reinterpret_cast<uint4*>(s_word)[i] = make_uint4(0, 0, 0, 0);
       if (threadIdx.x == 0) s_listed = 0;
       __syncthreads();
       if (ids) {
         // the listed tokens come first on the list; each one's last entry is found by its place there, which
         // its word holds meanwhile
-        for (int i = threadIdx.x; i < a.n_bias; i += THREADS) sl.mark(__ldg(ids + i), Bits<Word>::kListed, false);
+        for (int i = threadIdx.x; i < a.n_bias; i += kRuleThreads) sl.mark(__ldg(ids + i), Bits<Word>::kListed, false);
         __syncthreads();
         biased = s_listed;
-        for (int i = threadIdx.x; i < biased; i += THREADS) {
+        for (int i = threadIdx.x; i < biased; i += kRuleThreads) {
           sl.set(sl.list[i], i);
           last[i] = 0;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < a.n_bias; i += THREADS) {
+        for (int i = threadIdx.x; i < a.n_bias; i += kRuleThreads) {
           const unsigned t = (unsigned)__ldg(ids + i) - (unsigned)s0;
           if (t < (unsigned)n) atomicMax(&last[sl.get(t)], i);
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < biased; i += THREADS) sl.set(sl.list[i], Bits<Word>::kListed);
+        for (int i = threadIdx.x; i < biased; i += kRuleThreads) sl.set(sl.list[i], Bits<Word>::kListed);
         __syncthreads();
       }
       int i0 = 0;
       if (hist4) {
         i0 = n_all & ~3;
 #pragma unroll 2
-        for (int i = 4 * threadIdx.x; i < i0; i += 4 * THREADS) {
+        for (int i = 4 * threadIdx.x; i < i0; i += 4 * kRuleThreads) {
           const int4 t = __ldg(reinterpret_cast<const int4*>(hist + i));
           sl.mark(t.x, Bits<Word>::kPrompt, i >= n_first);
           sl.mark(t.y, Bits<Word>::kPrompt, i + 1 >= n_first);
@@ -446,13 +449,13 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         }
       }
 #pragma unroll 4
-      for (int i = i0 + threadIdx.x; i < n_all; i += THREADS) sl.mark(__ldg(hist + i), Bits<Word>::kPrompt, i >= n_first);
+      for (int i = i0 + threadIdx.x; i < n_all; i += kRuleThreads) sl.mark(__ldg(hist + i), Bits<Word>::kPrompt, i >= n_first);
       __syncthreads();
     }
-    for (int j0 = s0; j0 < s1; j0 += 4 * GROUPS * THREADS) {
+    for (int j0 = s0; j0 < s1; j0 += 4 * kGroups * kRuleThreads) {
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        const int j = j0 + 4 * (threadIdx.x + g * THREADS);
+      for (int g = 0; g < kGroups; ++g) {
+        const int j = j0 + 4 * (threadIdx.x + g * kRuleThreads);
         if (j < s1) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) e[g][u] = bits[g] >> ((j & 31) + u) & 1 ? e[g][u] : none;
@@ -478,12 +481,12 @@ __global__ void __launch_bounds__(THREADS, CTAS)
           consider(max_nan(max_nan(e[g][0], e[g][1]), max_nan(e[g][2], e[g][3])), j);
         }
       }
-      request(j0 + 4 * GROUPS * THREADS);
+      request(j0 + 4 * kGroups * kRuleThreads);
     }
     if (any) {
       __syncthreads();                           // the slice is stored
       const int listed = s_listed;
-      for (int i = threadIdx.x; i < listed; i += THREADS) {
+      for (int i = threadIdx.x; i < listed; i += kRuleThreads) {
         const int t = sl.list[i], j = s0 + t;
         const float was = *(volatile const float*)(y + j);
         const uint32_t word = mask ? __ldg(mask + (j >> 5)) : ~0u;
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   if (lane == 0) s_warp[threadIdx.x >> 5] = m;
   __syncthreads();
   if (threadIdx.x < 32) {
-    Pick t = threadIdx.x < THREADS / 32 ? s_warp[threadIdx.x] : Pick{0.0f, -1, 0};
+    Pick t = threadIdx.x < kRuleThreads / 32 ? s_warp[threadIdx.x] : Pick{0.0f, -1, 0};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t = pick_comb(t, pick_shfl(t, o));
     if (threadIdx.x == 0) {
@@ -569,11 +572,16 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t st) {
 }
 
 namespace {
-template <bool VEC, class Word, int GROUPS, int THREADS, int CTAS>
-cudaError_t adjust(const tc_logits_rules& r, int cluster, int slice_bytes, cudaStream_t st) {
-  constexpr auto kern = k_adjust<VEC, Word, GROUPS, THREADS, CTAS>;
+template <bool VEC, class Word>
+cudaError_t adjust_of(const tc_logits_rules& r, cudaStream_t st) {
+  constexpr auto kern = k_adjust<VEC, Word>;
+  // As many CTAs a row as fit on the SMs at once, two to an SM, with 4096 tokens or more each. Measured on rows of
+  // 151936 (us for clusters of 16, 8, 4, 2): 1 row 9.5, 11.8, 17.3; 16 rows 20, 15, 18; 64 rows 59, 34, 28, 35;
+  // 128 rows 113, 63, 53, 45; 128 rows of 32000 90, 42, 24, 15.
+  int cluster = r.rows <= 4 ? 16 : 8;
+  while (cluster > 1 && ((int64_t)r.rows * cluster > 2 * 148 || r.vocab < 4096 * cluster)) cluster /= 2;
   const int share = ((r.vocab + cluster - 1) / cluster + 31) / 32 * 32;
-  const int slice = std::min(share, slice_bytes / (int)sizeof(Word));
+  const int slice = std::min(share, kSliceBytes / (int)sizeof(Word));
   // a word a token, a place a bias entry, and list entries for as many tokens as the history and the biases can name
   const int n_bias = r.bias ? r.n_bias : 0;
   const int64_t names = (r.history ? r.max_history : 0) + (int64_t)n_bias;
@@ -584,18 +592,13 @@ cudaError_t adjust(const tc_logits_rules& r, int cluster, int slice_bytes, cudaS
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !(ready.load() >> dev & 1)) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * slice_bytes + 8192);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kSliceBytes + 8192);
     if (e != cudaSuccess) return e;
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   tc_logits_rules a = r;
   a.n_bias = n_bias;
-  return launch_ex(kern, dim3((unsigned)r.rows * cluster), dim3(THREADS), smem, st, cluster, a, cluster, share, slice);
-}
-template <bool VEC, class Word>
-cudaError_t adjust_of(const tc_logits_rules& r, cudaStream_t st) {
-  // few rows: 16 CTAs of 1024 threads a row; many: 8 CTAs of 256, four to an SM
-  return r.rows * 8 <= 148 ? adjust<VEC, Word, 4, 1024, 1>(r, 16, 65536, st) : adjust<VEC, Word, 4, 256, 4>(r, 8, 32768, st);
+  return launch_ex(kern, dim3((unsigned)r.rows * cluster), dim3(kRuleThreads), smem, st, cluster, a, cluster, share, slice);
 }
 }  // namespace
 

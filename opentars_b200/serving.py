@@ -380,7 +380,7 @@ def adjust_logits(logits: torch.Tensor, token: torch.Tensor | None = None, none:
     int32 words, bit t % 32 of word t // 32 set where token t is allowed. A row whose mask allows
     nothing picks `none`."""
     if token is None:
-        token = torch.empty(logits.shape[:1], dtype=torch.int32, device=logits.device)
+        token = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
     r = rules_of(logits, token=token, none=none, **rules)
     _run(logits.device.index, "adjust_logits", lib().tc_adjust_logits, ctypes.byref(r))
     return token
