@@ -909,3 +909,38 @@ def test_adjust_logits_of_many_rows(vocab, ids):
         assert ((got[r].double() - want).abs()[fin] <= 5 * 2.0 ** -24 * size[fin]).all(), r
         ok = torch.nonzero(allowed)[:, 0]
         assert int(token[r]) == int(ok[int(np.argmax(got[r][ok].numpy()))]), r
+
+
+@pytest.mark.parametrize("n", [1, 70], ids=["rows", "tiles"])
+def test_heads_first_rows_and_empty_batches(n):
+    """q and out in memory as [heads, rows, dim]; a batch of empty sequences; calls of no rows."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(16)
+    lens, hd, page = [90, 0, 75], 128, 16
+    k, v, table = _pools(lens, 2, hd, page, torch.bfloat16, g)
+    cache = _cache(k, v, table, lens)
+    new = [n, 0, n]
+    cu = torch.tensor([0] + new).cumsum(0).int()
+    store = torch.randn(4, 2 * n, hd, generator=g).bfloat16()
+    q = store.permute(1, 0, 2)
+    ref = R.attend_prompt(k, v, table, lens, q, cu, 0.09, 0, 0, page)
+    out = torch.zeros(4, 2 * n, hd, dtype=torch.bfloat16, device="cuda")
+    S.attend_prompt(cache, store.cuda().permute(1, 0, 2), cu.cuda(), 0.09, out=out.permute(1, 0, 2))
+    _close(out.permute(1, 0, 2), ref, _tolerance(ref, q, k, v, 0.09, torch.bfloat16))
+    rows = torch.randn(4, 3, hd, generator=g).bfloat16()
+    ref, _ = R.attend(k, v, table, lens, rows.permute(1, 0, 2), 0.09, 0, 0, page)
+    one = torch.ones(4, 3, hd, dtype=torch.bfloat16, device="cuda")
+    S.attend(cache, rows.cuda().permute(1, 0, 2), 0.09, out=one.permute(1, 0, 2))
+    _close(one.permute(1, 0, 2), ref, _tolerance(ref, rows, k, v, 0.09, torch.bfloat16))
+    empty = S.PagedCache.empty(2, 16, 2, hd, 3, 2, track=True)
+    q0 = torch.randn(3, 4, hd, device="cuda").bfloat16()
+    assert (S.attend(empty, q0, 0.09, weight_out=empty.weight) == 0).all() and (empty.weight == 0).all()
+    none = torch.zeros(4, dtype=torch.int32, device="cuda")
+    assert S.attend_prompt(empty, q0[:0], none, 0.09).shape == (0, 4, hd)
+    keep = torch.full_like(q0, 5.0)
+    S.attend_prompt(empty, q0, none, 0.09, out=keep)             # no sequence owns a row
+    S.append(empty, q0[:, :2], q0[:, :2], none)
+    S.append(empty, q0[:, :2], q0[:, :2])                       # lengths of zero: every row is skipped
+    S.evict(empty, 4)
+    _no_error()
+    assert (keep == 5.0).all() and (empty.length == 0).all() and (empty.pos == 0).all()
