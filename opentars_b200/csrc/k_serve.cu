@@ -384,9 +384,10 @@ __global__ void __launch_bounds__(kRuleThreads, 2)
   const float none = __int_as_float(0xFF800000);
   float best = none;                             // the best group's value and first token (-1: all -infinity so far)
   int best_at = -1;
-  // of two groups of one value the first counts (a thread meets its groups out of order)
+  // of two groups of one value, or of two with a NaN, the first counts (a thread meets its groups out of order)
   auto consider = [&](float v, int j) {
-    const bool take = best == best && (!(v <= best) || (v == best && best_at >= 0 && j < best_at));
+    const bool take = is_nan(v) ? !is_nan(best) || j < best_at
+                                : !is_nan(best) && (v > best || (v == best && best_at >= 0 && j < best_at));
     best = take ? v : best;
     best_at = take ? j : best_at;
   };

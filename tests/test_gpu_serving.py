@@ -944,3 +944,27 @@ def test_heads_first_rows_and_empty_batches(n):
     S.evict(empty, 4)
     _no_error()
     assert (keep == 5.0).all() and (empty.length == 0).all() and (empty.pos == 0).all()
+
+
+@pytest.mark.parametrize("vocab,second", [(5000, 2050), (5000, 3000), (151936, 9000), (151936, 140000)])
+@pytest.mark.parametrize("how", ["history", "bias"])
+def test_adjust_logits_picks_the_first_of_several_nan(vocab, second, how):
+    """NaN at two or more tokens, of which the earlier, the later, both or none are listed (a listed token meets a
+    thread after the stream of its slice, in any order): the pick is the lowest one, every time."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(vocab + second)
+    at = [[5, second], [5, second], [5, second], [5, second], [4, 5, 6, 7, 8, 9, second], [second, 700, 1999, 31, 32]]
+    listed = [[5], [second], [5, second], [], [9, 8, 7, 6, second], [second, 1999, 700, 31]]
+    x = torch.randn(len(at), vocab, generator=g)
+    ids = torch.full((len(at), 40), -1, dtype=torch.int32)
+    for r in range(len(at)):
+        x[r, at[r]] = NAN
+        ids[r, torch.randperm(40, generator=g)[:len(listed[r])]] = torch.tensor(listed[r], dtype=torch.int32)
+    rules = dict(history=ids.cuda(), presence=torch.full((len(at),), 0.5).cuda()) if how == "history" else \
+        dict(bias_ids=ids.cuda(), bias=torch.ones(len(at), 40).cuda())
+    for _ in range(5):
+        out = torch.empty_like(x, device="cuda")
+        token = S.adjust_logits(x.cuda(), out=out, **rules)
+        assert token.tolist() == [min(a) for a in at]
+        assert torch.equal(torch.isnan(out.cpu()), torch.isnan(x))
+    _no_error()
