@@ -32,7 +32,8 @@ extern "C" {
 /* A paged key-value cache of `batch` sequences. Slot s of sequence b is row s % page_size of page
  * table[b * table_stride + s / page_size] of both pools; key-value head h of a row is `head_dim`
  * contiguous elements at page * page_stride + row * slot_stride + h * head_stride (elements; bases
- * and strides 16-byte aligned). length[b] slots are in use. Entries of the page list behind the
+ * and strides 16-byte aligned, the three dimensions nested in any order so that no two rows share
+ * memory; the stride of a dimension of one entry is not used). length[b] slots are in use. Entries of the page list behind the
  * used slots, and rows of a page behind them, are never read. */
 typedef struct {
   void* k;

@@ -788,7 +788,7 @@ bool make_map_pool(CUtensorMap* m, const KvCache& c, const void* pool, int rows)
   auto fn = encode_fn();
   if (!fn) return false;
   // a dimension of one entry is never stepped over: any legal stride serves
-  auto stride = [&](int64_t s, int n) { return (cuuint64_t)(n > 1 && s > 0 ? 2 * s : 2 * (int64_t)c.hd); };
+  auto stride = [&](int64_t s, int n) { return (cuuint64_t)(n > 1 ? 2 * s : 2 * (int64_t)c.hd); };
   const cuuint64_t dims[4] = {(cuuint64_t)c.hd, (cuuint64_t)1 << c.shift, (cuuint64_t)c.n_kv, (cuuint64_t)c.n_pages};
   const cuuint64_t strides[3] = {stride(c.ss, 1 << c.shift), stride(c.sh, c.n_kv), stride(c.sp, c.n_pages)};
   const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, estr[4] = {1, 1, 1, 1};

@@ -18,6 +18,25 @@ bool al16(const void* p) { return (uintptr_t)p % 16 == 0; }
 // A stride in elements of `bytes` each that keeps rows 16-byte aligned.
 bool stride_ok(int64_t s, int bytes) { return s >= 0 && s < kMaxStride && s * bytes % 16 == 0; }
 
+// Whether a pool's rows of head_dim elements lie apart, its dimensions nested in any order (a stride of 0 or
+// one that steps into the next row has rows share memory; a dimension of one entry is never stepped over).
+bool pool_apart(const tc_kv_cache* c) {
+  int64_t stride[3] = {c->page_stride, c->slot_stride, c->head_stride}, n[3] = {c->n_pages, c->page_size, c->n_kv};
+  int64_t width = c->head_dim;                   // elements from the first to behind the last of the dimensions so far
+  for (int left = 3; left > 0; --left) {
+    int at = 0;
+    for (int i = 1; i < left; ++i)
+      if (stride[i] < stride[at]) at = i;
+    if (n[at] > 1) {
+      if (stride[at] < width) return false;
+      width = std::min(kMaxStride, stride[at] > kMaxStride / n[at] ? kMaxStride : (n[at] - 1) * stride[at] + width);
+    }
+    stride[at] = stride[left - 1];
+    n[at] = n[left - 1];
+  }
+  return true;
+}
+
 // Everything of a cache that the host can check.
 bool take_cache(const tc_kv_cache* c, KvCache* o) {
   if (!c || !c->k || !c->v || !c->table || !c->length) return false;
@@ -30,6 +49,7 @@ bool take_cache(const tc_kv_cache* c, KvCache* o) {
   if (c->max_pages < 1 || c->max_pages > (INT_MAX >> 1 >> shift) || c->table_stride < c->max_pages) return false;
   if (!al16(c->k) || !al16(c->v)) return false;
   if (!stride_ok(c->page_stride, 2) || !stride_ok(c->slot_stride, 2) || !stride_ok(c->head_stride, 2)) return false;
+  if (!pool_apart(c)) return false;
   const bool any = c->weight || c->pos || c->seen, all = c->weight && c->pos && c->seen;
   if (any && (!all || c->track_stride < (int64_t)c->max_pages << shift)) return false;
   o->k = static_cast<uint8_t*>(c->k);

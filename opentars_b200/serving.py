@@ -108,12 +108,13 @@ def _stride(t: torch.Tensor, d: int) -> int:
 
 
 def _apart(t: torch.Tensor) -> bool:
-    """Whether the rows of t [rows, heads, dim] lie apart in memory, in either order."""
-    width = t.shape[2]
-    for stride, n in sorted((t.stride(d), t.shape[d]) for d in (0, 1) if t.shape[d] > 1):
+    """Whether the rows of t [.., dim] lie apart in memory, its other dimensions nested in any order."""
+    last = t.dim() - 1
+    width = t.shape[last]
+    for stride, n in sorted((t.stride(d), t.shape[d]) for d in range(last) if t.shape[d] > 1):
         if stride < width:
             return False
-        width = stride * n
+        width += stride * (n - 1)
     return True
 
 
@@ -121,8 +122,8 @@ class PagedCache:
     """Pools, page lists and lengths of `batch` sequences: a handle over the caller's tensors.
 
     k, v      [n_pages, page_size, n_kv, head_dim] bf16 or fp16, the last dimension contiguous, equal
-              strides (a permuted view of another order is fine; [page, kv head, slot, dim] in memory
-              reads fastest)
+              strides, no two rows sharing memory (a permuted view of another order is fine; [page,
+              kv head, slot, dim] in memory reads fastest)
     table     [batch, max_pages] int32 page ids; entries behind a sequence's length are not read
     length    [batch] int32 slots in use
     weight, pos, seen   what eviction needs, all or none: [batch, n_kv, slots] fp32 attention weight and
@@ -137,6 +138,7 @@ class PagedCache:
         _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype and
               k.device == v.device, "k and v: two pools of one shape, type and stride")
         _need(k.dtype in (torch.bfloat16, torch.float16), f"the pools are bf16 or fp16, not {k.dtype}")
+        _need(_apart(k), "the pools' rows must lie apart (an expanded dimension shares them)")
         _need(k.is_cuda, "the pools must be on a CUDA device")
         n_pages, page, n_kv, hd = k.shape
         _need(page in PAGE_SIZES, f"page size {page}: one of {PAGE_SIZES}")

@@ -151,3 +151,36 @@ def test_the_wrappers_refuse_tensors_they_cannot_take():
     t = torch.zeros(3, 4, 64)
     assert S._apart(t) and S._apart(t.permute(1, 0, 2)) and S._apart(t[:, :1]) and S._apart(t[:1])
     assert not S._apart(t[:1].expand(3, 4, 64)) and not S._apart(torch.zeros(300)[:].as_strided((2, 2, 64), (64, 64, 1)))
+
+
+def test_pools_whose_rows_share_memory_are_refused(L):
+    """A stride of 0 over several entries (a pool expanded over its heads), and strides that step into the next
+    row: refused by every call and by the handle; any nesting of the dimensions is taken."""
+    import torch
+
+    from opentars_b200 import serving as S
+    p = 1 << 20
+    ok = dict(n_kv=2, n_pages=8, page_size=64, page_stride=2 * 64 * 128, head_stride=64 * 128, slot_stride=128)
+    for bad in (dict(head_stride=0), dict(slot_stride=0), dict(page_stride=0), dict(slot_stride=64), dict(head_stride=128),
+                dict(page_stride=64 * 128), dict(head_stride=63 * 128), dict(slot_stride=256), dict(page_stride=128),
+                dict(n_pages=2 ** 31 - 1, page_stride=1 << 39, head_stride=(1 << 39) + 128)):
+        c = ctypes.byref(_cache(**dict(ok, **bad), **TRACK, max_pages=1, table_stride=1))
+        assert L.tc_kv_append(c, p, p, 1, 256, 128, None, 1, None) == -2, bad
+        assert L.tc_attend(c, p, 256, 128, p, 256, 128, 2, 1.0, 0, 0, None, p, 1 << 30, None) == -2, bad
+        assert L.tc_attend_prompt(c, p, 256, 128, p, 256, 128, 2, p, 1, 1.0, 0, 0, p, 1 << 30, None) == -2, bad
+        assert L.tc_kv_evict(c, 16, 0, 0, p, p, p, p, 1 << 30, None) == -2, bad
+        assert L.tc_attend_workspace(c, 2, 0) == 0, bad
+    for good in (dict(), dict(slot_stride=256, head_stride=128), dict(slot_stride=256, head_stride=64 * 256, page_stride=2 * 64 * 256),
+                 dict(page_stride=128, slot_stride=8 * 128, head_stride=8 * 64 * 128), dict(n_kv=1, head_stride=0),
+                 dict(n_pages=1, page_stride=0), dict(page_stride=(64 * 2 - 1) * 128 + 136)):
+        c = ctypes.byref(_cache(**dict(ok, **good), max_pages=1, table_stride=1))
+        assert L.tc_attend_workspace(c, 2, 0) > 0, good
+    pool = torch.zeros(4, 64, 2, 128, dtype=torch.bfloat16)
+    table, length = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for bad in (pool[:, :, :1].expand(4, 64, 2, 128), pool[:1].expand(4, 64, 2, 128), pool[:, :1].expand(4, 64, 2, 128),
+                pool.as_strided((4, 64, 2, 128), (16384, 256, 64, 1))):
+        with pytest.raises(ValueError, match="apart"):
+            S.PagedCache(bad, bad, table, length)
+    for good in (pool, pool.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3), pool[:, :, :1], pool[:1]):
+        with pytest.raises(ValueError, match="CUDA"):           # everything else about it is right
+            S.PagedCache(good, good, table, length)
