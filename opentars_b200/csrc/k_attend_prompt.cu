@@ -102,19 +102,25 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
   return m;
 }
-// 2^x of two values <= 9 on the FMA units: x = n + f with n the nearest integer (added to 1.5 x 2^23, n stands in
-// the sum's low bits) and f in [-1/2, 1/2]; 2^f by a polynomial fitted to least relative error (2.6e-6), n added
-// to its exponent. Below 2^-126 the result is 2^-126; a NaN stays one.
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 2^x of two values <= 9 on the FMA units: x = n + f with n the nearest integer (1.5 x 2^23 + 127 is added, so that
+// n + 127, the exponent field of 2^n, stands in the sum's low bits) and f in [-1/2, 1/2]; 2^f by a polynomial fitted
+// to least relative error (2.6e-6), times 2^n. Below 2^-126 the result is 2^-126. A NaN stays one (its bits make a
+// factor of -infinity, and NaN x -infinity is NaN).
 __device__ __forceinline__ uint64_t ex2_fma(uint64_t x2) {
   const float2 x = halves(x2);
   x2 = pair(__float_as_uint(max_nan(x.x, -126.0f)), __float_as_uint(max_nan(x.y, -126.0f)));
-  const uint64_t t = add2(x2, pair(12582912.0f)), f = add2(x2, fma2(t, pair(-1.0f), pair(12582912.0f)));
+  const uint64_t t = add2(x2, pair(12583039.0f)), f = add2(x2, fma2(t, pair(-1.0f), pair(12583039.0f)));
   uint64_t p = fma2(f, pair(0.009570101276040077f), pair(0.05591785907745361f));
   p = fma2(p, f, pair(0.240247443318367f));
   p = fma2(p, f, pair(0.6931217908859253f));
   p = fma2(p, f, pair(0.9999992847442627f));
-  const float2 n = halves(t), y = halves(p);
-  return pair(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23), __float_as_uint(y.y) + (__float_as_uint(n.y) << 23));
+  const float2 n = halves(t);
+  return mul2(p, pair(__float_as_uint(n.x) << 23, __float_as_uint(n.y) << 23));
 }
 // v[i] = 2^(v[i] scale - base) for N scores, rounded to T two by two into out; their sum (of the unrounded values).
 // MIX: every fourth pair goes to the FMA units, which are idle while the others wait for the special function
@@ -573,7 +579,8 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   tc_fence_after();
   if (!s_dead) {
     const bool any = p >= 0;
-    const float inv = any ? 1.0f / l : 0.0f;
+    // a row whose scores are all -infinity is 0 / 0; its sum is not 0, because ex2_fma ends at 2^-126
+    const float inv = !any ? 0.0f : m == neg_inf() ? __int_as_float(0x7FC00000) : 1.0f / l;
     bool good = true;
     // the warp's rows go out through the query tile's place (no tensor core reads it any more), so
     // that consecutive lanes store consecutive pieces of a row

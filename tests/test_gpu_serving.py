@@ -968,3 +968,29 @@ def test_adjust_logits_picks_the_first_of_several_nan(vocab, second, how):
         assert token.tolist() == [min(a) for a in at]
         assert torch.equal(torch.isnan(out.cpu()), torch.isnan(x))
     _no_error()
+
+
+@pytest.mark.parametrize("dtype,hd,page", [(torch.bfloat16, 128, 64), (torch.bfloat16, 128, 16), (torch.bfloat16, 64, 128),
+                                           (torch.bfloat16, 256, 64), (torch.float16, 128, 64), (torch.float16, 256, 16)])
+@pytest.mark.parametrize("n,room", [(300, 0), (3, 700)], ids=["tiles", "chunk"])
+def test_attend_prompt_rows_whose_scores_are_all_minus_infinity(dtype, hd, page, n, room):
+    """Keys with an infinity against queries of one sign: rows that see nothing but scores of -infinity are NaN as
+    the formula's 0 / 0 is, rows with a score of +infinity as well, and rows that see one finite score are its."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(21)
+    L, far = 400, 390
+    k, v, table = _pools([L], 1, hd, page, dtype, g)
+    for s in range(far):
+        k[int(table[0, s // page]), s % page, 0, 0] = -math.inf
+    q = torch.randn(n, 3, hd, generator=g).to(dtype)
+    q[:, 0, 0], q[:, 1, 0] = 1.0, -1.0
+    q[:, 2, 0] = q[:, 2, 0].abs() + 0.5
+    table = torch.cat([table, torch.full((1, room), -1, dtype=torch.int32)], 1)
+    for length in (far, L):
+        cu = torch.tensor([0, n], dtype=torch.int32)
+        ref = R.attend_prompt(k, v, table, [length], q, cu, 0.1, 0, 0, page)
+        out = S.attend_prompt(_cache(k, v, table, [length]), q.cuda(), cu.cuda(), 0.1)
+        _no_error()
+        _close(out, ref, _tolerance(ref, q, k, v, 0.1, dtype))
+        assert torch.isnan(ref[:, 1]).all() and torch.isnan(ref[:n - (L - far), 0]).all()
+    assert n == 3 or torch.isfinite(ref[n - (L - far):, 0]).all()
