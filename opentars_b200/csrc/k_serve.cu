@@ -384,12 +384,19 @@ __global__ void __launch_bounds__(kRuleThreads, 2)
   const float none = __int_as_float(0xFF800000);
   float best = none;                             // the best group's value and first token (-1: all -infinity so far)
   int best_at = -1;
-  // of two groups of one value, or of two with a NaN, the first counts (a thread meets its groups out of order)
+  auto take = [&](float v, int j) {
+    best = v;
+    best_at = j;
+  };
+  // a group of the stream: a thread meets these in ascending order, so that of equal ones the first is held
   auto consider = [&](float v, int j) {
-    const bool take = is_nan(v) ? !is_nan(best) || j < best_at
-                                : !is_nan(best) && (v > best || (v == best && best_at >= 0 && j < best_at));
-    best = take ? v : best;
-    best_at = take ? j : best_at;
+    if (!is_nan(best) && !(v <= best)) take(v, j);
+  };
+  // a listed token's group: of two of one value, or of two with a NaN, the first counts
+  auto consider_any = [&](float v, int j) {
+    if (is_nan(v) ? !is_nan(best) || j < best_at
+                  : !is_nan(best) && (v > best || (v == best && best_at >= 0 && j < best_at)))
+      take(v, j);
   };
   for (int s0 = lo; s0 < hi; s0 += slice) {
     const int s1 = min(hi, s0 + slice), n = s1 - s0;
@@ -495,7 +502,7 @@ __global__ void __launch_bounds__(kRuleThreads, 2)
           float v = penalties<Word>(was, sl.get(t), r);
           if (i < biased) v = __fadd_rn(v, __ldg(bias + last[i]));
           y[j] = v;
-          consider(v, j & ~3);
+          consider_any(v, j & ~3);
         }
       }
       __syncthreads();
