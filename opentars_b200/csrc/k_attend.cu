@@ -564,7 +564,8 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
           if (all) {
             const float inv = met ? 1.0f / sum : 0.0f;
             v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
-            good &= fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < __int_as_float(0x7F800000);
+            // (a sum that is NaN makes a NaN of every output, as the formula does)
+            good &= sum != sum || fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < __int_as_float(0x7F800000);
             const int tok = ONE ? 0 : h / heads;
             *reinterpret_cast<uint2*>(a.out + 2 * ((int64_t)(row0 + tok) * a.orow + (int64_t)(h0 + h - tok * heads) * a.oh +
                                                    col)) = make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
@@ -588,8 +589,9 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
 
 // The items whose tiles lie in several CTAs' runs: their states at the common maximum. One CTA per
 // (block, head block, row): its warps take the pieces in turn, and their sums are added in warp
-// order. Blocks that see no slot get zeros. A row with a NaN or an infinity is computed again key by
-// key: the second half of a split probability times an infinite value would make a NaN of it.
+// order. Blocks that see no slot get zeros. A row with a NaN or an infinity and a sum that is a
+// number is computed again key by key: the second half of a split probability times an infinite value would
+// make a NaN of it.
 constexpr int kJoinWarps = 8, kJoinThreads = 32 * kJoinWarps;
 template <class T, int HD, bool ONE>
 __global__ void __launch_bounds__(kJoinThreads)
@@ -685,7 +687,7 @@ __global__ void __launch_bounds__(kJoinThreads)
       }
       v.x *= inv;
       v.y *= inv;
-      good = fabsf(v.x) + fabsf(v.y) < __int_as_float(0x7F800000);
+      good = l != l || fabsf(v.x) + fabsf(v.y) < __int_as_float(0x7F800000);
       to[threadIdx.x] = Elem<T>::pack(v.x, v.y);
     }
     if (ws.ml && threadIdx.x == 0) ws.ml[(int64_t)q.b * a.nh + h] = make_float2(m, l);

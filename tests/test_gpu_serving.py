@@ -994,3 +994,48 @@ def test_attend_prompt_rows_whose_scores_are_all_minus_infinity(dtype, hd, page,
         _close(out, ref, _tolerance(ref, q, k, v, 0.1, dtype))
         assert torch.isnan(ref[:, 1]).all() and torch.isnan(ref[:n - (L - far), 0]).all()
     assert n == 3 or torch.isfinite(ref[n - (L - far):, 0]).all()
+
+
+@pytest.mark.parametrize("op,what", [("prompt", "key"), ("prompt", "value"), ("attend", "key"), ("chunk", "key")])
+def test_a_nonfinite_row_that_everyone_sees_costs_no_second_pass(op, what):
+    """A NaN in the first key makes every score's sum, and so every output, a NaN; an infinity in the first value makes
+    infinities of its column: neither sends the rows to the pass over single keys, which takes hundreds of times as
+    long (eight times is the bound, for a busy machine)."""
+    from opentars_b200 import serving as S
+    B, L, kv, nh, hd, page = (1, 4096, 8, 16, 128, 64) if op == "prompt" else (16, 8192, 8, 16, 128, 16)
+    n = dict(prompt=4096, attend=1, chunk=2)[op]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pages = B * L // page
+    pool = lambda: torch.randn(pages, kv, page, hd, generator=g, device="cuda").bfloat16().permute(0, 2, 1, 3)  # noqa: E731
+    cache = S.PagedCache(pool(), pool(), torch.arange(pages, device="cuda").reshape(B, -1).int(),
+                         torch.full((B,), L, dtype=torch.int32, device="cuda"))
+    q = torch.randn(B * n, nh, hd, generator=g, device="cuda").bfloat16()
+    cu = torch.arange(B + 1, device="cuda").int() * n
+    call = lambda: S.attend(cache, q, 0.09) if op == "attend" else S.attend_prompt(cache, q, cu, 0.09)  # noqa: E731
+
+    def best():
+        times = []
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            out = call()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times), out
+    clean, was = best()
+    assert torch.isfinite(was).all()
+    first = cache.table[:, 0].long()
+    if what == "key":
+        cache.k[first, 0] = NAN
+    else:
+        cache.v[first, 0, :, 3] = math.inf
+    slow, out = best()
+    _no_error()
+    assert slow < 8 * clean, (slow, clean)
+    if what == "key":
+        assert torch.isnan(out).all()
+    else:
+        assert (out[:, :, 3] == math.inf).all()
+        rest = [i for i in range(hd) if i != 3]
+        assert torch.equal(out[:, :, rest], was[:, :, rest])
