@@ -225,6 +225,11 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (
 // The factor a state kept at maximum m takes at maximum m2 >= m (1 where both are still -infinity).
 __device__ __forceinline__ float shrink(float m, float m2) { return m2 == neg_inf() ? 1.0f : ex2(m - m2); }
 
+// Probabilities and sums are kept 2^kLift times as large: fp16 ends at 2^-25, and slots of less than that share of a
+// warp's maximum, tens of thousands of them, would count in the sum but not in the output. From 2^14 two parts reach 2^-39.
+template <class T>
+constexpr float kLift = __is_same(T, __half) ? 14.0f : 0.0f;
+
 // What a call keeps in its workspace: the CTAs' states, the scores and the final statistics.
 struct AttendWs {
   float* part;
@@ -473,7 +478,7 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float base = m[nb][e & 1] == neg_inf() ? 0.0f : m[nb][e & 1];
+          const float base = m[nb][e & 1] == neg_inf() ? 0.0f : m[nb][e & 1] - kLift<T>;
           p[e] = seen(nb, e) ? ex2(s[nb][e] - base) : 0.0f;
         }
         l[nb][0] += p[0] + p[2];
@@ -569,7 +574,7 @@ __global__ void __launch_bounds__(AttendShape<HD>::kThreads, 1)
             const int tok = ONE ? 0 : h / heads;
             *reinterpret_cast<uint2*>(a.out + 2 * ((int64_t)(row0 + tok) * a.orow + (int64_t)(h0 + h - tok * heads) * a.oh +
                                                    col)) = make_uint2(Elem<T>::pack(v.x, v.y), Elem<T>::pack(v.z, v.w));
-            if (col == 0 && ws.ml) ws.ml[(int64_t)w.q.b * a.nh + h0 + h] = make_float2(mm, sum);
+            if (col == 0 && ws.ml) ws.ml[(int64_t)w.q.b * a.nh + h0 + h] = make_float2(mm - kLift<T>, sum);
           } else {
             *reinterpret_cast<float4*>(part + h * HD + col) = v;
             if (col == 0) {
@@ -690,7 +695,7 @@ __global__ void __launch_bounds__(kJoinThreads)
       good = l != l || fabsf(v.x) + fabsf(v.y) < __int_as_float(0x7F800000);
       to[threadIdx.x] = Elem<T>::pack(v.x, v.y);
     }
-    if (ws.ml && threadIdx.x == 0) ws.ml[(int64_t)q.b * a.nh + h] = make_float2(m, l);
+    if (ws.ml && threadIdx.x == 0) ws.ml[(int64_t)q.b * a.nh + h] = make_float2(m - kLift<T>, l);
     redo = __syncthreads_or(!good);
   }
   if (redo && warp == 0) {

@@ -1039,3 +1039,42 @@ def test_a_nonfinite_row_that_everyone_sees_costs_no_second_pass(op, what):
         assert (out[:, :, 3] == math.inf).all()
         rest = [i for i in range(hd) if i != 3]
         assert torch.equal(out[:, :, rest], was[:, :, rest])
+
+
+@pytest.mark.parametrize("op,n", [("attend", 1), ("weights", 1), ("chunk", 2), ("tiles", 8000)])
+@pytest.mark.parametrize("hd,page", [(64, 64), (256, 16)])
+def test_small_probabilities_of_many_slots_count_in_fp16(op, n, hd, page):
+    """One slot draws nearly everything and 60000 others a share below the smallest fp16 number each, together
+    more than the output's rounding: they must reach the output as they reach the sum. With values 0 and 1 the
+    output is their total share t, rounded to fp16 once: half a step is 2^-11 t. attend_prompt rounds every share to a
+    step of 2^-31 of the maximum (2^-24, the probabilities kept 2^7 times as large) once, attend in two parts to
+    one of 2^-38: half of that a slot. The exponentials and fp32 sums are allowed 2^-13 t: the exponent, 26, is off
+    by 2^-18 at most and each of some 200 additions in a row by 2^-24."""
+    from opentars_b200 import serving as S
+    L = 60000
+    B = 300 if n == 1 else 1                                   # (over the same pages, so that a few warps see a whole one)
+    k = torch.zeros(-(-L // page), page, 1, hd, dtype=torch.float16)
+    v = torch.ones_like(k)
+    k[0, 0, 0, 0], v[0, 0] = 4.5, 0.0
+    table = torch.arange(k.shape[0], dtype=torch.int32)[None].expand(B, -1).contiguous()
+    q = torch.zeros(B * n, 1, hd, dtype=torch.float16)
+    q[:, 0, 0] = 4.0                                           # exp(-18) = 2^-25.97 each
+    track = None
+    if op == "weights":
+        cap = table.shape[1] * page
+        track = (torch.zeros(B, 1, cap), torch.zeros(B, 1, cap, dtype=torch.int32), torch.full((B,), L, dtype=torch.int32))
+    cache = _cache(k, v, table, [L] * B, "heads", track)
+    small = math.exp(-18)
+    others = torch.full((B,), L - 1.0).double() if n == 1 else torch.arange(L - n, L).double()
+    t = others * small / (1 + others * small)
+    if n == 1:
+        out = S.attend(cache, q.cuda(), 1.0, weight_out=cache.weight)
+    else:
+        out = S.attend_prompt(cache, q.cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), 1.0)
+    _no_error()
+    off = (out.double().cpu()[:, 0] - t[:, None]).abs()
+    assert (off <= (t * (2.0 ** -11 + 2.0 ** -13) + L * 2.0 ** (-32 if op == "tiles" else -39))[:, None]).all(), off.max()
+    if op == "weights":
+        w, whole = cache.weight[:, 0].double(), 1 + (L - 1) * small
+        assert ((w[:, 0] * whole - 1).abs() < 2.0 ** -13).all()
+        assert ((w[:, 1:L] * whole / small - 1).abs() < 2.0 ** -13).all() and (w[:, L:] == 0).all()
