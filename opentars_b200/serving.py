@@ -75,6 +75,13 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _whole(low: int, **values: int) -> None:
+    """Whole numbers from `low` up that the C side holds in 32 bits (ctypes would drop the higher ones)."""
+    for name, v in values.items():
+        if not low <= v <= 0x7FFFFFFF:
+            raise ValueError(f"{name} = {v}: between {low} and 2^31 - 1")
+
+
 def _check(rc: int, what: str) -> None:
     if rc == TC_ERR_ARG:
         raise ValueError(f"{what}: an argument is out of range or not 16-byte aligned")
@@ -244,8 +251,8 @@ def _attend_args(cache: PagedCache, q: torch.Tensor, out: torch.Tensor | None, w
     n, row, head = _rows(q, cache, 0, "q")
     if q.dtype is not cache.dtype:
         raise ValueError(f"q has the cache's type {cache.dtype}, not {q.dtype}")
-    if window < 0 or sinks < 0:
-        raise ValueError("window and sinks are not negative")
+    if not (0 <= window <= 0x7FFFFFFF and 0 <= sinks <= 0x7FFFFFFF):
+        _whole(0, window=window, sinks=sinks)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.dtype is not q.dtype or out.shape != q.shape or not (out.is_contiguous() or _apart(out)):
@@ -297,7 +304,8 @@ def evict(cache: PagedCache, budget: int, sinks: int = 0, recent: int = 0, lengt
     the holes before it. The new lengths, weights and positions go to the *_out tensors (None: the
     cache's own)."""
     _need(cache.weight is not None, "the cache keeps no weights")
-    _need(budget >= 1 and sinks >= 0 and recent >= 0 and sinks + recent <= budget, "0 <= sinks + recent <= budget")
+    _whole(1, budget=budget)
+    _need(sinks >= 0 and recent >= 0 and sinks + recent <= budget, "0 <= sinks + recent <= budget")
     length_out = cache.length if length_out is None else length_out
     pos_out = cache.pos if pos_out is None else pos_out
     _ints(length_out, (cache.batch,), cache.device, "length_out")
@@ -334,6 +342,7 @@ def rules_of(logits: torch.Tensor | None, out: torch.Tensor | None = None, histo
              none: int = -1, shape: tuple | None = None, device: torch.device | None = None) -> Rules_t:
     """The checked C description of adjust_logits' arguments; without logits, of rules on a decode engine's
     own logits of this shape and device."""
+    _whole(-1 << 31, none=none)
     if logits is None:
         (rows, vocab), dev = shape, device
         x = y = None

@@ -1078,3 +1078,19 @@ def test_small_probabilities_of_many_slots_count_in_fp16(op, n, hd, page):
         w, whole = cache.weight[:, 0].double(), 1 + (L - 1) * small
         assert ((w[:, 0] * whole - 1).abs() < 2.0 ** -13).all()
         assert ((w[:, 1:L] * whole / small - 1).abs() < 2.0 ** -13).all() and (w[:, L:] == 0).all()
+
+
+def test_whole_numbers_beyond_32_bits_are_refused():
+    from opentars_b200 import serving as S
+    cache = S.PagedCache.empty(4, 16, 2, 64, 2, 2, track=True)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    x = torch.zeros(2, 10, device="cuda")
+    big = 2 ** 32 + 8
+    for i, call in enumerate([lambda: S.attend(cache, q, 1.0, window=big), lambda: S.attend(cache, q, 1.0, sinks=big),
+                 lambda: S.attend_prompt(cache, q, cu, 1.0, window=big), lambda: S.attend_prompt(cache, q, cu, 1.0, sinks=big),
+                 lambda: S.evict(cache, big), lambda: S.evict(cache, big, recent=2 ** 32),
+                 lambda: S.adjust_logits(x, none=big), lambda: S.adjust_logits(x, none=-2 ** 31 - 1)]):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")

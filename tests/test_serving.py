@@ -184,3 +184,19 @@ def test_pools_whose_rows_share_memory_are_refused(L):
     for good in (pool, pool.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3), pool[:, :, :1], pool[:1]):
         with pytest.raises(ValueError, match="CUDA"):           # everything else about it is right
             S.PagedCache(good, good, table, length)
+
+
+def test_whole_numbers_that_32_bits_do_not_hold_are_refused():
+    """ctypes drops the higher bits without a word: a budget of 2^32 + 8 would cut a cache to 8 slots."""
+    import torch
+
+    from opentars_b200 import serving as S
+    S._whole(0, window=0, sinks=2 ** 31 - 1)
+    S._whole(-2 ** 31, none=-2 ** 31)
+    for low, v in ((0, 2 ** 31), (0, 2 ** 32 + 8), (0, -1), (1, 0), (-2 ** 31, -2 ** 31 - 1), (0, 2 ** 64)):
+        with pytest.raises(ValueError, match="window"):
+            S._whole(low, window=v)
+    for none in (2 ** 31, 2 ** 32 + 7, -2 ** 31 - 1):
+        with pytest.raises(ValueError, match="none"):
+            S.rules_of(None, shape=(2, 10), device=torch.device("cpu"), none=none)
+    assert S.rules_of(None, shape=(2, 10), device=torch.device("cpu"), none=-5).none == -5
