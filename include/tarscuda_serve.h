@@ -69,7 +69,7 @@ int tc_kv_append(const tc_kv_cache* c, const void* k, const void* v, int32_t src
  * p = softmax over the visible slots j of scale * q[b][h] . k_j; head h reads key-value head
  * h / (n_heads / n_kv). Slot j of length[b] = L is visible if j >= L - window or j < sinks (window 0:
  * all). A sequence of length 0 gets zeros. q and out have the cache's type, rows [batch][n_heads]
- * [head_dim] with strides in elements, 16-byte aligned. With weight_out (laid out as the cache's
+ * [head_dim] with strides in elements, 16-byte aligned, and share no memory. With weight_out (laid out as the cache's
  * weight, which may be it) weight_out[b][g][j] = weight[b][g][j] + the p_j of the heads of
  * key-value head g, for j < L; slots behind are left alone.
  * ws: tc_attend_workspace bytes, 256-byte aligned. */
@@ -81,7 +81,8 @@ uint64_t tc_attend_workspace(const tc_kv_cache* c, int32_t n_heads, int32_t weig
 /* Attention of the tokens of a prompt, or of a chunk of one, whose key and value rows are in the
  * cache already: rows cu[b] .. cu[b+1] - 1 of q are the last tokens of sequence b, row i of n at
  * position p = length[b] - n + i. It sees slot j if j <= p and (p - j < window or j < sinks; window
- * 0: all). Rows at a negative position get zeros; rows at and behind cu[batch] are left alone.
+ * 0: all). Rows at a negative position get zeros; rows at and behind cu[batch] are left alone. q and out
+ * share no memory.
  * ws: tc_attend_prompt_workspace bytes, 256-byte aligned (0 bytes, and NULL, for calls of many
  * rows). */
 int tc_attend_prompt(const tc_kv_cache* c, const void* q, int64_t q_row_stride, int64_t q_head_stride, void* out,
@@ -97,8 +98,8 @@ uint64_t tc_attend_prompt_workspace(const tc_kv_cache* c, int32_t n_heads, int32
  * before it, in ascending order: every other slot stays where it is, nothing is read that was
  * written, and attention without a window is unchanged but for what was evicted. Afterwards
  * length_out[b] = min(length[b], budget), and weight_out and pos_out hold the slots' weights and
- * positions (each may be the cache's own array; otherwise all slots before length_out[b] are
- * written). Pages of such a sequence must not be shared with another one.
+ * positions (each may be the cache's own array, but no shifted part of it; otherwise all slots before
+ * length_out[b] are written). Pages of such a sequence must not be shared with another one.
  * ws: tc_kv_evict_workspace bytes, 256-byte aligned. */
 int tc_kv_evict(const tc_kv_cache* c, int32_t budget, int32_t sinks, int32_t recent, int32_t* length_out,
                 float* weight_out, int32_t* pos_out, void* ws, uint64_t ws_bytes, void* stream);
@@ -115,7 +116,7 @@ uint64_t tc_kv_evict_workspace(const tc_kv_cache* c, int32_t budget);
  * order); `none` when the mask allows no token. Ids outside the vocabulary are ignored. */
 typedef struct {
   const float* logits;          /* [rows][vocab], rows logits_stride elements apart */
-  float* out;                   /* the same logits, or another array */
+  float* out;                   /* the same logits, or rows that share no memory with them */
   int64_t logits_stride, out_stride;
   int32_t rows, vocab;
   const int32_t* history;       /* [rows][max_history] token ids: the prompt's, then the generated ones */

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 
 #include "mma.h"
 #include "serve.h"
@@ -17,6 +18,35 @@ constexpr int64_t kMaxStride = 1ll << 40;
 bool al16(const void* p) { return (uintptr_t)p % 16 == 0; }
 // A stride in elements of `bytes` each that keeps rows 16-byte aligned.
 bool stride_ok(int64_t s, int bytes) { return s >= 0 && s < kMaxStride && s * bytes % 16 == 0; }
+
+// Whether two sets of rows, rows x heads runs of `width` elements with strides of their own, may share an element.
+// Exact for two of the same nested strides (interleaved parts of one buffer are apart); with different strides they
+// may as soon as their ranges meet. `ahead`: how many elements the second set starts behind the first.
+bool may_share(int64_t ahead, int64_t ra, int64_t ha, int64_t rb, int64_t hb, int64_t rows, int64_t heads, int64_t width) {
+  if (rows == 1) ra = rb = 0;                    // a dimension of one entry is never stepped over
+  if (heads == 1) ha = hb = 0;
+  const auto reach = [&](int64_t r, int64_t h) { return (double)(rows - 1) * r + (double)(heads - 1) * h + width; };
+  if ((double)ahead >= reach(ra, ha) || -(double)ahead >= reach(rb, hb)) return false;
+  if (ra != rb || ha != hb) return true;
+  const int64_t big = std::max(ra, ha), small = std::min(ra, ha), nb = ra >= ha ? rows : heads, ns = ra >= ha ? heads : rows;
+  if ((nb > 1 && (double)(ns - 1) * small + width > (double)big) || (ns > 1 && small < width)) return true;
+  const int64_t d = std::abs(ahead), i0 = big ? d / big : 0;
+  for (int64_t i = i0; i <= i0 + (big > 0); ++i) {
+    const int64_t left = d - i * big, j0 = small ? std::abs(left) / small : 0;
+    if (i >= nb) break;
+    for (int64_t j = j0; j <= j0 + (small > 0); ++j)
+      if (j < ns && std::abs(left) - j * small < width && j * small - std::abs(left) < width) return true;
+  }
+  return false;
+}
+int64_t ahead_of(const void* a, const void* b, int bytes) {
+  return ((int64_t)(uintptr_t)b - (int64_t)(uintptr_t)a) / bytes;
+}
+// An output of n 4-byte elements that may be the array it is computed from, but no shifted part of it.
+bool same_or_apart(const void* a, const void* b, int64_t n) {
+  const int64_t ahead = ahead_of(a, b, 4);
+  return a == b || ahead >= n || -ahead >= n;
+}
 
 // Whether a pool's rows of head_dim elements lie apart, its dimensions nested in any order (a stride of 0 or
 // one that steps into the next row has rows share memory; a dimension of one entry is never stepped over).
@@ -36,6 +66,9 @@ bool pool_apart(const tc_kv_cache* c) {
   }
   return true;
 }
+
+// Entries of a cache's weight and pos.
+int64_t tracked(const tc_kv_cache* c) { return (int64_t)c->batch * c->n_kv * c->track_stride; }
 
 // Everything of a cache that the host can check.
 bool take_cache(const tc_kv_cache* c, KvCache* o) {
@@ -67,10 +100,12 @@ bool take_cache(const tc_kv_cache* c, KvCache* o) {
 bool take_error(KvCache* c) { return (c->err = wait_error_flag()) != nullptr; }
 
 bool take_attend(const tc_kv_cache* c, const void* q, int64_t qr, int64_t qh, void* out, int64_t orow, int64_t oh,
-                 int32_t nh, float scale, int32_t window, int32_t sinks, AttendArgs* a) {
+                 int32_t nh, float scale, int32_t window, int32_t sinks, int64_t rows, AttendArgs* a) {
   if (!take_cache(c, &a->c) || !q || !out || !al16(q) || !al16(out)) return false;
   if (!stride_ok(qr, 2) || !stride_ok(qh, 2) || !stride_ok(orow, 2) || !stride_ok(oh, 2)) return false;
   if (nh < 1 || nh % c->n_kv || nh > (1 << 16) || window < 0 || sinks < 0 || !std::isfinite(scale)) return false;
+  // (a row is read again after its output is stored where that is not finite)
+  if (may_share(ahead_of(q, out, 2), qr, qh, orow, oh, rows, nh, c->head_dim)) return false;
   a->dtype = c->dtype;
   a->q = static_cast<const uint8_t*>(q); a->qr = qr; a->qh = qh;
   a->out = static_cast<uint8_t*>(out); a->orow = orow; a->oh = oh;
@@ -116,9 +151,9 @@ int tc_attend(const tc_kv_cache* c, const void* q, int64_t q_row_stride, int64_t
               int32_t sinks, float* weight_out, void* ws, uint64_t ws_bytes, void* stream) {
   AttendArgs a{};
   if (!take_attend(c, q, q_row_stride, q_head_stride, out, out_row_stride, out_head_stride, n_heads, scale, window,
-                   sinks, &a))
+                   sinks, c ? c->batch : 1, &a))
     return TC_ERR_ARG;
-  if (weight_out && !c->weight) return TC_ERR_ARG;
+  if (weight_out && (!c->weight || !same_or_apart(c->weight, weight_out, tracked(c)))) return TC_ERR_ARG;
   const uint64_t need = attend_workspace(a.c, n_heads, weight_out != nullptr);
   if (need && (!ws || (uintptr_t)ws % 256 || ws_bytes < need)) return TC_ERR_ARG;
   a.weight_out = weight_out;
@@ -135,7 +170,7 @@ int tc_attend_prompt(const tc_kv_cache* c, const void* q, int64_t q_row_stride, 
   if (tokens < 0 || tokens > (1 << 28) || !cu) return TC_ERR_ARG;
   if (tokens == 0) return take_cache(c, &a.c) ? TC_OK : TC_ERR_ARG;
   if (!take_attend(c, q, q_row_stride, q_head_stride, out, out_row_stride, out_head_stride, n_heads, scale, window,
-                   sinks, &a))
+                   sinks, tokens, &a))
     return TC_ERR_ARG;
   const uint64_t need = chunk_workspace(a.c, n_heads, tokens, a.window, a.sinks);
   if (need && (!ws || (uintptr_t)ws % 256 || ws_bytes < need)) return TC_ERR_ARG;
@@ -168,6 +203,9 @@ int tc_kv_evict(const tc_kv_cache* c, int32_t budget, int32_t sinks, int32_t rec
   if (!take_cache(c, &a.c) || !c->weight || budget < 1 || sinks < 0 || recent < 0 ||
       (int64_t)sinks + recent > budget || !length_out || !weight_out || !pos_out)
     return TC_ERR_ARG;
+  if (!same_or_apart(c->weight, weight_out, tracked(c)) || !same_or_apart(c->pos, pos_out, tracked(c)) ||
+      !same_or_apart(c->length, length_out, c->batch))
+    return TC_ERR_ARG;
   if (!ws || (uintptr_t)ws % 256 || ws_bytes < evict_workspace(a.c, budget)) return TC_ERR_ARG;
   a.budget = budget; a.sinks = sinks; a.recent = recent;
   a.length_out = length_out; a.weight_out = weight_out; a.pos_out = pos_out;
@@ -181,6 +219,9 @@ int tc_adjust_logits(const tc_logits_rules* r, void* stream) {
       r->logits_stride < r->vocab || r->out_stride < r->vocab)
     return TC_ERR_ARG;
   tc_logits_rules a = *r;
+  if ((a.logits != a.out || (a.rows > 1 && a.logits_stride != a.out_stride)) &&
+      may_share(ahead_of(a.logits, a.out, 4), a.logits_stride, 0, a.out_stride, 0, a.rows, 1, a.vocab))
+    return TC_ERR_ARG;
   if (a.history) {
     if (a.max_history < 0 || a.max_history >= (1 << 20) || a.history_stride < a.max_history) return TC_ERR_ARG;
   } else if (a.n_history || a.n_prompt || a.repetition || a.presence || a.frequency) {

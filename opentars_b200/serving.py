@@ -84,7 +84,7 @@ def _whole(low: int, **values: int) -> None:
 
 def _check(rc: int, what: str) -> None:
     if rc == TC_ERR_ARG:
-        raise ValueError(f"{what}: an argument is out of range or not 16-byte aligned")
+        raise ValueError(f"{what}: an argument is out of range, not 16-byte aligned, or shares memory with an output")
     if rc != 0:
         raise RuntimeError(f"{what} failed ({rc})")
 
@@ -265,7 +265,8 @@ def attend(cache: PagedCache, q: torch.Tensor, scale: float, window: int = 0, si
            out: torch.Tensor | None = None, weight_out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one query row per sequence, q [batch, heads, head_dim], over its slots: those of the
     last `window` (0: all) and the first `sinks`. weight_out (cache.weight, or a tensor like it)
-    receives cache.weight plus the attention weight each slot draws. Length 0 gives zeros."""
+    receives cache.weight plus the attention weight each slot draws. Length 0 gives zeros. out must not share
+    memory with q."""
     n, out, args = _attend_args(cache, q, out, window, sinks)
     if n != cache.batch:
         raise ValueError(f"{n} query rows for {cache.batch} sequences")
@@ -280,7 +281,7 @@ def attend_prompt(cache: PagedCache, q: torch.Tensor, cu: torch.Tensor, scale: f
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the last tokens of each sequence, rows cu[b] .. cu[b+1]-1 of q [tokens, heads,
     head_dim] for sequence b, each over the slots up to its own position, of the last `window` (0: all)
-    and the first `sinks`. Rows at and behind cu[batch] are left alone."""
+    and the first `sinks`. Rows at and behind cu[batch] are left alone. out must not share memory with q."""
     n, out, args = _attend_args(cache, q, out, window, sinks)
     cu_p = _cu(cu, cache)
     if n:
@@ -385,7 +386,7 @@ def rules_of(logits: torch.Tensor | None, out: torch.Tensor | None = None, histo
 
 def adjust_logits(logits: torch.Tensor, token: torch.Tensor | None = None, none: int = -1, **rules) -> torch.Tensor:
     """Penalties, biases and a grammar mask on fp32 logits [rows, vocab], and the greedy pick: the picks
-    [rows] int32 (`token`, or a new tensor). Keywords, each optional: out (None: in place), history
+    [rows] int32 (`token`, or a new tensor). Keywords, each optional: out (None: in place; no shifted part of logits), history
     [rows, ids] int32 with n_history and n_prompt [rows] (prompt ids first), repetition / presence /
     frequency [rows] fp32, bias_ids / bias [rows, entries] (the last entry of a token counts), mask
     int32 words, bit t % 32 of word t // 32 set where token t is allowed. A row whose mask allows

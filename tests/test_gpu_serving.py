@@ -1094,3 +1094,46 @@ def test_whole_numbers_beyond_32_bits_are_refused():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_attend_takes_parts_of_one_buffer_that_are_apart():
+    """q and out as parts of one buffer: taken where no row of one shares an element with a row of the other, refused
+    where one does (in place as well: a row whose output is not finite reads its query again)."""
+    import random
+
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(31)
+    rng = random.Random(31)
+    k, v, table = _pools([30, 77, 5], 1, 64, 16, torch.bfloat16, g)
+    cache = _cache(k, v, table, [30, 77, 5])
+    cu = torch.arange(4).int().cuda()
+    plain = torch.randn(3, 2, 64, generator=g).bfloat16().cuda()
+    want = [S.attend(cache, plain, 0.1), S.attend_prompt(cache, plain, cu, 0.1)]
+    strides = [(128, 64), (64, 192), (256, 128), (384, 64), (128, 512), (256, 64), (72, 320)]
+    taken = 0
+    for i in range(60):
+        row, head = strides[i % len(strides)]
+        buf = torch.zeros(4000, dtype=torch.bfloat16, device="cuda")
+        part = lambda at: buf.as_strided((3, 2, 64), (row, head, 1), at)  # noqa: E731
+        a, b = 8 * rng.randrange(200), 8 * rng.randrange(200)
+        if i % 4 == 0:
+            b = a + rng.choice([64, 128, -64, 192]) if a >= 64 else a
+        of = lambda at: set((at + torch.arange(3)[:, None, None] * row + torch.arange(2)[:, None] * head + torch.arange(64)).flatten().tolist())  # noqa: E731
+        q, out = part(a), part(b)
+        q.copy_(plain)
+        for call, ref in zip((lambda: S.attend(cache, q, 0.1, out=out), lambda: S.attend_prompt(cache, q, cu, 0.1, out=out)), want):
+            if of(a) & of(b):
+                with pytest.raises(ValueError):
+                    call()
+            else:
+                assert torch.equal(call(), ref)
+                taken += 1
+    assert 20 < taken < 100
+    logits = torch.randn(5, 40, generator=g).cuda()
+    with pytest.raises(ValueError):
+        S.adjust_logits(logits[:4], out=logits[1:])
+    wide = torch.zeros(4, 80, device="cuda")
+    wide[:, :40] = logits[:4]
+    S.adjust_logits(wide[:, :40], out=wide[:, 40:])
+    assert torch.equal(wide[:, 40:], logits[:4]) and torch.equal(wide[:, :40], logits[:4])
+    _no_error()

@@ -200,3 +200,25 @@ def test_whole_numbers_that_32_bits_do_not_hold_are_refused():
         with pytest.raises(ValueError, match="none"):
             S.rules_of(None, shape=(2, 10), device=torch.device("cpu"), none=none)
     assert S.rules_of(None, shape=(2, 10), device=torch.device("cpu"), none=-5).none == -5
+
+
+def test_outputs_that_share_memory_with_inputs_are_refused(L):
+    from opentars_b200.serving import Rules_t
+    p = 1 << 20
+    c = ctypes.byref(_cache(**TRACK))                          # 2 sequences, a head of 128, 64 slots tracked
+    # (q's strides, out's start in elements and strides)
+    for qr, qh, at, orow, oh in ((256, 128, 0, 256, 128), (256, 128, 128, 256, 128), (256, 128, -384, 256, 128), (256, 128, 504, 256, 128),
+                                 (512, 128, 512, 512, 128), (512, 128, 128, 512, 128), (128, 512, 384, 128, 512),
+                                 (512, 256, 120, 512, 256), (512, 128, 256, 256, 128), (0, 128, 128, 256, 128)):
+        out = p + 2 * at
+        assert L.tc_attend(c, p, qr, qh, out, orow, oh, 2, 1.0, 0, 0, None, p, 1 << 30, None) == -2, (qr, qh, at)
+        assert L.tc_attend_prompt(c, p, qr, qh, out, orow, oh, 2, p, 2, 1.0, 0, 0, p, 1 << 30, None) == -2, (qr, qh, at)
+    n = 2 * 64
+    for at in (4, -4, 4 * (n - 1), -4 * (n - 1)):
+        assert L.tc_attend(c, p, 256, 128, p + 4096, 256, 128, 2, 1.0, 0, 0, p + at, p, 1 << 30, None) == -2, at
+        assert L.tc_kv_evict(c, 16, 0, 0, p, p + at, p, p, 1 << 30, None) == -2, at
+        assert L.tc_kv_evict(c, 16, 0, 0, p, p, p + at, p, 1 << 30, None) == -2, at
+    assert L.tc_kv_evict(c, 16, 0, 0, p + 4, p, p, p, 1 << 30, None) == -2
+    for at, stride, ostride in ((4, 100, 100), (-4, 100, 100), (400, 100, 100), (0, 100, 104), (200, 200, 200), (400, 200, 208)):
+        r = Rules_t(logits=p, out=p + at, logits_stride=stride, out_stride=ostride, rows=2, vocab=100)
+        assert L.tc_adjust_logits(ctypes.byref(r), None) == -2, (at, stride)
