@@ -83,7 +83,8 @@ int tc_engine_positions(tc_engine* e, int32_t* pos_host);
  * vocab, token and strides of the two are the engine's own and not read. Each sequence's pick becomes
  * the rules' pick: tc_engine_tokens returns it, and a following step without host tokens feeds it.
  * `none`, the pick where a mask allows nothing, must be a token of the vocabulary when there is a mask.
- * tc_engine_logits then returns the changed logits. No counterpart in the reference. */
+ * tc_engine_logits then returns the changed logits. To be called once a step: a second call applies the
+ * penalties and biases to the changed logits again. No counterpart in the reference. */
 int tc_engine_adjust(tc_engine* e, const tc_logits_rules* r);
 /* The fused decode step: one-token steps run as one cooperative kernel over every SM (all layers,
  * the final norm and the head; then the greedy pick) when the model and batch fit it (batch <= 64,

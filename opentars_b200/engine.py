@@ -183,12 +183,14 @@ class DecodeEngine:
         self._check(lib().tc_engine_logits(self.h, out.ctypes.data_as(ctypes.c_void_p)), "logits")
         return out
 
-    def adjust(self, none: int = 0, **rules) -> None:
+    def adjust(self, none: int = 0, *, history=None, n_history=None, n_prompt=None, repetition=None, presence=None,
+               frequency=None, bias_ids=None, bias=None, mask=None) -> None:
         """Rules on the last step's logits before its picks are used (serving.adjust_logits' keywords
-        history, n_history, n_prompt, repetition, presence, frequency, bias_ids, bias and mask: torch
-        tensors on the engine's device, a row per sequence): logits() and tokens() then return the changed
-        logits and their picks, and step(None) feeds those. A sequence whose mask allows nothing picks
-        `none`. Ordered after the work that torch's current stream holds, and before what it gets next."""
+        without its out and token: torch tensors on the engine's device, a row per sequence): logits() and
+        tokens() then return the changed logits and their picks, and step(None) feeds those. A sequence whose
+        mask allows nothing picks `none`. Once a step: a second call would apply the penalties and biases to
+        the changed logits again. Ordered after the work that torch's current stream holds, and before
+        what it gets next."""
         import torch
 
         from .serving import rules_of
@@ -196,7 +198,9 @@ class DecodeEngine:
             own = torch.cuda.ExternalStream(lib().tc_engine_stream(self.h), device=self.device)
             now = torch.cuda.current_stream(self.device)
             own.wait_stream(now)
-            r = rules_of(None, shape=(self.B, self.vocab), device=torch.device("cuda", self.device), none=none, **rules)
+            r = rules_of(None, shape=(self.B, self.vocab), device=torch.device("cuda", self.device), none=none,
+                         history=history, n_history=n_history, n_prompt=n_prompt, repetition=repetition,
+                         presence=presence, frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask)
             self._check(lib().tc_engine_adjust(self.h, ctypes.byref(r)), "adjust")
             now.wait_stream(own)
 

@@ -222,3 +222,17 @@ def test_outputs_that_share_memory_with_inputs_are_refused(L):
     for at, stride, ostride in ((4, 100, 100), (-4, 100, 100), (400, 100, 100), (0, 100, 104), (200, 200, 200), (400, 200, 208)):
         r = Rules_t(logits=p, out=p + at, logits_stride=stride, out_stride=ostride, rows=2, vocab=100)
         assert L.tc_adjust_logits(ctypes.byref(r), None) == -2, (at, stride)
+
+
+def test_the_engines_rules_take_no_outputs():
+    """DecodeEngine.adjust works on the engine's own logits and picks: out and token, which it would never
+    write, are not among its keywords (no engine is needed to refuse them)."""
+    import inspect
+
+    from opentars_b200 import serving as S
+    from opentars_b200.engine import DecodeEngine
+    for name in ("out", "token", "logits", "no_such_rule"):
+        with pytest.raises(TypeError, match=name):
+            DecodeEngine.adjust(object(), **{name: None})
+    rules = set(inspect.signature(S.rules_of).parameters) - {"logits", "out", "token", "shape", "device"}
+    assert set(inspect.signature(DecodeEngine.adjust).parameters) == rules | {"self"}
