@@ -12,7 +12,8 @@
 Work is enqueued on torch's current stream of the tensors' device and can be captured into a CUDA
 graph. Wrong arguments raise ValueError before anything is enqueued; what only the device can see
 (a page id outside the pool, a length beyond the page list) is left out and recorded, and
-`device_error` reads it. Only forward passes: the framework trains nothing.
+`device_error` reads it. Only forward passes: the framework trains nothing, and tensors that
+require a gradient are refused outside torch.no_grad.
 """
 from __future__ import annotations
 
@@ -87,6 +88,13 @@ def _check(rc: int, what: str) -> None:
         raise ValueError(f"{what}: an argument is out of range, not 16-byte aligned, or shares memory with an output")
     if rc != 0:
         raise RuntimeError(f"{what} failed ({rc})")
+
+
+def _no_gradient() -> None:
+    """Called where a tensor requires a gradient: the calls have no backward pass, and a request for one is
+    refused, not silently cut off."""
+    if torch.is_grad_enabled():
+        raise ValueError("a tensor requires a gradient: the operators have none (detach it, or use torch.no_grad)")
 
 
 def _ints(t: torch.Tensor, shape: tuple, device: torch.device, name: str) -> None:
@@ -241,6 +249,8 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor
         raise ValueError("k and v: rows of one shape, type (fp32, bf16 or fp16) and stride")
     if cu is None:
         _need(n <= cache.batch, "without cu there is one row per sequence")
+    if k.requires_grad or v.requires_grad:
+        _no_gradient()
     cu_p = None if cu is None else _cu(cu, cache)
     if n:
         _run(cache.index, "append", lib().tc_kv_append, cache.ref, k.data_ptr(), v.data_ptr(), code, row, head, cu_p, n)
@@ -257,6 +267,8 @@ def _attend_args(cache: PagedCache, q: torch.Tensor, out: torch.Tensor | None, w
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.dtype is not q.dtype or out.shape != q.shape or not (out.is_contiguous() or _apart(out)):
         raise ValueError("out has q's shape and type, its rows apart")
+    if q.requires_grad or out.requires_grad:
+        _no_gradient()
     _, orow, ohead = _rows(out, cache, q.shape[1], "out")
     return n, out, (q.data_ptr(), row, head, out.data_ptr(), orow, ohead, q.shape[1])
 
@@ -343,7 +355,8 @@ def rules_of(logits: torch.Tensor | None, out: torch.Tensor | None = None, histo
              none: int = -1, shape: tuple | None = None, device: torch.device | None = None) -> Rules_t:
     """The checked C description of adjust_logits' arguments; without logits, of rules on a decode engine's
     own logits of this shape and device."""
-    _whole(-1 << 31, none=none)
+    if not -0x80000000 <= none <= 0x7FFFFFFF:
+        _whole(-0x80000000, none=none)
     if logits is None:
         (rows, vocab), dev = shape, device
         x = y = None
@@ -351,6 +364,8 @@ def rules_of(logits: torch.Tensor | None, out: torch.Tensor | None = None, histo
     else:
         _need(logits.is_cuda and logits.dim() == 2 and logits.shape[0] >= 1 and logits.shape[1] >= 1,
               "logits: fp32 [rows, vocab] on a CUDA device")
+        if logits.requires_grad or (out is not None and out.requires_grad):
+            _no_gradient()
         rows, dev = logits.shape[0], logits.device
         x, x_stride, vocab = _matrix(logits, torch.float32, rows, dev, "logits")
         y, y_stride, n = (x, x_stride, vocab) if out is None else _matrix(out, torch.float32, rows, dev, "out")

@@ -1137,3 +1137,23 @@ def test_attend_takes_parts_of_one_buffer_that_are_apart():
     S.adjust_logits(wide[:, :40], out=wide[:, 40:])
     assert torch.equal(wide[:, 40:], logits[:4]) and torch.equal(wide[:, :40], logits[:4])
     _no_error()
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    from opentars_b200 import serving as S
+    cache = S.PagedCache.empty(4, 16, 2, 64, 2, 2)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    x = torch.zeros(2, 10, device="cuda", requires_grad=True)
+    plain = q.detach()
+    calls = [lambda: S.attend(cache, q, 1.0), lambda: S.attend_prompt(cache, q, cu, 1.0), lambda: S.append(cache, q[:, :2], q[:, 2:]),
+             lambda: S.append(cache, plain[:, :2], q[:, 2:]), lambda: S.adjust_logits(x, out=torch.zeros(2, 10, device="cuda")),
+             lambda: S.attend(cache, plain, 1.0, out=torch.zeros_like(q, requires_grad=True))]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+            pytest.fail(f"call {i} was taken")
+    with torch.no_grad():
+        for call in calls:
+            call()
+    _no_error()

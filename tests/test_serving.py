@@ -236,3 +236,25 @@ def test_the_engines_rules_take_no_outputs():
             DecodeEngine.adjust(object(), **{name: None})
     rules = set(inspect.signature(S.rules_of).parameters) - {"logits", "out", "token", "shape", "device"}
     assert set(inspect.signature(DecodeEngine.adjust).parameters) == rules | {"self"}
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    from types import SimpleNamespace
+
+    import torch
+
+    from opentars_b200 import serving as S
+    cpu = torch.device("cpu")
+    cache = SimpleNamespace(head_dim=64, n_kv=2, device=cpu, dtype=torch.bfloat16)
+    plain = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16, requires_grad=True)
+    S._attend_args(cache, plain, None, 0, 0)
+    S._attend_args(cache, q.detach(), None, 0, 0)
+    for args in ((q, None), (plain, q), (2 * q, None)):
+        with pytest.raises(ValueError, match="gradient"):
+            S._attend_args(cache, *args, 0, 0)
+    for k, v in ((q, plain), (plain, q)):
+        with pytest.raises(ValueError, match="gradient"):
+            S.append(cache, k[:, :2], v[:, 2:], torch.zeros(2))
+    with torch.no_grad():
+        S._attend_args(cache, q, None, 0, 0)
