@@ -16,9 +16,8 @@ namespace {
 
 // ----------------------------------------------------------------------------------- append
 // One thread rounds 8 consecutive elements of a key row and of its value row: 16-byte stores, a
-// row's threads side by side. Bound by memory (each source element read once, each cache element
-// written once): four prompts of up to 2048 rows of 256, 3.6 us (2.9 TB/s); a step's 64 rows are bound by
-// the launch (3.4 us).
+// row's threads side by side. Bound by the launch and one trip to memory and back: a step's 64 rows and four
+// prompts of up to 2048 rows of 256 (10.5 MB, 1.6 us at the copy rate) both take 3.4 us.
 constexpr int kAppendThreads = 256;
 
 template <class S>
@@ -101,7 +100,7 @@ cudaError_t append_to(const AppendArgs& a, cudaStream_t st) {
 // A few rows are moved at once (a cache one slot over its budget moves one); more of them in a second
 // kernel over the lists. Bound by the chain of block-wide steps (some 0.5 us each with 1024 threads): 16 x 8
 // heads one slot over a budget of 1024, 10 us with the second launch; the rows' move by memory: six sequences
-// of up to 8192 slots cut to 2048, 13 us of ranking and 13 us of moving 75 MB.
+// of up to 8192 slots cut to 2048, 27 us: 13 us of ranking on 32 CTAs, then as long for moving 75 MB.
 constexpr int kRankThreads = 1024, kRankWarps = kRankThreads / 32, kBins = 2048, kKeysMax = 49152, kFewMoves = 32;
 
 __device__ __forceinline__ uint32_t rank_key(float w, int pos, int sinks, int64_t recent_from) {
@@ -312,9 +311,11 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(EvictArgs a, Moves mv) {
 // (divisions and bias reads inside the stream made it three times as long). Each thread keeps its
 // best group of four; the candidates are combined over the cluster and the winning group is read once
 // more for the token. Words of 16 bits for histories below 2^14 ids: 32768 tokens in 64 KB.
-// Bound by memory, 8 bytes a token and the mask: 64 rows of 262144 with histories of up to 4000 ids, 40 us
-// (3.4 TB/s; the words' filling is the rest); one row of 151936, 9.5 us (a chain of latencies). Tried and not
-// kept: a prefetch of the share to L2 (48 us), eight groups in flight (109 us, with the penalties in the stream).
+// 64 rows of 262144 with histories of up to 4000 ids take 39 us, 21 us at the copy rate (8 bytes a token and the
+// mask): bound by the filling, seven or eight steps behind a barrier each before a slice streams, and twice
+// where a share is two slices as here (DRAM at 26 %, barriers the first stall). One row of 151936: 9.3 us (a
+// chain of latencies). Tried and not kept: a prefetch of the share to L2 (48 us), eight groups in flight (109
+// us, with the penalties in the stream).
 template <class Word>
 struct Bits {
   static constexpr uint32_t kListed = 1u << (8 * sizeof(Word) - 1), kPrompt = kListed >> 1, kCount = kPrompt - 1;
