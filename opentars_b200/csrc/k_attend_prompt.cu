@@ -121,11 +121,11 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 // 2^x of two values <= 16 on the FMA units: x = n + f with n the nearest integer (1.5 x 2^23 + 127 is added, so that
 // n + 127, the exponent field of 2^n, stands in the sum's low bits) and f in [-1/2, 1/2]; 2^f by a polynomial fitted
-// to least relative error (2.6e-6), times 2^n. Below 2^-126 the result is 2^-126. A NaN stays one (its bits make a
-// factor of -infinity, and NaN x -infinity is NaN).
+// to least relative error (2.6e-6), times 2^n. From 2^-126.5 down the field is 0 and so is the result. A NaN stays
+// one (its low bits make a factor of 0 or -infinity).
 __device__ __forceinline__ uint64_t ex2_fma(uint64_t x2) {
   const float2 x = halves(x2);
-  x2 = pair(__float_as_uint(max_nan(x.x, -126.0f)), __float_as_uint(max_nan(x.y, -126.0f)));
+  x2 = pair(__float_as_uint(max_nan(x.x, -127.0f)), __float_as_uint(max_nan(x.y, -127.0f)));
   const uint64_t t = add2(x2, pair(12583039.0f)), f = add2(x2, fma2(t, pair(-1.0f), pair(12583039.0f)));
   uint64_t p = fma2(f, pair(0.009570101276040077f), pair(0.05591785907745361f));
   p = fma2(p, f, pair(0.240247443318367f));
@@ -594,8 +594,7 @@ __global__ void __launch_bounds__(PromptShape<HD>::kThreads, 1)
   tc_fence_after();
   if (!s_dead) {
     const bool any = p >= 0;
-    // a row whose scores are all -infinity is 0 / 0; its sum is not 0, because ex2_fma ends at 2^-126
-    const float inv = !any ? 0.0f : m == neg_inf() ? __int_as_float(0x7FC00000) : 1.0f / l;
+    const float inv = any ? 1.0f / l : 0.0f;       // (scores of -infinity alone: 0 / 0)
     const bool sure = m == neg_inf() || (l != l && scale2 != 0.0f);
     float most = 0.0f;                             // NaN once an output is
     // the warp's rows go out through the query tile's place (no tensor core reads it any more), so

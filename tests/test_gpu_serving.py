@@ -1157,3 +1157,29 @@ def test_tensors_that_require_a_gradient_are_refused():
         for call in calls:
             call()
     _no_error()
+
+
+@pytest.mark.parametrize("dtype,hd,page", [(torch.bfloat16, 128, 64), (torch.bfloat16, 64, 16), (torch.float16, 256, 64)])
+@pytest.mark.parametrize("op,n", [("attend", 1), ("chunk", 3), ("tiles", 300)])
+@pytest.mark.parametrize("places", [(0, 3), (6, 7)])
+def test_a_score_of_minus_infinity_against_an_infinite_value(op, n, dtype, hd, page, places):
+    """Visible slots whose score is -infinity (probability 0) and whose value is infinite: 0 x infinity is NaN in
+    their columns, wherever in a block of slots they lie; the other columns are as without them."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(41)
+    L = 420
+    k, v, table = _pools([L], 1, hd, page, dtype, g)
+    slots = [s for s in range(16, 16 + 64) if s % 8 in places]  # visible to every row, in a block that is not masked
+    for i, s in enumerate(slots):
+        k[int(table[0, s // page]), s % page, 0, 0] = -math.inf
+        v[int(table[0, s // page]), s % page, 0, i] = math.inf
+    q = torch.randn(n, 2, hd, generator=g).to(dtype)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.25
+    room = torch.full((1, 700 if op == "chunk" else 0), -1, dtype=torch.int32)
+    cache = _cache(k, v, torch.cat([table, room], 1), [L])
+    cu = torch.tensor([0, n], dtype=torch.int32)
+    ref = R.attend_prompt(k, v, table, [L], q, cu, 0.1, 0, 0, page)
+    out = S.attend(cache, q.cuda(), 0.1) if op == "attend" else S.attend_prompt(cache, q.cuda(), cu.cuda(), 0.1)
+    _no_error()
+    assert torch.isnan(ref[:, :, :len(slots)]).all() and torch.isfinite(ref[:, :, len(slots):]).all()
+    _close(out, ref, _tolerance(ref, q, k, v, 0.1, dtype))
