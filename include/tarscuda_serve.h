@@ -33,8 +33,9 @@ extern "C" {
  * table[b * table_stride + s / page_size] of both pools; key-value head h of a row is `head_dim`
  * contiguous elements at page * page_stride + row * slot_stride + h * head_stride (elements; bases
  * and strides 16-byte aligned, the three dimensions nested in any order so that no two rows share
- * memory; the stride of a dimension of one entry is not used). length[b] slots are in use. Entries of the page list behind the
- * used slots, and rows of a page behind them, may hold anything: they never reach a result. */
+ * memory; the stride of a dimension of one entry is not used). length[b] slots are in use. Entries
+ * of the page list behind the used slots, and rows of a page behind them, may hold anything: they
+ * never reach a result. */
 typedef struct {
   void* k;
   void* v;
@@ -69,12 +70,12 @@ int tc_kv_append(const tc_kv_cache* c, const void* k, const void* v, int32_t src
  * p = softmax over the visible slots j of scale * q[b][h] . k_j; head h reads key-value head
  * h / (n_heads / n_kv). Slot j of length[b] = L is visible if j >= L - window or j < sinks (window 0:
  * all). A sequence of length 0 gets zeros. q and out have the cache's type, rows [batch][n_heads]
- * [head_dim] with strides in elements, 16-byte aligned, and share no memory. With weight_out (laid out as the cache's
- * weight, which may be it) weight_out[b][g][j] = weight[b][g][j] + the p_j of the heads of
- * key-value head g, for j < L; slots behind are left alone.
- * ws: tc_attend_workspace bytes, 256-byte aligned; with weights they hold a score for every sequence, head and
- * slot that the page lists have room for (batch * n_heads * max_pages * page_size * 4 bytes), whatever the
- * lengths. */
+ * [head_dim] with strides in elements, 16-byte aligned, and share no memory. With weight_out (laid
+ * out as the cache's weight, which may be it, but no shifted part of it) weight_out[b][g][j] =
+ * weight[b][g][j] + the p_j of the heads of key-value head g, for j < L; slots behind are left alone.
+ * ws: tc_attend_workspace bytes, 256-byte aligned; with weights they hold a score for every sequence,
+ * head and slot that the page lists have room for (batch * n_heads * max_pages * page_size * 4
+ * bytes), whatever the lengths. */
 int tc_attend(const tc_kv_cache* c, const void* q, int64_t q_row_stride, int64_t q_head_stride, void* out,
               int64_t out_row_stride, int64_t out_head_stride, int32_t n_heads, float scale, int32_t window,
               int32_t sinks, float* weight_out, void* ws, uint64_t ws_bytes, void* stream);

@@ -225,8 +225,9 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (
 // The factor a state kept at maximum m takes at maximum m2 >= m (1 where both are still -infinity).
 __device__ __forceinline__ float shrink(float m, float m2) { return m2 == neg_inf() ? 1.0f : ex2(m - m2); }
 
-// Probabilities and sums are kept 2^kLift times as large: fp16 ends at 2^-25, and slots of less than that share of a
-// warp's maximum, tens of thousands of them, would count in the sum but not in the output. From 2^14 two parts reach 2^-39.
+// Probabilities and sums are kept 2^kLift times as large: fp16 ends at 2^-25, and slots of less than that share
+// of a warp's maximum, tens of thousands of them, would count in the sum but not in the output. From 2^14 on two
+// parts reach 2^-39.
 template <class T>
 constexpr float kLift = __is_same(T, __half) ? 14.0f : 0.0f;
 

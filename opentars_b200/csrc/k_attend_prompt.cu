@@ -19,7 +19,7 @@
 //              running maximum is only moved (and O rescaled) when it grows by more than 2^8, and
 //              P is rounded once to the cache's type, whose range holds that: the output's error against
 //              64 bits is 1.29 (bf16) and 1.40 (fp16) times that of the output's own rounding alone. A second
-//              part, as attend keeps, would make 3072 cycles of the 2048 that the MMAs of a pair of tiles
+//              part, as attend keeps, would add half to the 2048 cycles that the MMAs of a pair of tiles
 //              take (below). The row's sum is of the unrounded fp32 values
 // Three prompts of up to 8192 tokens, 16 heads on 8 of 128, bf16: 365 us (1005 TFLOP/s; 430 us in long runs under
 // the power limit). A pair of tiles takes 3400 cycles for 128 slots, of which its MMAs are 2048: the rest is the

@@ -22,13 +22,15 @@ bool stride_ok(int64_t s, int bytes) { return s >= 0 && s < kMaxStride && s * by
 // Whether two sets of rows, rows x heads runs of `width` elements with strides of their own, may share an element.
 // Exact for two of the same nested strides (interleaved parts of one buffer are apart); with different strides they
 // may as soon as their ranges meet. `ahead`: how many elements the second set starts behind the first.
-bool may_share(int64_t ahead, int64_t ra, int64_t ha, int64_t rb, int64_t hb, int64_t rows, int64_t heads, int64_t width) {
+bool may_share(int64_t ahead, int64_t ra, int64_t ha, int64_t rb, int64_t hb, int64_t rows, int64_t heads,
+               int64_t width) {
   if (rows == 1) ra = rb = 0;                    // a dimension of one entry is never stepped over
   if (heads == 1) ha = hb = 0;
   const auto reach = [&](int64_t r, int64_t h) { return (double)(rows - 1) * r + (double)(heads - 1) * h + width; };
   if ((double)ahead >= reach(ra, ha) || -(double)ahead >= reach(rb, hb)) return false;
   if (ra != rb || ha != hb) return true;
-  const int64_t big = std::max(ra, ha), small = std::min(ra, ha), nb = ra >= ha ? rows : heads, ns = ra >= ha ? heads : rows;
+  const int64_t big = std::max(ra, ha), small = std::min(ra, ha);
+  const int64_t nb = ra >= ha ? rows : heads, ns = ra >= ha ? heads : rows;
   if ((nb > 1 && (double)(ns - 1) * small + width > (double)big) || (ns > 1 && small < width)) return true;
   const int64_t d = std::abs(ahead), i0 = big ? d / big : 0;
   for (int64_t i = i0; i <= i0 + (big > 0); ++i) {

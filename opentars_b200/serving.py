@@ -401,11 +401,11 @@ def rules_of(logits: torch.Tensor | None, out: torch.Tensor | None = None, histo
 
 def adjust_logits(logits: torch.Tensor, token: torch.Tensor | None = None, none: int = -1, **rules) -> torch.Tensor:
     """Penalties, biases and a grammar mask on fp32 logits [rows, vocab], and the greedy pick: the picks
-    [rows] int32 (`token`, or a new tensor). Keywords, each optional: out (None: in place; no shifted part of logits), history
-    [rows, ids] int32 with n_history and n_prompt [rows] (prompt ids first), repetition / presence /
-    frequency [rows] fp32, bias_ids / bias [rows, entries] (the last entry of a token counts), mask
-    int32 words, bit t % 32 of word t // 32 set where token t is allowed. A row whose mask allows
-    nothing picks `none`."""
+    [rows] int32 (`token`, or a new tensor). Keywords, each optional: out (None: in place; not a shifted
+    part of logits), history [rows, ids] int32 with n_history and n_prompt [rows] (prompt ids first),
+    repetition / presence / frequency [rows] fp32, bias_ids / bias [rows, entries] (the last entry of a
+    token counts), mask int32 words, bit t % 32 of word t // 32 set where token t is allowed. A row
+    whose mask allows nothing picks `none`."""
     if token is None:
         token = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
     r = rules_of(logits, token=token, none=none, **rules)

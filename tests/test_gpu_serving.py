@@ -1183,3 +1183,34 @@ def test_a_score_of_minus_infinity_against_an_infinite_value(op, n, dtype, hd, p
     _no_error()
     assert torch.isnan(ref[:, :, :len(slots)]).all() and torch.isfinite(ref[:, :, len(slots):]).all()
     _close(out, ref, _tolerance(ref, q, k, v, 0.1, dtype))
+
+
+@pytest.mark.parametrize("batch", [1, 3])
+def test_a_handle_over_the_front_of_the_page_lists(batch):
+    """A handle over table[:, :n] of wide page lists does what one over the whole lists does."""
+    from opentars_b200 import serving as S
+    g = torch.Generator().manual_seed(51)
+    lens = [70, 33, 0][:batch]
+    k, v, table = _pools([n + 9 for n in lens], 2, 64, 16, torch.float16, g)
+    wide = torch.cat([table, torch.full((batch, 500), 10 ** 9, dtype=torch.int32)], 1).cuda()
+    k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+    new, q = torch.randn(2 * batch, 2, 64, generator=g).cuda(), torch.randn(2 * batch, 4, 64, generator=g).half().cuda()
+    cu = (torch.arange(batch + 1) * 2).int().cuda()
+    got = []
+    for width in (wide.shape[1], 5):
+        w = torch.rand(batch, 2, wide.shape[1] * 16, generator=torch.Generator().manual_seed(1)).cuda()
+        pos = torch.arange(wide.shape[1] * 16, dtype=torch.int32).repeat(batch, 2, 1).cuda()
+        c = S.PagedCache(_cuda_pool(k, "heads"), _cuda_pool(v, "heads"), wide[:, :width], torch.tensor(lens).int().cuda(), weight=w,
+                         pos=pos, seen=torch.tensor(lens).int().cuda())
+        c.length.add_(2)
+        c.seen.add_(2)
+        S.append(c, new, -new, cu)
+        a = S.attend_prompt(c, q, cu, 0.125)
+        b = S.attend(c, q[:batch], 0.125, weight_out=c.weight)
+        S.evict(c, 40, 2, 8)
+        got.append([a, b, c.k.contiguous(), c.v.contiguous(), w, pos, c.length])
+    _no_error()
+    close = _tolerance(got[0][0].double().cpu(), q.cpu(), k, v, 0.125, torch.float16)
+    _close(got[1][0], got[0][0].double().cpu(), 2 * close)      # (the room may take the chunk to another kernel)
+    for x, y in zip(got[0][1:], got[1][1:]):
+        assert torch.equal(x, y)
